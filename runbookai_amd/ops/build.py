@@ -23,7 +23,17 @@ SOURCES = [
     os.path.join(CSRC, "skinny_gemm.hip"),
     os.path.join(CSRC, "decode_gemv.hip"),
     os.path.join(CSRC, "retrieval_sampling.hip"),
+    os.path.join(CSRC, "training.cpp"),
+    os.path.join(CSRC, "packed_attn.hip"),
+    os.path.join(CSRC, "cross_entropy.hip"),
+    os.path.join(CSRC, "grad_norm.hip"),
 ]
+
+# hipcc would otherwise form packed fp32 instructions from ordinary float code,
+# some of which have given wrong results on this hardware. (The host pass does
+# not know the feature and says so.)
+HIP_FLAGS = ["-O3", "-std=c++17",
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def build(verbose: bool = False):
@@ -37,7 +47,7 @@ def build(verbose: bool = False):
         sources=SOURCES,
         build_directory=BUILD_DIR,
         extra_cflags=["-O3"],
-        extra_cuda_cflags=["-O3", "-std=c++17"],
+        extra_cuda_cflags=HIP_FLAGS,
         verbose=verbose,
         with_cuda=True,  # ROCm build: drives hipcc for the .hip sources
     )

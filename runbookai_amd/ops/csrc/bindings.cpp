@@ -7,6 +7,8 @@
 
 #include <mutex>
 
+void bind_training(pybind11::module_& m);   // training.cpp
+
 extern "C" {
 void launch_rmsnorm(const void*, const void*, void*, int, int, float, void*);
 void launch_rmsnorm_residual(const void*, const void*, void*, const void*, void*,
@@ -454,4 +456,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("masked_argmax", &masked_argmax, "greedy sampling under validity mask");
     m.def("masked_topp", &masked_topp,
           "fused temperature softmax + nucleus sampling under validity mask");
+    bind_training(m);
 }

@@ -1,0 +1,305 @@
+// Cross-entropy of next tokens and its gradient (gfx950).
+//
+//   loss_i = log sum_j exp(x_ij) - x_it      rows with a label t
+//   dx_ij  = (exp(x_ij - m_i) / l_i - [j = t]) g_i
+// with m_i the row's maximum and l_i = sum_j exp(x_ij - m_i).
+//
+// Both kernels are bound by memory.  The forward one reads a labelled row once
+// (running maximum and sum in each thread, joined at the end) and keeps m and l
+// for the backward one, which reads the row again and writes the gradient; a
+// row without a label is not read, and its gradient is written as zeros.  The
+// gradient is not made in the forward pass: the factor g that comes back
+// (a loss scale, say) has to be in it before it is rounded to 16 bits, where a
+// mean's 1/n alone would push small values below fp16's range.
+//
+// m and l are kept apart, not as one log-sum: x - m is nearly exact, while a
+// log-sum near 12 is rounded by 5e-7, which would be in every gradient.
+#include "common.h"
+
+namespace {
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+    static constexpr int VEC = 4;
+    static DEVINL float get(float v) { return v; }
+    static DEVINL float put(float v) { return v; }
+};
+template <> struct Elem<__bf16> {
+    static constexpr int VEC = 8;
+    static DEVINL float get(__bf16 v) { return (float)v; }
+    static DEVINL __bf16 put(float v) { return (__bf16)v; }
+};
+template <> struct Elem<_Float16> {
+    static constexpr int VEC = 8;
+    static DEVINL float get(_Float16 v) { return (float)v; }
+    static DEVINL _Float16 put(float v) { return (_Float16)v; }
+};
+template <typename T>
+using Vec = T __attribute__((ext_vector_type(Elem<T>::VEC)));
+
+constexpr float L2E = 1.4426950408889634f;
+constexpr float L2E_LO = 1.9259629911266175e-8f;   // log2(e) - L2E
+constexpr float LN2 = 0.6931471805599453f;
+
+// exp(t), t <= 0.  For 32-bit results the product t log2(e) is carried in two
+// parts: rounded to one, it alone is off by 6e-8 |t|.
+template <typename T>
+DEVINL float exp_neg(float t) {
+    const float a = t * L2E;
+    const float e = __builtin_amdgcn_exp2f(a);
+    if (sizeof(T) < 4 || a < -126.f) return e;
+    const float rest = fmaf(t, L2E, -a) + t * L2E_LO;
+    return fmaf(e, rest * LN2, e);
+}
+
+// (m, l) of two parts of a row; a part without a finite value has m = -inf
+DEVINL void join(float& m, float& l, float m2, float l2) {
+    const float to = fmaxf(m, m2);
+    const float base = to == -INFINITY ? 0.f : to;
+    l = l * __builtin_amdgcn_exp2f((m - base) * L2E) +
+        l2 * __builtin_amdgcn_exp2f((m2 - base) * L2E);
+    m = to;
+}
+
+// Elements before the row's first 16-byte boundary
+template <typename T>
+DEVINL int head_of(const T* row, int V) {
+    const int h = (int)((16 - (reinterpret_cast<unsigned long>(row) & 15)) & 15) / (int)sizeof(T);
+    return min(h, V);
+}
+
+}  // namespace
+
+// WAVES waves a row, 4 waves a workgroup at least.  A wave a row needs no
+// barrier and keeps its whole row in flight up to V = 4096; long rows take 16.
+template <typename T, int WAVES>
+__global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
+xent_fwd_kernel(const T* __restrict__ x, long stride, const long* __restrict__ targets,
+                long ignore, int N, int V, float* __restrict__ loss,
+                float2_t* __restrict__ stats) {
+    constexpr int VEC = Elem<T>::VEC, LANES = WAVES * 64;
+    constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1;
+    constexpr int U = 4;
+    const int row = blockIdx.x * ROWS + (ROWS > 1 ? (int)threadIdx.x / LANES : 0);
+    if (ROWS > 1 && row >= N) return;   // a whole wave; there is no barrier then
+    const int tid = threadIdx.x % LANES;
+    const long t = targets[row];
+    if (t == ignore) {
+        if (tid == 0) loss[row] = 0.f;
+        return;
+    }
+    const T* r = x + row * stride;
+    float m = -INFINITY, l = 0.f;
+    auto one = [&](float v) {
+        if (v > m) {
+            l *= __builtin_amdgcn_exp2f((m - v) * L2E);
+            m = v;
+        }
+        l += __builtin_amdgcn_exp2f((v - (m == -INFINITY ? 0.f : m)) * L2E);
+    };
+    const int head = head_of(r, V);
+    const int vecs = (V - head) / VEC;
+    const Vec<T>* body = reinterpret_cast<const Vec<T>*>(r + head);
+    for (int i0 = tid; i0 < vecs; i0 += U * LANES) {
+        Vec<T> v[U];
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * LANES;
+            if (i < vecs) v[u] = body[i];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * LANES < vecs)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) top = fmaxf(top, Elem<T>::get(v[u][j]));
+        if (top > m) {
+            l *= __builtin_amdgcn_exp2f((m - top) * L2E);
+            m = top;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * LANES < vecs)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    l += __builtin_amdgcn_exp2f((Elem<T>::get(v[u][j]) - base) * L2E);
+    }
+    // the rest: fewer than VEC elements at each end
+    const int tail = head + vecs * VEC;
+    if (tid < head) one(Elem<T>::get(r[tid]));
+    if (tail + tid < V) one(Elem<T>::get(r[tail + tid]));
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const float m2 = __shfl_xor(m, off, WAVE), l2 = __shfl_xor(l, off, WAVE);
+        join(m, l, m2, l2);
+    }
+    if (WAVES > 1) {
+        __shared__ float ms[WAVES], lsum[WAVES];
+        if ((tid & 63) == 0) { ms[tid >> 6] = m; lsum[tid >> 6] = l; }
+        __syncthreads();
+        m = ms[0];
+        l = lsum[0];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) join(m, l, ms[w], lsum[w]);
+    }
+    if (tid == 0) {
+        // a label that is no place of the row: no value, and no read
+        const bool in = t >= 0 && t < V;
+        loss[row] = in ? __logf(l) + (m - Elem<T>::get(r[in ? t : 0])) : NAN;
+        if (stats) stats[row] = float2_t{m, in ? 1.f / l : NAN};
+    }
+}
+
+// Sum of the rows' losses, or their mean over the labels (NaN where there is
+// none), and the factor 1, or 1 / number of labels.
+__global__ void __launch_bounds__(1024)
+xent_reduce_kernel(const float* __restrict__ loss, const long* __restrict__ targets,
+                   long ignore, int N, int mean, float* __restrict__ result,
+                   float* __restrict__ factor) {
+    double s = 0.0;
+    int n = 0;
+    for (int i = threadIdx.x; i < N; i += 1024) {
+        s += loss[i];
+        n += targets[i] != ignore;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        s += __shfl_xor(s, off, WAVE);
+        n += __shfl_xor(n, off, WAVE);
+    }
+    __shared__ double ss[16];
+    __shared__ int ns[16];
+    if ((threadIdx.x & 63) == 0) { ss[threadIdx.x >> 6] = s; ns[threadIdx.x >> 6] = n; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) { s += ss[w]; n += ns[w]; }
+        *result = (float)(mean ? s / (double)n : s);
+        *factor = mean ? (float)(1.0 / (double)n) : 1.f;
+    }
+}
+
+// `gout`: one value, or one a row (gstride 1).  `factor`: the 1/n of a mean.
+// x and dx have the same distance to 16-byte boundaries in every row.
+template <typename T, int WAVES>
+__global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
+xent_bwd_kernel(const T* __restrict__ x, long stride, const long* __restrict__ targets,
+                long ignore, int N, int V, const float2_t* __restrict__ stats,
+                const float* __restrict__ gout, long gstride,
+                const float* __restrict__ factor, T* __restrict__ dx, long dstride) {
+    constexpr int VEC = Elem<T>::VEC, LANES = WAVES * 64;
+    constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1;
+    constexpr int U = 4;
+    const int row = blockIdx.x * ROWS + (ROWS > 1 ? (int)threadIdx.x / LANES : 0);
+    if (row >= N) return;
+    const int tid = threadIdx.x % LANES;
+    const long t = targets[row];
+    const T* r = x + row * stride;
+    T* d = dx + row * dstride;
+    const int head = head_of(d, V);
+    const int vecs = (V - head) / VEC;
+    const int tail = head + vecs * VEC;
+    Vec<T>* out = reinterpret_cast<Vec<T>*>(d + head);
+    if (t == ignore) {
+        for (int i = tid; i < vecs; i += LANES) out[i] = Vec<T>{};
+        if (tid < head) d[tid] = T{};
+        if (tail + tid < V) d[tail + tid] = T{};
+        return;
+    }
+    const float2_t st = stats[row];
+    const float g = gout[row * gstride] * (factor ? *factor : 1.f);
+    const float m = st[0] == -INFINITY ? 0.f : st[0], inv = st[1];
+    auto one = [&](int j, float v) {
+        return Elem<T>::put((exp_neg<T>(v - m) * inv - (j == t ? 1.f : 0.f)) * g);
+    };
+    const Vec<T>* body = reinterpret_cast<const Vec<T>*>(r + head);
+    for (int i0 = tid; i0 < vecs; i0 += U * LANES) {
+        Vec<T> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * LANES;
+            if (i < vecs) v[u] = body[i];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * LANES;
+            if (i < vecs) {
+                Vec<T> w;
+                const int j0 = head + i * VEC;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) w[j] = one(j0 + j, Elem<T>::get(v[u][j]));
+                out[i] = w;
+            }
+        }
+    }
+    if (tid < head) d[tid] = one(tid, Elem<T>::get(r[tid]));
+    if (tail + tid < V) d[tail + tid] = one(tail + tid, Elem<T>::get(r[tail + tid]));
+}
+
+// ---------------------------------------------------------------- launchers
+// Each returns the launch's hipError_t.  kind: 0 fp32, 1 bf16, 2 fp16.
+
+namespace {
+
+template <typename T, int WAVES>
+void fwd(const void* x, long stride, const void* targets, long ignore, int N, int V,
+         void* loss, void* stats, hipStream_t st) {
+    constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1;
+    hipLaunchKernelGGL((xent_fwd_kernel<T, WAVES>), dim3((N + ROWS - 1) / ROWS),
+                       dim3(ROWS * WAVES * 64), 0, st, (const T*)x, stride,
+                       (const long*)targets, ignore, N, V, (float*)loss, (float2_t*)stats);
+}
+
+template <typename T, int WAVES>
+void bwd(const void* x, long stride, const void* targets, long ignore, int N, int V,
+         const void* stats, const void* gout, long gstride, const void* factor, void* dx,
+         long dstride, hipStream_t st) {
+    constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1;
+    hipLaunchKernelGGL((xent_bwd_kernel<T, WAVES>), dim3((N + ROWS - 1) / ROWS),
+                       dim3(ROWS * WAVES * 64), 0, st, (const T*)x, stride,
+                       (const long*)targets, ignore, N, V, (const float2_t*)stats,
+                       (const float*)gout, gstride, (const float*)factor, (T*)dx, dstride);
+}
+
+}  // namespace
+
+extern "C" int launch_xent_fwd(int kind, const void* x, long stride, const void* targets,
+                               long ignore, int N, int V, void* loss, void* stats,
+                               void* stream) {
+    const hipStream_t st = (hipStream_t)stream;
+#define FWD(T)                                                                    \
+    if (V <= 8192) fwd<T, 1>(x, stride, targets, ignore, N, V, loss, stats, st);  \
+    else fwd<T, 16>(x, stride, targets, ignore, N, V, loss, stats, st)
+    if (kind == 0) { FWD(float); }
+    else if (kind == 1) { FWD(__bf16); }
+    else { FWD(_Float16); }
+#undef FWD
+    return (int)hipGetLastError();
+}
+
+extern "C" int launch_xent_reduce(const void* loss, const void* targets, long ignore, int N,
+                                  int mean, void* result, void* factor, void* stream) {
+    hipLaunchKernelGGL(xent_reduce_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream,
+                       (const float*)loss, (const long*)targets, ignore, N, mean,
+                       (float*)result, (float*)factor);
+    return (int)hipGetLastError();
+}
+
+extern "C" int launch_xent_bwd(int kind, const void* x, long stride, const void* targets,
+                               long ignore, int N, int V, const void* stats,
+                               const void* gout, long gstride, const void* factor, void* dx,
+                               long dstride, void* stream) {
+    const hipStream_t st = (hipStream_t)stream;
+#define BWD(T)                                                                          \
+    if (V <= 8192)                                                                      \
+        bwd<T, 1>(x, stride, targets, ignore, N, V, stats, gout, gstride, factor, dx,   \
+                  dstride, st);                                                         \
+    else                                                                                \
+        bwd<T, 16>(x, stride, targets, ignore, N, V, stats, gout, gstride, factor, dx,  \
+                   dstride, st)
+    if (kind == 0) { BWD(float); }
+    else if (kind == 1) { BWD(__bf16); }
+    else { BWD(_Float16); }
+#undef BWD
+    return (int)hipGetLastError();
+}

@@ -1,0 +1,782 @@
+// Causal attention of packed sequences with its gradients, for training
+// (gfx950): bf16, grouped heads, head dim 64 or 128.
+//
+// With s_ij = scale q_i.k_j over the places j <= i of i's own sequence:
+//   forward    P_ij = exp(s_ij) / l_i,  l_i = sum_j exp(s_ij),  o_i = sum_j P_ij v_j
+//   backward   dP_ij = do_i.v_j,  delta_i = sum_j P_ij dP_ij = do_i.o_i
+//              dS_ij = P_ij (dP_ij - delta_i)
+//              dq_i = scale sum_j dS_ij k_j,   dk_j = scale sum_i dS_ij q_i,
+//              dv_j = sum_i P_ij do_i          (dk, dv also over the group's heads)
+// P is recomputed from q, k and the row's log-sum in the backward pass.
+//
+// Every product is a v_mfma_f32_32x32x16_bf16.  Its fragments, for lane l with
+// c = l & 31, hi = l >> 5:
+//   A[32x16]: j=0..7 -> A[c][8 hi + j]      B[16x32]: j -> B[8 hi + j][c]
+//   C[32x32]: r=0..15 -> C[(r & 3) + 8 (r >> 2) + 4 hi][c]
+// The sum over k may run in any order that A and B share.  Taking
+//   k' = 16 s + 4 hi + (j & 3) + 8 (j >> 2)   for slice s, element j,
+// the C registers 8s..8s+7 of one product ARE the B fragment of slice s of the
+// next, in place: P and dS never leave their lane, neither through LDS nor
+// across lanes.  So each chain is laid out with the shared index on C's rows:
+//   forward  S^T = K Q^T -> O^T += V^T P^T
+//   dq       S^T = K Q^T, dP^T = V dO^T -> dQ^T += K^T dS^T
+//   dk, dv   S = Q K^T, dP = dO V^T -> dV^T += dO^T P, dK^T += Q^T dS
+// and the other operand (V^T, K^T, dO^T, Q^T) is read from its row-major LDS
+// tile by ds_read_b64_tr_b16: of a group of 16 lanes, lane i passes the
+// address of 4 elements of row i/4 and receives column i of the 4 rows.  With
+// the softmax statistics on the columns, each lane keeps its own row's.
+//
+// dq and (dk, dv) are two kernels that both recompute P: 7 products where one
+// pass would need 5, but no atomics, so the same inputs give the same bits.
+//
+// Precision: scores, statistics, delta and all sums are fp32; P and dS are
+// rounded to bf16 as operands of a product, which bf16 inputs ask for anyway.
+// delta_i = do_i.o_i is off by about 2^-9 |do| |o| from the roundings in o.
+// Where a row has n open places, |o| falls as 1/sqrt(n) and the error in dq as
+// 1/sqrt(n) of dq's own rounding: nothing, but for the first rows of a
+// sequence, where dP - delta cancels.  The first tile of each sequence
+// therefore takes delta_i = sum_j P_ij dP_ij in fp32, by a sweep of its own
+// over its (at most 128) keys.
+#include "common.h"
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef int int4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4_t lds_short4_t;
+
+#define ROWS 128        // rows of a tile, of queries or of keys
+#define LOG2E 1.4426950408889634f
+
+namespace {
+
+DEVINL f32x16_t mfma(bf16x8_t a, bf16x8_t b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+DEVINL f32x16_t zero16() {
+    f32x16_t z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.f;
+    return z;
+}
+
+// C-fragment row of register r
+DEVINL int crow(int r, int hi) { return (r & 3) + 8 * (r >> 2) + 4 * hi; }
+
+// Registers 8s..8s+7 of a C fragment, rounded, as the B fragment of slice s.
+DEVINL bf16x8_t pack8(const f32x16_t& c, int s) {
+    bf16x8_t b;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = (__bf16)c[8 * s + j];
+    return b;
+}
+
+// LDS tile of rows of D bf16, in 16-byte chunks, chunk c of row r at c ^ f(r).
+// f spreads both kinds of reads over all 64 banks: 16 lanes with the same
+// chunk of 16 rows (16 bytes each), and 32 lanes with 64 bytes of 4 rows each
+// (8 bytes each).
+template <int D>
+DEVINL unsigned tile_at(unsigned row, unsigned chunk) {
+    const unsigned f = D == 128 ? ((row & 3u) << 2) | ((row >> 2) & 3u)
+                                : (((row >> 1) & 1u) << 2) | ((row >> 2) & 3u);
+    return row * (D * 2) + ((chunk ^ f) << 4);
+}
+
+// A fragment of rows row0..row0+31, columns 16 s..16 s+15
+template <int D>
+DEVINL bf16x8_t rows_frag(const char* tile, int row0, int s, int lane) {
+    return *reinterpret_cast<const bf16x8_t*>(
+        tile + tile_at<D>(row0 + (lane & 31), 2 * s + (lane >> 5)));
+}
+
+// A fragment of the tile's transpose: columns 32 db..32 db+31 as its rows, and
+// the rows row0 + k' (k' as above, slice 0) as its columns
+template <int D>
+DEVINL bf16x8_t cols_frag(char* tile, int row0, int db, int lane) {
+    const int i = lane & 15;
+    const unsigned row = row0 + 4 * (lane >> 5) + (i >> 2);
+    const unsigned chunk = 4 * db + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1);
+    const unsigned half = 8 * (i & 1);
+    union { short4_t h[2]; bf16x8_t v; } u;
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_short4_t*)(tile + tile_at<D>(row, chunk) + half));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_short4_t*)(tile + tile_at<D>(row + 8, chunk) + half));
+    return u.v;
+}
+
+// A 64-row tile on its way through registers; rows at or past `end` are zero.
+template <int D, int THREADS>
+struct Stage {
+    static constexpr int N = 64 * D / 8 / THREADS;
+    bf16x8_t x[N];
+    DEVINL void load(const ushort_t* base, long stride, int row0, int end) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int at = (int)threadIdx.x + i * THREADS;
+            const int row = row0 + at / (D / 8);
+            x[i] = bf16x8_t{};
+            if (row < end)
+                x[i] = *reinterpret_cast<const bf16x8_t*>(base + row * stride + (at % (D / 8)) * 8);
+        }
+    }
+    DEVINL void store(char* tile) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int at = (int)threadIdx.x + i * THREADS;
+            *reinterpret_cast<bf16x8_t*>(tile + tile_at<D>(at / (D / 8), at % (D / 8))) = x[i];
+        }
+    }
+};
+
+// One row's values as a B fragment set: B[k][c] = x[row of lane c][k]
+template <int D>
+DEVINL void load_row(bf16x8_t (&f)[D / 16], const ushort_t* row, bool real, int hi) {
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+        f[s] = bf16x8_t{};
+        if (real) f[s] = *reinterpret_cast<const bf16x8_t*>(row + s * 16 + hi * 8);
+    }
+}
+
+// Writes a transposed accumulator's column (the lane's row) times `factor`.
+template <int D>
+DEVINL void store_row(const f32x16_t (&acc)[D / 32], float factor, ushort_t* row, int hi) {
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            bf16x4_t x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = (__bf16)(acc[db][4 * g + j] * factor);
+            *reinterpret_cast<bf16x4_t*>(row + db * 32 + 8 * g + 4 * hi) = x;
+        }
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------- the tiles
+//
+// A tile is {first row, end row, start and end of its sequence}; rows outside
+// every sequence make tiles of an empty sequence, whose outputs are zero, and
+// if the starts are no starts at all (negative, falling, past the rows), all
+// rows make tiles with end -1, whose outputs are NaN: no start that a caller
+// passes leads a kernel out of its buffers.  `by_query` has the tiles with the
+// most keys first, `by_key` those with the most queries, so that the longest
+// run first and the short ones fill the gaps.  One workgroup: a pass that
+// counts tiles by their number in the sequence, a scan, a pass that places
+// them.  (The order within one count is free and changes no result.)
+#define BUCKETS 4096
+
+__global__ void __launch_bounds__(512)
+packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
+                    int4_t* __restrict__ by_query, int4_t* __restrict__ by_key,
+                    int* __restrict__ count) {
+    __shared__ int first[BUCKETS], fill_q[BUCKETS], fill_k[BUCKETS];
+    __shared__ int part[512], total, bad;
+    const int tid = threadIdx.x;
+    const int lane = tid & (WAVE - 1), wid = tid / WAVE;
+    int shift = 0;
+    while (((T / ROWS) >> shift) >= BUCKETS) ++shift;
+    const int used = ((T / ROWS) >> shift) + 1;
+    if (tid == 0) { total = 0; bad = 0; }
+    for (int i = tid; i < used; i += 512) first[i] = fill_q[i] = fill_k[i] = 0;
+    __syncthreads();
+    for (int b = tid; b <= B; b += 512) {
+        const int s = starts[b];
+        if (s < 0 || s > T || (b && s < starts[b - 1])) bad = 1;
+    }
+    __syncthreads();
+    const bool wrong = bad != 0;
+    // sequences -1 and B: the rows before the first and behind the last
+    const int lo = wrong ? B : -1;
+    auto range = [&](int b, int& s, int& e) {
+        s = wrong ? 0 : b < 0 ? 0 : starts[b];
+        e = wrong || b == B ? T : starts[b + 1];
+    };
+    for (int b = lo + wid; b <= B; b += 512 / WAVE) {
+        int s, e;
+        range(b, s, e);
+        const int n = (e - s + ROWS - 1) / ROWS;
+        for (int i = lane; i < n; i += WAVE) atomicAdd(&first[i >> shift], 1);
+    }
+    __syncthreads();
+    // first[k] = number of tiles in buckets above k
+    constexpr int PER = BUCKETS / 512;
+    int sum = 0;
+    for (int i = 0; i < PER; ++i) {
+        const int k = tid * PER + i;
+        if (k < used) sum += first[k];
+    }
+    part[tid] = sum;
+    __syncthreads();
+    for (int off = 1; off < 512; off <<= 1) {
+        const int v = tid + off < 512 ? part[tid + off] : 0;
+        __syncthreads();
+        part[tid] += v;
+        __syncthreads();
+    }
+    if (tid == 0) total = part[0];
+    int above = part[tid] - sum;
+    for (int i = PER - 1; i >= 0; --i) {
+        const int k = tid * PER + i;
+        if (k < used) {
+            const int n = first[k];
+            first[k] = above;
+            above += n;
+        }
+    }
+    __syncthreads();
+    for (int b = lo + wid; b <= B; b += 512 / WAVE) {
+        int s, e;
+        range(b, s, e);
+        const int n = (e - s + ROWS - 1) / ROWS;
+        const bool real = !wrong && b >= 0 && b < B;
+        for (int i = lane; i < n; i += WAVE) {
+            const int r0 = s + i * ROWS;
+            const int4_t t = {r0, min(r0 + ROWS, e), real ? s : r0, real ? e : wrong ? -1 : r0};
+            const int kq = i >> shift, kk = (n - 1 - i) >> shift;
+            const int at_q = first[kq] + atomicAdd(&fill_q[kq], 1);
+            const int at_k = first[kk] + atomicAdd(&fill_k[kk], 1);
+            if (at_q < max_tiles) by_query[at_q] = t;
+            if (at_k < max_tiles) by_key[at_k] = t;
+        }
+    }
+    if (tid == 0) *count = min(total, max_tiles);
+}
+
+// ------------------------------------------------------------------ forward
+//
+// A workgroup takes a tile of 128 rows and NH heads of one group, a wave 32 of
+// the rows for all NH heads, so that a key or value fragment read from LDS
+// feeds NH products.  64 keys at a time stand in LDS, the next 64 are on their
+// way in registers meanwhile.
+template <int D, int NH, bool SAVE>
+__global__ void __launch_bounds__(256, D == 128 && NH == 2 ? 1 : 2)
+packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
+                       const ushort_t* __restrict__ k, long kt, long kh,
+                       const ushort_t* __restrict__ v, long vt, long vh,
+                       const int4_t* __restrict__ tiles, const int* __restrict__ count,
+                       ushort_t* __restrict__ out, float* __restrict__ lse, int T, int Hq, int Hk, float scale) {
+    const int per_tile = Hq / NH;
+    const int t = blockIdx.x / per_tile;
+    if (t >= *count) return;
+    // the kv head runs fastest: workgroups go round the 8 XCDs in turn, so with
+    // 1, 2, 4 or 8n of them an XCD's L2 sees the same heads' keys every time
+    const int which = blockIdx.x % per_tile;
+    const int hk = which % Hk;
+    const int h0 = hk * (Hq / Hk) + which / Hk * NH;
+    const int4_t tile = tiles[t];
+    const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
+    const bool real = seq1 > seq0;
+    const int kv0 = seq0, kv1 = real ? row1 : seq0;
+    const int lane = threadIdx.x & (WAVE - 1), wid = threadIdx.x / WAVE;
+    const int hi = lane >> 5;
+    const int wrow = row0 + wid * 32;
+    const int row = wrow + (lane & 31);
+    const bool mine = row < row1;
+    const float c2 = scale * LOG2E;
+
+    __shared__ char k_lds[2][64 * D * 2], v_lds[2][64 * D * 2];
+
+    bf16x8_t qf[NH][D / 16];
+    f32x16_t acc[NH][D / 32];
+    float m[NH], l[NH];
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+        load_row<D>(qf[n], q + row * qt + (h0 + n) * qh, mine, hi);
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) acc[n][db] = zero16();
+        m[n] = -INFINITY;
+        l[n] = 0.f;
+    }
+    k += hk * kh;
+    v += hk * vh;
+    Stage<D, 256> sk, sv;
+    const int steps = (kv1 - kv0 + 63) / 64;
+    if (steps > 0) {
+        sk.load(k, kt, kv0, kv1);
+        sv.load(v, vt, kv0, kv1);
+        sk.store(k_lds[0]);
+        sv.store(v_lds[0]);
+        if (steps > 1) {
+            sk.load(k, kt, kv0 + 64, kv1);
+            sv.load(v, vt, kv0 + 64, kv1);
+        }
+    }
+    __syncthreads();
+    const int wave_end = min(wrow + 32, row1);   // keys this wave's rows reach
+    for (int it = 0; it < steps; ++it) {
+        char* kl = k_lds[it & 1];
+        char* vl = v_lds[it & 1];
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+            const int key0 = kv0 + it * 64 + sub * 32;
+            if (key0 >= wave_end) continue;
+            f32x16_t s[NH];
+#pragma unroll
+            for (int n = 0; n < NH; ++n) s[n] = zero16();
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                const bf16x8_t kf = rows_frag<D>(kl, sub * 32, d, lane);
+#pragma unroll
+                for (int n = 0; n < NH; ++n) s[n] = mfma(kf, qf[n][d], s[n]);
+            }
+            const bool inner = key0 + 31 <= wrow;   // every key open to every row
+            bf16x8_t pf[NH][2];
+#pragma unroll
+            for (int n = 0; n < NH; ++n) {
+                if (!inner) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (key0 + crow(r, hi) > row) s[n][r] = -INFINITY;
+                }
+                float top = s[n][0];
+#pragma unroll
+                for (int r = 1; r < 16; ++r) top = fmaxf(top, s[n][r]);
+                top = fmaxf(top, __shfl_xor(top, 32, WAVE));
+                // the sums follow the maximum only when a row's has grown by
+                // over 2^8: until then P stays below 2^8, which costs no bits
+                if (!__all(top * c2 <= m[n] + 8.f)) {
+                    const float to = fmaxf(m[n], top * c2);
+                    const float f = to == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - to);
+                    m[n] = to;
+                    l[n] *= f;
+#pragma unroll
+                    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[n][db][r] *= f;
+                }
+                const float base = m[n] == -INFINITY ? 0.f : m[n];
+                float sum = 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], c2, -base));
+                    sum += s[n][r];
+                }
+                l[n] += sum;
+                pf[n][0] = pack8(s[n], 0);
+                pf[n][1] = pack8(s[n], 1);
+            }
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int db = 0; db < D / 32; ++db) {
+                    const bf16x8_t vf = cols_frag<D>(vl, sub * 32 + ks * 16, db, lane);
+#pragma unroll
+                    for (int n = 0; n < NH; ++n) acc[n][db] = mfma(vf, pf[n][ks], acc[n][db]);
+                }
+        }
+        if (it + 1 < steps) {
+            // the other buffer was last read before the barrier of the step before
+            sk.store(k_lds[(it + 1) & 1]);
+            sv.store(v_lds[(it + 1) & 1]);
+            if (it + 2 < steps) {
+                sk.load(k, kt, kv0 + (it + 2) * 64, kv1);
+                sv.load(v, vt, kv0 + (it + 2) * 64, kv1);
+            }
+            __syncthreads();
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+        const float sum = l[n] + __shfl_xor(l[n], 32, WAVE);
+        if (!mine) continue;
+        const long at = ((long)row * Hq + h0 + n) * D;
+        const float f = seq1 < 0 ? NAN : real ? 1.f / sum : 0.f;
+        store_row<D>(acc[n], f, out + at, hi);
+        if (SAVE && hi == 0)
+            lse[(long)(h0 + n) * T + row] = m[n] + __builtin_amdgcn_logf(sum);
+    }
+}
+
+// ----------------------------------------------------------------------- dq
+//
+// The forward kernel's split.  Also writes delta for the kernel below.
+template <int D, int NH>
+__global__ void __launch_bounds__(256, D == 128 && NH == 2 ? 1 : 2)
+packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
+                      const ushort_t* __restrict__ k, long kt, long kh,
+                      const ushort_t* __restrict__ v, long vt, long vh,
+                      const ushort_t* __restrict__ dout, long ot, long oh,
+                      const ushort_t* __restrict__ out, const int4_t* __restrict__ tiles, const int* __restrict__ count,
+                      const float* __restrict__ lse, float* __restrict__ delta,
+                      ushort_t* __restrict__ dq, int T, int Hq, int Hk, float scale) {
+    const int per_tile = Hq / NH;
+    const int t = blockIdx.x / per_tile;
+    if (t >= *count) return;
+    const int which = blockIdx.x % per_tile;
+    const int hk = which % Hk;
+    const int h0 = hk * (Hq / Hk) + which / Hk * NH;
+    const int4_t tile = tiles[t];
+    const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
+    const bool real = seq1 > seq0;
+    const int kv0 = seq0, kv1 = real ? row1 : seq0;
+    const int lane = threadIdx.x & (WAVE - 1), wid = threadIdx.x / WAVE;
+    const int hi = lane >> 5;
+    const int wrow = row0 + wid * 32;
+    const int row = wrow + (lane & 31);
+    const bool mine = row < row1;
+    const float c2 = scale * LOG2E;
+
+    __shared__ char k_lds[2][64 * D * 2], v_lds[2][64 * D * 2];
+
+    bf16x8_t qf[NH][D / 16], of[NH][D / 16];
+    f32x16_t acc[NH][D / 32];
+    float ls[NH], dl[NH];
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+        load_row<D>(qf[n], q + row * qt + (h0 + n) * qh, mine, hi);
+        load_row<D>(of[n], dout + row * ot + (h0 + n) * oh, mine, hi);
+        const long at = ((long)row * Hq + h0 + n) * D;
+        float sum = 0.f;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+            if (!mine) continue;
+            const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(out + at + s * 16 + hi * 8);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum = fmaf((float)of[n][s][j], (float)a[j], sum);
+        }
+        dl[n] = sum + __shfl_xor(sum, 32, WAVE);
+        ls[n] = mine ? lse[(long)(h0 + n) * T + row] : 0.f;
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) acc[n][db] = zero16();
+    }
+    k += hk * kh;
+    v += hk * vh;
+    Stage<D, 256> sk, sv;
+    const int steps = (kv1 - kv0 + 63) / 64;
+    const int wave_end = min(wrow + 32, row1);
+    // One pass over the keys.  Of s and dP, `use` makes what the pass is for.
+    auto sweep = [&](auto use) {
+        if (steps > 0) {
+            sk.load(k, kt, kv0, kv1);
+            sv.load(v, vt, kv0, kv1);
+            sk.store(k_lds[0]);
+            sv.store(v_lds[0]);
+            if (steps > 1) {
+                sk.load(k, kt, kv0 + 64, kv1);
+                sv.load(v, vt, kv0 + 64, kv1);
+            }
+        }
+        __syncthreads();
+        for (int it = 0; it < steps; ++it) {
+            char* kl = k_lds[it & 1];
+            char* vl = v_lds[it & 1];
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub) {
+                const int key0 = kv0 + it * 64 + sub * 32;
+                if (key0 >= wave_end) continue;
+                f32x16_t s[NH], dp[NH];
+#pragma unroll
+                for (int n = 0; n < NH; ++n) s[n] = dp[n] = zero16();
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                    const bf16x8_t kf = rows_frag<D>(kl, sub * 32, d, lane);
+                    const bf16x8_t vf = rows_frag<D>(vl, sub * 32, d, lane);
+#pragma unroll
+                    for (int n = 0; n < NH; ++n) {
+                        s[n] = mfma(kf, qf[n][d], s[n]);
+                        dp[n] = mfma(vf, of[n][d], dp[n]);
+                    }
+                }
+                use(s, dp, key0, kl, sub);
+            }
+            if (it + 1 < steps) {
+                sk.store(k_lds[(it + 1) & 1]);
+                sv.store(v_lds[(it + 1) & 1]);
+                if (it + 2 < steps) {
+                    sk.load(k, kt, kv0 + (it + 2) * 64, kv1);
+                    sv.load(v, vt, kv0 + (it + 2) * 64, kv1);
+                }
+                __syncthreads();
+            }
+        }
+    };
+    if (row0 == seq0) {
+        float sum[NH];
+#pragma unroll
+        for (int n = 0; n < NH; ++n) sum[n] = 0.f;
+        sweep([&](f32x16_t (&s)[NH], f32x16_t (&dp)[NH], int key0, char*, int) {
+#pragma unroll
+            for (int n = 0; n < NH; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (key0 + crow(r, hi) <= row)
+                        sum[n] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[n][r], c2, -ls[n])),
+                                      dp[n][r], sum[n]);
+        });
+#pragma unroll
+        for (int n = 0; n < NH; ++n) dl[n] = sum[n] + __shfl_xor(sum[n], 32, WAVE);
+        __syncthreads();   // before the second sweep writes over the tiles
+    }
+#pragma unroll
+    for (int n = 0; n < NH; ++n)
+        if (mine && hi == 0) delta[(long)(h0 + n) * T + row] = dl[n];
+    sweep([&](f32x16_t (&s)[NH], f32x16_t (&dp)[NH], int key0, char* kl, int sub) {
+        const bool inner = key0 + 31 <= wrow;   // every key open to every row
+        bf16x8_t df[NH][2];
+#pragma unroll
+        for (int n = 0; n < NH; ++n) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[n][r], c2, -ls[n]));
+                const float ds = p * (dp[n][r] - dl[n]);
+                s[n][r] = inner || key0 + crow(r, hi) <= row ? ds : 0.f;
+            }
+            df[n][0] = pack8(s[n], 0);
+            df[n][1] = pack8(s[n], 1);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db) {
+                const bf16x8_t kf = cols_frag<D>(kl, sub * 32 + ks * 16, db, lane);
+#pragma unroll
+                for (int n = 0; n < NH; ++n) acc[n][db] = mfma(kf, df[n][ks], acc[n][db]);
+            }
+    });
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+        if (!mine) continue;
+        store_row<D>(acc[n], seq1 < 0 ? NAN : scale, dq + ((long)row * Hq + h0 + n) * D, hi);
+    }
+}
+
+// ------------------------------------------------------------------- dk, dv
+//
+// A workgroup takes a tile of 128 keys of one kv head, a wave 32 of them, whose
+// k and v stay in registers; the queries of all the group's heads that see the
+// tile pass through LDS, 64 at a time.
+template <int D>
+__global__ void __launch_bounds__(256, D == 128 ? 1 : 2)
+packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
+                       const ushort_t* __restrict__ k, long kt, long kh,
+                       const ushort_t* __restrict__ v, long vt, long vh,
+                       const ushort_t* __restrict__ dout, long ot, long oh,
+                       const int4_t* __restrict__ tiles, const int* __restrict__ count,
+                       const float* __restrict__ lse, const float* __restrict__ delta,
+                       ushort_t* __restrict__ dk, ushort_t* __restrict__ dv,
+                       int T, int Hq, int Hk, float scale) {
+    const int t = blockIdx.x / Hk;
+    if (t >= *count) return;
+    const int hk = blockIdx.x % Hk;
+    const int group = Hq / Hk;
+    const int4_t tile = tiles[t];
+    const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
+    const bool real = seq1 > seq0;
+    const int lane = threadIdx.x & (WAVE - 1), wid = threadIdx.x / WAVE;
+    const int hi = lane >> 5;
+    const int wkey = row0 + wid * 32;
+    const int key = wkey + (lane & 31);
+    const bool mine = key < row1;
+    const float c2 = scale * LOG2E;
+
+    __shared__ char q_lds[2][64 * D * 2], o_lds[2][64 * D * 2];
+    __shared__ float4_t ls_lds[2][16], dl_lds[2][16];
+
+    bf16x8_t kf[D / 16], vf[D / 16];
+    load_row<D>(kf, k + key * kt + hk * kh, mine, hi);
+    load_row<D>(vf, v + key * vt + hk * vh, mine, hi);
+    f32x16_t ak[D / 32], av[D / 32];
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) ak[db] = av[db] = zero16();
+
+    Stage<D, 256> sq, so;
+    float stat = 0.f;   // threads 0..63: a row's log-sum, 64..127: its delta
+    const int per_head = real ? (seq1 - row0 + 63) / 64 : 0;
+    const int steps = per_head * group;
+    auto load = [&](int it) {
+        const int h = hk * group + it / per_head;
+        const int r0 = row0 + it % per_head * 64;
+        sq.load(q + h * qh, qt, r0, seq1);
+        so.load(dout + h * oh, ot, r0, seq1);
+        const int r = r0 + (threadIdx.x & 63);
+        if (threadIdx.x < 128) {
+            // past the sequence: P = exp2(0 - inf) = 0
+            const bool first = threadIdx.x < 64;
+            stat = first ? INFINITY : 0.f;
+            if (r < seq1) stat = (first ? lse : delta)[(long)h * T + r];
+        }
+    };
+    auto store = [&](int buf) {
+        sq.store(q_lds[buf]);
+        so.store(o_lds[buf]);
+        if (threadIdx.x < 64) reinterpret_cast<float*>(ls_lds[buf])[threadIdx.x] = stat;
+        else if (threadIdx.x < 128) reinterpret_cast<float*>(dl_lds[buf])[threadIdx.x - 64] = stat;
+    };
+    if (steps > 0) {
+        load(0);
+        store(0);
+        if (steps > 1) load(1);
+    }
+    __syncthreads();
+    for (int it = 0; it < steps; ++it) {
+        const int buf = it & 1;
+        char* ql = q_lds[buf];
+        char* ol = o_lds[buf];
+        const int r0 = row0 + it % per_head * 64;
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+            const int first = r0 + sub * 32;
+            // queries all before the wave's keys, or past the sequence
+            if (first + 31 < wkey || first >= seq1) continue;
+            f32x16_t s = zero16(), dp = zero16();
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                s = mfma(rows_frag<D>(ql, sub * 32, d, lane), kf[d], s);
+                dp = mfma(rows_frag<D>(ol, sub * 32, d, lane), vf[d], dp);
+            }
+            const bool inner = first >= wkey + 31;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4_t ls = ls_lds[buf][sub * 8 + 2 * g + hi];
+                const float4_t dl = dl_lds[buf][sub * 8 + 2 * g + hi];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = 4 * g + j;
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -ls[j]));
+                    const bool open = inner || first + crow(r, hi) >= key;
+                    dp[r] = open ? p * (dp[r] - dl[j]) : 0.f;
+                    s[r] = open ? p : 0.f;
+                }
+            }
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const bf16x8_t pf = pack8(s, ks), df = pack8(dp, ks);
+#pragma unroll
+                for (int db = 0; db < D / 32; ++db) {
+                    av[db] = mfma(cols_frag<D>(ol, sub * 32 + ks * 16, db, lane), pf, av[db]);
+                    ak[db] = mfma(cols_frag<D>(ql, sub * 32 + ks * 16, db, lane), df, ak[db]);
+                }
+            }
+        }
+        if (it + 1 < steps) {
+            store(buf ^ 1);
+            if (it + 2 < steps) load(it + 2);
+            __syncthreads();
+        }
+    }
+    if (mine) {
+        const long at = ((long)key * Hk + hk) * D;
+        store_row<D>(ak, seq1 < 0 ? NAN : scale, dk + at, hi);
+        store_row<D>(av, seq1 < 0 ? NAN : 1.f, dv + at, hi);
+    }
+}
+
+// ---------------------------------------------------------------- launchers
+// Each returns the launch's hipError_t.  `tiles` holds max_tiles tiles by
+// query, as many by key, and the count.
+
+extern "C" int launch_packed_tiles(const void* starts, int B, int T, int max_tiles,
+                                   void* tiles, void* stream) {
+    int4_t* a = (int4_t*)tiles;
+    hipLaunchKernelGGL(packed_tiles_kernel, dim3(1), dim3(512), 0, (hipStream_t)stream,
+                       (const int*)starts, B, T, max_tiles, a, a + max_tiles,
+                       (int*)(a + 2 * (long)max_tiles));
+    return (int)hipGetLastError();
+}
+
+namespace {
+
+template <int D, int NH, bool SAVE>
+void fwd(const void* q, long qt, long qh, const void* k, long kt, long kh,
+         const void* v, long vt, long vh, const void* tiles, int max_tiles, void* out,
+         void* lse, int T, int Hq, int Hk, float scale, hipStream_t st) {
+    const int4_t* a = (const int4_t*)tiles;
+    hipLaunchKernelGGL((packed_attn_fwd_kernel<D, NH, SAVE>),
+                       dim3((unsigned)max_tiles * (Hq / NH)), dim3(256), 0, st,
+                       (const ushort_t*)q, qt, qh, (const ushort_t*)k, kt, kh,
+                       (const ushort_t*)v, vt, vh, a, (const int*)(a + 2 * (long)max_tiles),
+                       (ushort_t*)out, (float*)lse, T, Hq, Hk, scale);
+}
+
+template <int D, int NH>
+void dq_(const void* q, long qt, long qh, const void* k, long kt, long kh,
+         const void* v, long vt, long vh, const void* dout, long ot, long oh,
+         const void* out, const void* tiles, int max_tiles,
+         const void* lse, void* delta, void* dq, int T, int Hq, int Hk, float scale,
+         hipStream_t st) {
+    const int4_t* a = (const int4_t*)tiles;
+    hipLaunchKernelGGL((packed_attn_dq_kernel<D, NH>),
+                       dim3((unsigned)max_tiles * (Hq / NH)), dim3(256), 0, st,
+                       (const ushort_t*)q, qt, qh, (const ushort_t*)k, kt, kh,
+                       (const ushort_t*)v, vt, vh, (const ushort_t*)dout, ot, oh,
+                       (const ushort_t*)out, a, (const int*)(a + 2 * (long)max_tiles), (const float*)lse,
+                       (float*)delta, (ushort_t*)dq, T, Hq, Hk, scale);
+}
+
+template <int D>
+void dkv(const void* q, long qt, long qh, const void* k, long kt, long kh,
+         const void* v, long vt, long vh, const void* dout, long ot, long oh,
+         const void* tiles, int max_tiles, const void* lse, const void* delta,
+         void* dk, void* dv, int T, int Hq, int Hk, float scale, hipStream_t st) {
+    const int4_t* a = (const int4_t*)tiles;
+    hipLaunchKernelGGL((packed_attn_dkv_kernel<D>), dim3((unsigned)max_tiles * Hk),
+                       dim3(256), 0, st,
+                       (const ushort_t*)q, qt, qh, (const ushort_t*)k, kt, kh,
+                       (const ushort_t*)v, vt, vh, (const ushort_t*)dout, ot, oh,
+                       a + max_tiles, (const int*)(a + 2 * (long)max_tiles),
+                       (const float*)lse, (const float*)delta, (ushort_t*)dk,
+                       (ushort_t*)dv, T, Hq, Hk, scale);
+}
+
+}  // namespace
+
+// lse is null where no backward pass will follow.
+extern "C" int launch_packed_attn_fwd(const void* q, long qt, long qh, const void* k,
+                                      long kt, long kh, const void* v, long vt, long vh,
+                                      const void* tiles, int max_tiles, void* out,
+                                      void* lse, int T, int Hq, int Hk, int D, float scale, void* stream) {
+    const bool pair = Hq / Hk % 2 == 0;
+#define FWD(d, n, s)                                                                   \
+    fwd<d, n, s>(q, qt, qh, k, kt, kh, v, vt, vh, tiles, max_tiles, out, lse, \
+                 T, Hq, Hk, scale, (hipStream_t)stream)
+    if (D == 128) {
+        if (lse) FWD(128, 1, true);
+        else FWD(128, 1, false);
+    } else if (pair) {
+        if (lse) FWD(64, 2, true);
+        else FWD(64, 2, false);
+    } else {
+        if (lse) FWD(64, 1, true);
+        else FWD(64, 1, false);
+    }
+#undef FWD
+    return (int)hipGetLastError();
+}
+
+extern "C" int launch_packed_attn_dq(const void* q, long qt, long qh, const void* k,
+                                     long kt, long kh, const void* v, long vt, long vh,
+                                     const void* dout, long ot, long oh, const void* out,
+                                     const void* tiles, int max_tiles,
+                                     const void* lse, void* delta, void* dq, int T, int Hq,
+                                     int Hk, int D, float scale, void* stream) {
+    const bool pair = Hq / Hk % 2 == 0;
+#define DQ(d, n)                                                                     \
+    dq_<d, n>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, out, tiles,             \
+              max_tiles, lse, delta, dq, T, Hq, Hk, scale, (hipStream_t)stream)
+    if (D == 128) DQ(128, 1);
+    else if (pair) DQ(64, 2);
+    else DQ(64, 1);
+#undef DQ
+    return (int)hipGetLastError();
+}
+
+extern "C" int launch_packed_attn_dkv(const void* q, long qt, long qh, const void* k,
+                                      long kt, long kh, const void* v, long vt, long vh,
+                                      const void* dout, long ot, long oh, const void* tiles,
+                                      int max_tiles, const void* lse, const void* delta,
+                                      void* dk, void* dv, int T, int Hq, int Hk, int D,
+                                      float scale, void* stream) {
+    if (D == 128)
+        dkv<128>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, tiles, max_tiles, lse,
+                 delta, dk, dv, T, Hq, Hk, scale, (hipStream_t)stream);
+    else
+        dkv<64>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, tiles, max_tiles, lse,
+                delta, dk, dv, T, Hq, Hk, scale, (hipStream_t)stream);
+    return (int)hipGetLastError();
+}

@@ -1,0 +1,350 @@
+// Bindings of the training kernels: packed attention with gradients,
+// cross-entropy, gradient norm and clipping.  Arguments are checked here, every
+// launch runs on the tensors' own device and its current stream, and scratch
+// memory comes from torch's allocator for each call, so that two streams or two
+// captured graphs never share any.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <algorithm>
+#include <cmath>
+#include <tuple>
+#include <vector>
+
+#include "grad_norm.h"
+
+extern "C" {
+int launch_packed_tiles(const void*, int, int, int, void*, void*);
+int launch_packed_attn_fwd(const void*, long, long, const void*, long, long, const void*,
+                           long, long, const void*, int, void*, void*, int, int, int, int,
+                           float, void*);
+int launch_packed_attn_dq(const void*, long, long, const void*, long, long, const void*,
+                          long, long, const void*, long, long, const void*, const void*,
+                          int, const void*, void*, void*, int, int, int, int,
+                          float, void*);
+int launch_packed_attn_dkv(const void*, long, long, const void*, long, long, const void*,
+                           long, long, const void*, long, long, const void*, int,
+                           const void*, const void*, void*, void*, int, int, int, int, float,
+                           void*);
+int launch_xent_fwd(int, const void*, long, const void*, long, int, int, void*, void*, void*);
+int launch_xent_reduce(const void*, const void*, long, int, int, void*, void*, void*);
+int launch_xent_bwd(int, const void*, long, const void*, long, int, int, const void*,
+                    const void*, long, const void*, void*, long, void*);
+int launch_grad_sums(const GradTable*, int, void*, void*);
+int launch_grad_norm(const void*, int, void*, void*);
+int launch_grad_clip(const GradTable*, int, const void*, int, double, double, void*, void*);
+}
+
+namespace {
+
+using torch::Tensor;
+
+void* stream_of(const Tensor& t) {
+    return (void*)at::cuda::getCurrentCUDAStream(t.device().index()).stream();
+}
+
+void launched(int code, const char* what) {
+    TORCH_CHECK(code == 0, what, ": the launch failed with HIP error ", code);
+}
+
+// ------------------------------------------------------------ packed attention
+
+void check_rows(const Tensor& t, const char* name, const Tensor& like) {
+    TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device());
+    TORCH_CHECK(t.scalar_type() == torch::kBFloat16, name, " must be bfloat16");
+    TORCH_CHECK(t.dim() == 3, name, " must have 3 dimensions: tokens, heads, head dim");
+    TORCH_CHECK(t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+                    t.stride(0) >= 0 && t.stride(1) >= 0 &&
+                    (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0,
+                name, " must have dense head rows at 16-byte boundaries");
+}
+
+long tiles_for(long T, long B) { return T / 128 + B + 2; }
+
+struct Sizes { int T, Hq, Hk, D; };
+
+Sizes check_qkv(const Tensor& q, const Tensor& k, const Tensor& v) {
+    check_rows(q, "q", q);
+    check_rows(k, "k", q);
+    check_rows(v, "v", q);
+    const long T = q.size(0), Hq = q.size(1), D = q.size(2), Hk = k.size(1);
+    TORCH_CHECK(D == 64 || D == 128, "head dim must be 64 or 128, not ", D);
+    TORCH_CHECK(k.size(0) == T && v.size(0) == T && k.size(2) == D && v.size(2) == D &&
+                    v.size(1) == Hk,
+                "q, k and v must have the same tokens and head dim, k and v the same heads");
+    TORCH_CHECK(Hk > 0 && Hq > 0 && Hq % Hk == 0,
+                "query heads must be a multiple of key/value heads");
+    TORCH_CHECK(T < (1L << 30), "at most 2^30 tokens");
+    return {(int)T, (int)Hq, (int)Hk, (int)D};
+}
+
+// -> out and, with `save`, lse and tiles
+std::vector<Tensor> packed_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor starts, double scale,
+                                    bool save) {
+    const Sizes s = check_qkv(q, k, v);
+    TORCH_CHECK(starts.device() == q.device() && starts.scalar_type() == torch::kInt32 &&
+                    starts.is_contiguous() && starts.dim() == 1 && starts.numel() >= 1,
+                "seq_starts must be a dense int32 vector on the device of q");
+    const long B = starts.numel() - 1, max_tiles = tiles_for(s.T, B);
+    TORCH_CHECK(max_tiles * s.Hq < (1L << 31), "too many sequences");
+    const c10::cuda::CUDAGuard guard(q.device());
+    const auto opt = q.options();
+    Tensor out = torch::empty({s.T, s.Hq, s.D}, opt), lse;
+    Tensor tiles = torch::empty({8 * max_tiles + 4}, opt.dtype(torch::kInt32));
+    if (save) lse = torch::empty({s.Hq, s.T}, opt.dtype(torch::kFloat32));
+    if (s.T > 0) {
+        void* st = stream_of(q);
+        launched(launch_packed_tiles(starts.data_ptr(), (int)B, s.T, (int)max_tiles,
+                                     tiles.data_ptr(), st), "packed_attention");
+        launched(launch_packed_attn_fwd(
+                     q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
+                     k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), tiles.data_ptr(),
+                     (int)max_tiles, out.data_ptr(), save ? lse.data_ptr() : nullptr, s.T, s.Hq, s.Hk, s.D, (float)scale, st),
+                 "packed_attention");
+    }
+    if (!save) return {out};
+    return {out, lse, tiles};
+}
+
+// -> dq, dk, dv
+std::vector<Tensor> packed_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out,
+                                    Tensor lse, Tensor tiles, double scale) {
+    const Sizes s = check_qkv(q, k, v);
+    check_rows(dout, "the gradient", q);
+    TORCH_CHECK(dout.sizes() == q.sizes(), "the gradient must have the shape of q");
+    const long max_tiles = (tiles.numel() - 4) / 8;
+    const c10::cuda::CUDAGuard guard(q.device());
+    const auto opt = q.options();
+    Tensor dq = torch::empty({s.T, s.Hq, s.D}, opt);
+    Tensor dk = torch::empty({s.T, s.Hk, s.D}, opt), dv = torch::empty_like(dk);
+    Tensor delta = torch::empty_like(lse);
+    if (s.T > 0) {
+        void* st = stream_of(q);
+        launched(launch_packed_attn_dq(
+                     q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
+                     k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), dout.data_ptr(),
+                     dout.stride(0), dout.stride(1), out.data_ptr(),
+                     tiles.data_ptr(), (int)max_tiles, lse.data_ptr(), delta.data_ptr(),
+                     dq.data_ptr(), s.T, s.Hq, s.Hk, s.D, (float)scale, st),
+                 "packed_attention's gradient");
+        launched(launch_packed_attn_dkv(
+                     q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
+                     k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), dout.data_ptr(),
+                     dout.stride(0), dout.stride(1), tiles.data_ptr(), (int)max_tiles,
+                     lse.data_ptr(), delta.data_ptr(), dk.data_ptr(), dv.data_ptr(), s.T, s.Hq,
+                     s.Hk, s.D, (float)scale, st),
+                 "packed_attention's gradient");
+    }
+    return {dq, dk, dv};
+}
+
+// --------------------------------------------------------------- cross-entropy
+
+int kind_of(const Tensor& t, const char* name) {
+    switch (t.scalar_type()) {
+        case torch::kFloat32: return 0;
+        case torch::kBFloat16: return 1;
+        case torch::kFloat16: return 2;
+        default: TORCH_CHECK(false, name, " must be float32, bfloat16 or float16");
+    }
+}
+
+void check_logits(const Tensor& x, const Tensor& targets) {
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.size(1) >= 1 &&
+                    (x.size(1) == 1 || x.stride(1) == 1),
+                "logits must be [rows, vocabulary] on the GPU with dense rows");
+    TORCH_CHECK(x.size(0) < (1L << 31) && x.size(1) < (1L << 30), "logits are too large");
+    TORCH_CHECK(targets.device() == x.device() && targets.scalar_type() == torch::kInt64 &&
+                    targets.is_contiguous() && targets.dim() == 1 &&
+                    targets.numel() == x.size(0),
+                "targets must be a dense int64 vector with one label a row, beside the logits");
+}
+
+// -> loss of each row, stats and, unless mode is 0, their mean (1) or sum (2) and
+// the factor that this puts before a row's gradient
+std::vector<Tensor> xent_fwd(Tensor x, Tensor targets, int64_t ignore, int64_t mode, bool save) {
+    check_logits(x, targets);
+    const int kind = kind_of(x, "logits");
+    const int N = (int)x.size(0), V = (int)x.size(1);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const auto opt = x.options().dtype(torch::kFloat32);
+    Tensor loss = torch::empty({N}, opt), stats = torch::empty({save ? N : 0, 2}, opt);
+    void* st = stream_of(x);
+    if (N > 0)
+        launched(launch_xent_fwd(kind, x.data_ptr(), x.stride(0), targets.data_ptr(), ignore, N,
+                                 V, loss.data_ptr(), save ? stats.data_ptr() : nullptr, st),
+                 "cross_entropy");
+    if (!mode) return {loss, stats};
+    Tensor result = torch::empty({}, opt), factor = torch::empty({}, opt);
+    launched(launch_xent_reduce(loss.data_ptr(), targets.data_ptr(), ignore, N, mode == 1,
+                                result.data_ptr(), factor.data_ptr(), st), "cross_entropy");
+    return {loss, stats, result, factor};
+}
+
+Tensor xent_bwd(Tensor gout, Tensor x, Tensor targets, int64_t ignore, Tensor stats,
+                c10::optional<Tensor> factor) {
+    check_logits(x, targets);
+    const int kind = kind_of(x, "logits");
+    const int N = (int)x.size(0), V = (int)x.size(1);
+    TORCH_CHECK(gout.device() == x.device() && gout.scalar_type() == torch::kFloat32 &&
+                    (gout.dim() == 0 || (gout.dim() == 1 && gout.numel() == N)),
+                "the gradient must be float32, one value or one a row");
+    const c10::cuda::CUDAGuard guard(x.device());
+    Tensor dx = torch::empty({N, V}, x.options());
+    // the kernel's vectors need the same distance to 16 bytes on both sides
+    const long size = x.element_size();
+    const auto off = [&](const Tensor& t) {
+        return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+    };
+    if (!off(x) || (N > 1 && (x.stride(0) - V) * size % 16 != 0))
+        x = x.clone(at::MemoryFormat::Contiguous);
+    if (N > 0)
+        launched(launch_xent_bwd(kind, x.data_ptr(), x.stride(0), targets.data_ptr(), ignore, N,
+                                 V, stats.data_ptr(), gout.data_ptr(),
+                                 gout.dim() ? gout.stride(0) : 0,
+                                 factor ? factor->data_ptr() : nullptr,
+                                 dx.data_ptr(), V, stream_of(x)),
+                 "cross_entropy's gradient");
+    return dx;
+}
+
+// --------------------------------------------------------------- gradient norm
+
+struct Grads {
+    std::vector<Tensor> at;     // dense memory, one for each gradient
+    std::vector<long> copied;   // those that are copies, to be written back
+    std::vector<GradTable> tables;
+    std::vector<int> blocks;
+    int partial = 0;
+};
+
+// Whether no two elements share memory, as in every slice of a dense tensor:
+// each stride reaches over all that the smaller ones cover.
+bool apart(const Tensor& t) {
+    std::vector<std::pair<long, long>> dims;
+    for (int64_t a = 0; a < t.dim(); ++a)
+        if (t.size(a) > 1) dims.emplace_back(t.stride(a), t.size(a));
+    std::sort(dims.begin(), dims.end());
+    long reach = 0;
+    for (const auto& d : dims) {
+        if (d.first <= reach) return false;
+        reach += (d.second - 1) * d.first;
+    }
+    return true;
+}
+
+Grads collect(const std::vector<Tensor>& grads, bool write) {
+    Grads g;
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    for (size_t i = 0; i < grads.size(); ++i) {
+        const Tensor& t = grads[i];
+        TORCH_CHECK(t.layout() == torch::kStrided && t.is_cuda() &&
+                        t.device() == grads[0].device(),
+                    "gradients must be dense and on one GPU");
+        kind_of(t, "gradients");
+        if (t.numel() == 0) continue;
+        Tensor d = t;
+        if (!t.is_non_overlapping_and_dense()) {
+            TORCH_CHECK(!write || apart(t),
+                        "a gradient must not share memory between its elements");
+            d = t.clone(at::MemoryFormat::Contiguous);
+            g.copied.push_back((long)i);
+        }
+        if (write) {
+            long last = 0;
+            for (int64_t a = 0; a < t.dim(); ++a) last += (t.size(a) - 1) * t.stride(a);
+            const auto p = reinterpret_cast<uintptr_t>(t.data_ptr());
+            spans.emplace_back(p, p + (last + 1) * t.element_size());
+        }
+        g.at.push_back(d);
+    }
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i)
+        TORCH_CHECK(spans[i].first >= spans[i - 1].second,
+                    "two of the gradients share memory");
+    for (const Tensor& d : g.at) {
+        const long size = d.element_size();
+        const auto p = reinterpret_cast<uintptr_t>(d.data_ptr());
+        const long chunks = ((long)(p & 15) / size + d.numel() + GRAD_CHUNK - 1) / GRAD_CHUNK;
+        TORCH_CHECK(p % size == 0 && chunks < (1L << 30), "a gradient is too large");
+        if (g.tables.empty() || g.tables.back().n == GRAD_TENSORS ||
+            g.tables.back().first[g.tables.back().n] + chunks >= (1L << 30)) {
+            g.tables.emplace_back();
+            g.tables.back().n = 0;
+            g.tables.back().first[0] = 0;
+        }
+        GradTable& t = g.tables.back();
+        t.ptr[t.n] = d.data_ptr();
+        t.size[t.n] = d.numel();
+        t.kind[t.n] = (unsigned char)kind_of(d, "gradients");
+        t.first[t.n + 1] = t.first[t.n] + (int)chunks;
+        ++t.n;
+    }
+    for (const GradTable& t : g.tables) {
+        g.blocks.push_back(std::min(t.first[t.n], 1024));
+        g.partial += g.blocks.back();
+    }
+    return g;
+}
+
+Tensor sums_of(const Grads& g, const Tensor& like, void* st) {
+    Tensor sums = torch::empty({g.partial}, like.options().dtype(torch::kFloat64));
+    int at = 0;
+    for (size_t i = 0; i < g.tables.size(); ++i) {
+        launched(launch_grad_sums(&g.tables[i], g.blocks[i], sums.data_ptr<double>() + at, st),
+                 "the gradient norm");
+        at += g.blocks[i];
+    }
+    return sums;
+}
+
+Tensor grad_norm(std::vector<Tensor> grads) {
+    TORCH_CHECK(!grads.empty(), "no gradients");
+    const Grads g = collect(grads, false);
+    const c10::cuda::CUDAGuard guard(grads[0].device());
+    void* st = stream_of(grads[0]);
+    Tensor norm = torch::empty({}, grads[0].options().dtype(torch::kFloat32));
+    const Tensor sums = sums_of(g, norm, st);
+    launched(launch_grad_norm(sums.data_ptr(), g.partial, norm.data_ptr(), st),
+             "the gradient norm");
+    return norm;
+}
+
+Tensor grad_clip(std::vector<Tensor> grads, double limit, double eps) {
+    TORCH_CHECK(!grads.empty(), "no gradients");
+    const Grads g = collect(grads, true);
+    const c10::cuda::CUDAGuard guard(grads[0].device());
+    void* st = stream_of(grads[0]);
+    Tensor norm = torch::empty({}, grads[0].options().dtype(torch::kFloat32));
+    const Tensor sums = sums_of(g, norm, st);
+    if (g.tables.empty())
+        launched(launch_grad_norm(sums.data_ptr(), 0, norm.data_ptr(), st), "the gradient norm");
+    for (size_t i = 0; i < g.tables.size(); ++i)
+        launched(launch_grad_clip(&g.tables[i], g.blocks[i], sums.data_ptr(), g.partial, limit,
+                                  eps, i ? nullptr : norm.data_ptr(), st),
+                 "clipping gradients");
+    size_t k = 0;
+    for (size_t i = 0, c = 0; i < grads.size(); ++i) {
+        if (grads[i].numel() == 0) continue;
+        if (c < g.copied.size() && g.copied[c] == (long)i) {
+            grads[i].copy_(g.at[k]);
+            ++c;
+        } else if (!grads[i].is_inference()) {
+            grads[i].unsafeGetTensorImpl()->bump_version();
+        }
+        ++k;
+    }
+    return norm;
+}
+
+}  // namespace
+
+void bind_training(pybind11::module_& m) {
+    m.def("packed_attn_fwd", &packed_attn_fwd, "causal attention of packed sequences");
+    m.def("packed_attn_bwd", &packed_attn_bwd, "its gradients");
+    m.def("xent_fwd", &xent_fwd, "cross-entropy of rows with labels");
+    m.def("xent_bwd", &xent_bwd, "its gradient");
+    m.def("grad_norm", &grad_norm, "norm of all gradients together");
+    m.def("grad_clip", &grad_clip, "norm of all gradients together, and clipping by it");
+}

@@ -210,3 +210,59 @@ def masked_sample(
         choice = torch.multinomial(sorted_probs, 1, generator=generator)
         return sorted_idx.gather(-1, choice).squeeze(-1)
     return torch.multinomial(probs, 1, generator=generator).squeeze(-1)
+
+
+def packed_attention(
+    q: torch.Tensor,              # [T, Hq, D]
+    k: torch.Tensor,              # [T, Hk, D]
+    v: torch.Tensor,              # [T, Hk, D]
+    seq_starts: torch.Tensor,     # [B+1] cumulative starts
+    scale: float,
+) -> torch.Tensor:
+    """Causal attention inside each packed sequence, differentiable; rows in
+    no sequence get zeros. Computes in fp32 (fp64 for fp64 inputs)."""
+    kind = torch.float64 if q.dtype == torch.float64 else torch.float32
+    group = q.shape[1] // k.shape[1]
+    starts = seq_starts.tolist()
+    parts = [q.new_zeros((starts[0], *q.shape[1:]))]
+    for s, e in zip(starts[:-1], starts[1:]):
+        qs = q[s:e].to(kind).transpose(0, 1)                                    # [Hq, S, D]
+        ks = k[s:e].to(kind).transpose(0, 1).repeat_interleave(group, dim=0)
+        vs = v[s:e].to(kind).transpose(0, 1).repeat_interleave(group, dim=0)
+        shut = torch.ones(e - s, e - s, dtype=torch.bool, device=q.device).triu(1)
+        probs = (qs @ ks.transpose(1, 2) * scale).masked_fill(shut, float("-inf")).softmax(-1)
+        parts.append((probs @ vs).transpose(0, 1).to(q.dtype))
+    parts.append(q.new_zeros((q.shape[0] - starts[-1], *q.shape[1:])))
+    return torch.cat(parts)
+
+
+def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,
+                  reduction: str = "mean") -> torch.Tensor:
+    """Cross-entropy over the labelled rows, differentiable; a label outside
+    the vocabulary makes its row's loss and gradient NaN. fp32 result (fp64
+    for fp64 logits)."""
+    real = targets != ignore_index
+    x, want = logits[real], targets[real]
+    x = x if x.dtype == torch.float64 else x.float()
+    inside = (want >= 0) & (want < x.shape[1])
+    some = -x.log_softmax(-1).gather(1, torch.where(inside, want, 0)[:, None])[:, 0]
+    some = some * torch.where(inside, 1.0, float("nan")).to(x.dtype)
+    each = torch.zeros(targets.shape, dtype=x.dtype, device=x.device)
+    each = each.index_put((real.nonzero()[:, 0],), some)
+    if reduction == "none":
+        return each
+    return each.sum() / real.sum() if reduction == "mean" else each.sum()
+
+
+def grad_norm(grads: list[torch.Tensor]) -> torch.Tensor:
+    """2-norm of all tensors together, summed in fp64."""
+    return torch.stack([g.double().square().sum() for g in grads]).sum().sqrt().float()
+
+
+def grad_clip(grads: list[torch.Tensor], max_norm: float, eps: float) -> torch.Tensor:
+    """Scales the tensors in place so that their norm is at most max_norm."""
+    norm = grad_norm(grads)
+    factor = (max_norm / (norm.double() + eps)).clamp(max=1.0).float()
+    for g in grads:
+        g.copy_(g.float() * factor)
+    return norm

@@ -1,0 +1,654 @@
+"""Operators of the packed training step: packed attention with gradients,
+cross-entropy, gradient norm and clipping. Everything is held to plain 64-bit
+arithmetic, with bounds that count the roundings a result goes through.
+
+The units: H = 2^-8, half a step of bf16 (2^-11 for fp16), and E = 2^-11 for
+all fp32 arithmetic on the way to a sum (a score is a sum of at most 128
+products: 128 * 2^-24 = 2^-17 of sum |q||k| scale, which is below 20 at these
+inputs, so a probability is off by less than 2^-12 of itself, twice)."""
+import math
+
+import pytest
+import torch
+
+from runbookai_amd import ops
+from runbookai_amd.ops import reference
+
+H, E = 2.0 ** -8, 2.0 ** -11
+
+gpu = pytest.mark.gpu
+
+
+def _starts(lens):
+    out = [0]
+    for n in lens:
+        out.append(out[-1] + n)
+    return out
+
+
+# ---------------------------------------------------------- packed attention
+
+def attention_oracle(q, k, v, dout, starts, scale):
+    """(out, dq, dk, dv) in 64 bits, and how far a kernel may be off each:
+    operands P and dS rounded once, the result once, delta from a rounded o
+    beyond a sequence's first 128 rows."""
+    q, k, v, dout = (x.detach().double().cpu() for x in (q, k, v, dout))
+    group = q.shape[1] // k.shape[1]
+    out, dq, dk, dv = (torch.zeros_like(x) for x in (q, q, k, v))
+    tol = [torch.zeros_like(x) for x in (q, q, k, v)]
+    for a, b in zip(starts[:-1], starts[1:]):
+        n = b - a
+        for h in range(q.shape[1]):
+            g = h // group
+            qs, ks, vs, do = q[a:b, h], k[a:b, g], v[a:b, g], dout[a:b, h]
+            s = (qs @ ks.T) * scale
+            s = s.masked_fill(torch.ones(n, n, dtype=torch.bool).triu(1), -math.inf)
+            p = s.softmax(-1)
+            o = p @ vs
+            dp = do @ vs.T
+            delta = (p * dp).sum(-1, keepdim=True)
+            ds = p * (dp - delta)
+            out[a:b, h] = o
+            dq[a:b, h] = ds @ ks * scale
+            dk[a:b, g] += ds.T @ qs * scale
+            dv[a:b, g] += p.T @ do
+            reach = p @ vs.abs()
+            tol[0][a:b, h] = (H + E) * reach + H * (o.abs() + H * reach)
+            # |error of dS| before its own rounding
+            far = (torch.arange(n) >= 128).double()[:, None]
+            e = E * p * (do.abs() @ vs.abs().T + delta.abs())
+            e = e + p * far * 2 * H * (do.abs() * reach).sum(-1, keepdim=True)
+            e = e + H * (ds.abs() + e)
+            tol[1][a:b, h] = e @ ks.abs() * scale * (1 + H) + H * dq[a:b, h].abs()
+            tol[2][a:b, g] += e.T @ qs.abs() * scale * (1 + H)
+            tol[3][a:b, g] += (H + E) * (p.T @ do.abs()) * (1 + H)
+    tol[2] += H * dk.abs()
+    tol[3] += H * dv.abs()
+    return (out, dq, dk, dv), tol
+
+
+def _inputs(lens, heads, d, pad=0, device="cpu", dtype=torch.bfloat16, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    T = sum(lens) + pad
+    hq, hk = heads
+    mk = lambda h, std: (torch.randn(T, h, d, generator=gen) * std).to(dtype).to(device)  # noqa: E731
+    return mk(hq, 1.0), mk(hk, 1.0), mk(hk, 1.0), mk(hq, 0.1)
+
+
+def _attend(q, k, v, dout, starts, scale=None):
+    q, k, v = (x.detach().requires_grad_() for x in (q, k, v))
+    out = ops.packed_attention(q, k, v, starts, scale=scale)
+    return (out.detach(), *torch.autograd.grad(out, (q, k, v), dout))
+
+
+def _within(got, want, tol, names=("out", "dq", "dk", "dv")):
+    for name, x, y, t in zip(names, got, want, tol):
+        x = x.double().cpu()
+        assert torch.isfinite(x).all(), name
+        over = (x - y).abs() - t
+        assert (over <= 1e-30).all(), (name, float(over.max()), int((over > 0).sum()))
+
+
+LENGTHS = [
+    [1], [2], [31], [32, 33], [63, 64, 65], [127, 128, 129], [0, 1, 0, 0, 5, 0],
+    [257, 3, 640], [1] * 70, [1000],
+]
+
+
+@pytest.mark.parametrize("lens", [[1], [5, 0, 3], [0], [7, 20]])
+@pytest.mark.parametrize("heads", [(4, 2), (3, 3)])
+def test_attention_reference(lens, heads):
+    q, k, v, dout = _inputs(lens, heads, 8, pad=2, dtype=torch.float64)
+    starts = torch.tensor(_starts(lens), dtype=torch.int32)
+    want, _ = attention_oracle(q, k, v, dout, starts.tolist(), 0.4)
+    for x, y in zip(_attend(q, k, v, dout, starts, 0.4), want):
+        torch.testing.assert_close(x, y, rtol=1e-12, atol=1e-12)
+
+
+def test_attention_reference_gradcheck():
+    q, k, v, _ = _inputs([4, 3], (2, 1), 4, pad=1, dtype=torch.float64)
+    starts = torch.tensor([0, 4, 7])
+    assert torch.autograd.gradcheck(
+        lambda *a: ops.packed_attention(*a, starts), [x.requires_grad_() for x in (q, k, v)])
+
+
+def test_attention_reference_agrees_with_prefill():
+    q, k, v, _ = _inputs([9, 14], (4, 2), 64)
+    starts = torch.tensor([0, 9, 23], dtype=torch.int32)
+    a = ops.packed_attention(q, k, v, starts)
+    b = reference.prefill_attention(q, k, v, starts)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_attention_refuses(device):
+    q, k, v, _ = _inputs([4], (4, 2), 64, device=device)
+    starts = torch.tensor([0, 4], dtype=torch.int32)
+    call = ops.packed_attention
+    bad = [
+        (q[0], k, v, starts), (q, k[:3], v, starts), (q, k, v[:, :1], starts),
+        (q[:, :3], k, v, starts), (q, k.float(), v, starts), (q, k[:, :0], v[:, :0], starts),
+        (q, k, v, starts.float()), (q, k, v, starts[None]), (q, k, v, starts[:0]),
+        (q, k, v, torch.tensor([0, 5])), (q, k, v, torch.tensor([-1, 4])),
+        (q, k, v, torch.tensor([0, 3, 2])),
+    ]
+    for args in bad:
+        with pytest.raises(ValueError):
+            call(*args)
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError):
+            call(q, k, v, starts, scale=scale)
+    if device == "cuda":
+        with pytest.raises(ValueError):
+            call(q.float(), k.float(), v.float(), starts)
+        with pytest.raises(ValueError):
+            call(q[..., :32], k[..., :32], v[..., :32], starts)
+        with pytest.raises(ValueError):
+            call(q, k.cpu(), v, starts)
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads", [(4, 2), (3, 3), (6, 2), (8, 1)])
+@pytest.mark.parametrize("lens", LENGTHS, ids=lambda x: "-".join(map(str, x))[:20])
+def test_attention_gpu(lens, heads, d):
+    q, k, v, dout = _inputs(lens, heads, d, pad=5, device="cuda")
+    starts = _starts(lens)
+    got = _attend(q, k, v, dout, torch.tensor(starts, dtype=torch.int32, device="cuda"))
+    want, tol = attention_oracle(q, k, v, dout, starts, 1.0 / math.sqrt(d))
+    _within(got, want, tol)
+    end = starts[-1]
+    assert all(not x[end:].any() for x in got)   # rows in no sequence
+    with torch.no_grad():
+        plain = ops.packed_attention(q, k, v, torch.tensor(starts))
+    assert torch.equal(plain, got[0])
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_gpu_sharp_scores(d):
+    """Scores far apart: the running maximum grows many times, and most
+    probabilities underflow."""
+    lens = [300, 41]
+    q, k, v, dout = _inputs(lens, (4, 2), d, device="cuda")
+    ramp = torch.linspace(0.1, 8.0, sum(lens), device="cuda")[:, None, None]
+    k = (k * ramp).to(torch.bfloat16)
+    starts = _starts(lens)
+    got = _attend(q, k, v, dout, torch.tensor(starts, device="cuda"))
+    want, tol = attention_oracle(q, k, v, dout, starts, 1.0 / math.sqrt(d))
+    # sum |q||k| scale is 8 times what E counts with
+    _within(got, want, [8 * t for t in tol])
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_gpu_views(d):
+    """q, k, v as slices of one projection, an expanded and a misaligned one,
+    and a broadcast gradient."""
+    lens, hq, hk = [70, 1, 130], 4, 2
+    T, starts = sum(lens), torch.tensor(_starts(lens), dtype=torch.int32, device="cuda")
+    gen = torch.Generator().manual_seed(3)
+    qkv = torch.randn(T, (hq + 2 * hk) * d, generator=gen).to(torch.bfloat16).cuda()
+    q, k, v = (x.view(T, -1, d) for x in qkv.split([hq * d, hk * d, hk * d], -1))
+    dout = (torch.randn(T, 1, 1, generator=gen) * 0.1).to(torch.bfloat16).cuda().expand(T, hq, d)
+    dense = _attend(*(x.contiguous() for x in (q, k, v, dout)), starts)
+    for x, y in zip(_attend(q, k, v, dout, starts), dense):
+        assert torch.equal(x, y)
+    off = torch.empty(T * hk * d + 1, dtype=torch.bfloat16, device="cuda")[1:].view(T, hk, d)
+    off.copy_(k)
+    turned = v.transpose(0, 1).contiguous().transpose(0, 1)
+    for x, y in zip(_attend(q, off, turned, dout, starts), dense):
+        assert torch.equal(x, y)
+    one = k[:, :1].expand(T, hk, d)
+    got = _attend(q, one, v, dout, starts)
+    for x, y in zip(got, _attend(q, one.contiguous(), v, dout, starts)):
+        assert torch.equal(x, y)
+
+
+@gpu
+def test_attention_gpu_fused_projection_gradient():
+    """The gradient arrives in the tensor that q, k and v are slices of."""
+    T, hq, hk, d = 90, 4, 2, 64
+    starts = torch.tensor([0, 40, 90], device="cuda")
+    x = torch.randn(T, (hq + 2 * hk) * d, device="cuda").to(torch.bfloat16).requires_grad_()
+    parts = [p.view(T, -1, d) for p in x.split([hq * d, hk * d, hk * d], -1)]
+    out = ops.packed_attention(*parts, starts)
+    dout = torch.randn_like(out)
+    out.backward(dout)
+    got = _attend(*(p.detach() for p in parts), dout, starts)[1:]
+    assert torch.equal(x.grad, torch.cat([g.reshape(T, -1) for g in got], -1))
+
+
+@gpu
+def test_attention_gpu_not_finite_elsewhere():
+    """What other sequences and unused rows hold changes nothing."""
+    lens, d = [60, 200, 1], 64
+    starts = torch.tensor([10, 70, 270, 271], dtype=torch.int32, device="cuda")
+    q, k, v, dout = _inputs(lens, (4, 2), d, pad=29, device="cuda")
+    clean = _attend(q, k, v, dout, starts)
+    for x in (q, k, v, dout):
+        x[:10] = math.nan
+        x[70:270, :, ::3] = math.inf
+        x[271:] = math.nan
+    got = _attend(q, k, v, dout, starts)
+    for x, y in zip(got, clean):
+        assert torch.equal(x[10:70], y[10:70]) and torch.equal(x[270], y[270])
+        assert not x[:10].any() and not x[271:].any()
+
+
+@gpu
+@pytest.mark.parametrize("starts", [[0, 300], [0, 120, 60, 200], [-4, 200], [5, 3]])
+def test_attention_gpu_wrong_starts(starts):
+    q, k, v, dout = _inputs([200], (4, 2), 64, device="cuda")
+    got = _attend(q, k, v, dout, torch.tensor(starts, dtype=torch.int32, device="cuda"))
+    assert all(torch.isnan(x).all() for x in got)
+
+
+@gpu
+def test_attention_gpu_nothing():
+    q, k, v, dout = _inputs([0], (4, 2), 64, device="cuda")
+    for starts in ([0], [0, 0, 0]):
+        got = _attend(q, k, v, dout, torch.tensor(starts, device="cuda"))
+        assert [x.shape[0] for x in got] == [0] * 4
+    q, k, v, dout = _inputs([3], (4, 2), 64, device="cuda")
+    assert not any(x.any() for x in _attend(q, k, v, dout, torch.tensor([0], device="cuda")))
+
+
+@gpu
+def test_attention_gpu_repeats_bit_for_bit_on_another_stream():
+    q, k, v, dout = _inputs([500, 77, 300], (8, 2), 128, device="cuda")
+    starts = torch.tensor([0, 500, 577, 877], device="cuda")
+    want = _attend(q, k, v, dout, starts)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a = _attend(q, k, v, dout, starts)
+    b = _attend(k.repeat_interleave(4, 1), k, v, dout, starts)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, y) for x, y in zip(a, want))
+    assert not torch.equal(b[0], want[0])
+
+
+@gpu
+def test_attention_gpu_captured():
+    """Forward and backward in one graph: new data and new sequences in the
+    same buffers, replayed between eager calls."""
+    T = 400
+    q, k, v, dout = _inputs([T], (4, 2), 64, device="cuda")
+    starts = torch.tensor([0, 100, 100, 380], dtype=torch.int32, device="cuda")
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+
+    def step():
+        out = ops.packed_attention(*leaves, starts)
+        return (out, *torch.autograd.grad(out, leaves, dout))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = step()
+    for i, ends in enumerate(([100, 100, 380], [1, 399, 400], [0, 0, 256])):
+        with torch.no_grad():
+            for x, y in zip((q, k, v, dout), _inputs([T], (4, 2), 64, device="cuda", seed=i)):
+                x.copy_(y)
+            starts.copy_(torch.tensor([0] + ends, dtype=torch.int32))
+        graph.replay()
+        got = [x.detach().clone() for x in static]
+        for x, y in zip(got, _attend(q, k, v, dout, starts)):
+            assert torch.equal(x, y)
+        torch.cuda.synchronize()
+
+
+@gpu
+def test_attention_gpu_gradient_against_differences():
+    """The gradients against differences of the loss in 64 bits."""
+    lens, d = [50, 150], 64
+    q, k, v, dout = _inputs(lens, (4, 2), d, device="cuda")
+    starts = _starts(lens)
+    got = _attend(q, k, v, dout, torch.tensor(starts, device="cuda"))[1:]
+    base = [x.double().cpu() for x in (q, k, v)]
+    gen = torch.Generator().manual_seed(1)
+
+    def loss(parts):
+        out = reference.packed_attention(*parts, torch.tensor(starts), 1 / math.sqrt(d))
+        return float((out * dout.double().cpu()).sum())
+
+    _, tol = attention_oracle(q, k, v, dout, starts, 1 / math.sqrt(d))
+    for i in range(3):
+        way = torch.randn(base[i].shape, generator=gen, dtype=torch.float64)
+        h = 1e-5
+        up, down = ([b + s * h * way if j == i else b for j, b in enumerate(base)]
+                    for s in (1, -1))
+        slope = (loss(up) - loss(down)) / (2 * h)
+        mine = float((got[i].double().cpu() * way).sum())
+        # what the bound allows each element, and 1e-6 for the third derivative
+        assert abs(mine - slope) <= float((tol[i + 1] * way.abs()).sum()) + 1e-6
+
+
+@gpu
+def test_attention_gpu_long():
+    """One sequence of many tiles; rows far apart in the result are checked."""
+    T, d = 20000, 64
+    q, k, v, _ = _inputs([T], (2, 1), d, device="cuda")
+    with torch.no_grad():
+        out = ops.packed_attention(q, k, v, torch.tensor([0, T], device="cuda"))
+    for row in (0, 127, 128, 9999, 16383, T - 1):
+        ks, vs = k[:row + 1, 0].double(), v[:row + 1, 0].double()
+        p = (q[row].double() @ ks.T / math.sqrt(d)).softmax(-1)
+        want, reach = p @ vs, p @ vs.abs()
+        assert ((out[row].double() - want).abs() <= (H + E) * reach + H * want.abs() + H * H).all()
+
+
+# ------------------------------------------------------------- cross-entropy
+
+def loss_oracle(x, targets, reduction, gout, ignore=-100):
+    x = x.detach().double().cpu().requires_grad_()
+    t = targets.cpu()
+    real = t != ignore
+    each = torch.zeros(t.shape, dtype=torch.float64)
+    each[real] = (x.logsumexp(-1) - x.gather(1, t.clamp(min=0).long()[:, None])[:, 0])[real]
+    loss = {"none": each, "sum": each.sum(), "mean": each.sum() / real.sum()}[reduction]
+    grad, = torch.autograd.grad(loss, x, gout.double().cpu())
+    return loss.detach(), grad
+
+
+SIZES = [(1, 1), (3, 2), (5, 7), (4, 64), (9, 511), (2, 4096), (3, 4099), (5, 8192), (2, 8193),
+         (2, 20001), (1, 128256)]
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def _loss_inputs(n, v, dtype, device, seed=0, labelled=0.6):
+    gen = torch.Generator().manual_seed(seed)
+    x = (torch.randn(n, v, generator=gen) * 3).to(dtype).to(device)
+    t = torch.randint(0, v, (n,), generator=gen)
+    t[torch.rand(n, generator=gen) >= labelled] = -100
+    t[0] = v - 1
+    return x, t.to(device)
+
+
+def _loss_and_grad(x, t, reduction, gout=None, **kw):
+    x = x.detach().requires_grad_()
+    loss = ops.cross_entropy(x, t, reduction=reduction, **kw)
+    gout = torch.ones_like(loss) if gout is None else gout
+    return loss.detach(), torch.autograd.grad(loss, x, gout)[0]
+
+
+def _check_loss(got, want, dtype, gout):
+    loss, grad = got
+    # a row: exp of a product rounded once, summed, logarithm, two additions of
+    # values below 32: 2^-24 * (32 + 32 + 16); sums of rows are fp64
+    assert loss.dtype == torch.float32
+    err = (loss.double().cpu() - want[0]).abs()
+    assert (err <= 2.0 ** -24 * (80 + want[0].abs())
+            * (loss.numel() == 1 and 64 or 1)).all(), float(err.max())
+    # a gradient: probability off by 2^-24 * 32 of itself, one rounding; fp16's
+    # steps end at 2^-24
+    g = gout.double().cpu().abs().max()
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    err = (grad.double().cpu() - want[1]).abs()
+    assert (err <= HALF[dtype] * 1.01 * want[1].abs() + 2.0 ** -18 * g * want[1].abs().clamp(max=1)
+            + 2.0 ** -23 * g + tiny).all(), float(err.max())
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("n,v", SIZES)
+def test_loss(n, v, reduction, dtype, device):
+    x, t = _loss_inputs(n, v, dtype, device)
+    got = _loss_and_grad(x, t, reduction)
+    gout = torch.ones_like(got[0])
+    _check_loss(got, loss_oracle(x, t, reduction, gout), dtype, gout)
+    assert got[1].dtype == dtype and not got[1][t == -100].any()
+    with torch.no_grad():
+        assert torch.equal(ops.cross_entropy(x, t, reduction=reduction), got[0])
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_loss_factors(device):
+    """What comes back multiplies the gradient before it is rounded: a loss
+    scale keeps fp16 gradients in range, one value a row reaches its row."""
+    x, t = _loss_inputs(40, 300, torch.float16, device)
+    scale = torch.tensor(65536.0, device=device)
+    _, grad = _loss_and_grad(x, t, "mean", scale)
+    want = loss_oracle(x, t, "mean", scale)[1]
+    err = (grad.double().cpu() - want).abs()
+    assert (err <= 2.0 ** -11 * 1.01 * want.abs() + 2.0 ** -16 * want.abs() + 2.0 ** -7).all()
+    each = torch.rand(40, device=device)
+    got = _loss_and_grad(x.float(), t, "none", each)
+    want = loss_oracle(x, t, "none", each)
+    _check_loss(got, want, torch.float32, each)
+    got = _loss_and_grad(x.float(), t, "none", torch.ones((), device=device).expand(40))
+    assert torch.equal(got[1], _loss_and_grad(x.float(), t, "sum")[1])
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("v", [37, 9001])
+def test_loss_edges(v, device):
+    x = torch.randn(7, v).to(device)
+    t = torch.tensor([0, 1, 2, 3, 4, 5, -1], device=device)
+    x[0, 5:] = -math.inf          # a vocabulary shut off but for five
+    x[1] = -math.inf              # nothing left
+    x[2, 2] = -math.inf           # the label shut off
+    x[3, 7] = math.nan
+    x[4] = 3e38                   # far from zero, all alike
+    t[5] = v                      # no such place, and another below zero
+    loss, grad = _loss_and_grad(x, t, "none")
+    assert torch.isfinite(loss[0]) and not grad[0, 5:].any()
+    assert abs(float(grad[0].sum())) < 1e-6
+    assert torch.isnan(loss[1])
+    assert loss[2] == math.inf
+    assert torch.isnan(loss[3]) and torch.isnan(grad[3]).any()
+    assert abs(float(loss[4]) - math.log(v)) < 1e-5
+    assert torch.isnan(loss[5]) and torch.isnan(grad[5]).all()
+    assert torch.isnan(loss[6]) and torch.isnan(grad[6]).all()
+    loss, grad = _loss_and_grad(x, t.fill_(-100), "mean")
+    assert torch.isnan(loss) and not grad.any()
+    loss, grad = _loss_and_grad(x, t, "sum")
+    assert loss == 0 and not grad.any()
+    assert float(ops.cross_entropy(x[:0], t[:0], reduction="sum")) == 0
+    assert ops.cross_entropy(x[:0], t[:0], reduction="none").shape == (0,)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_loss_views(dtype, device):
+    """Rows of a wider buffer, an odd start, transposed, other label types."""
+    wide, t = _loss_inputs(12, 1000, dtype, device)
+    t = t.clamp(max=900)
+    for x in (wide[:, :901], wide[:, 3:904], wide[::2, :901], wide[1:, :901],
+              wide[:, :901].t().contiguous().t()):
+        n = x.shape[0]
+        got = _loss_and_grad(x, t[:n].int(), "mean")
+        want = _loss_and_grad(x.clone(memory_format=torch.contiguous_format), t[:n], "mean")
+        assert abs(float(got[0] - want[0])) <= 2.0 ** -20 * float(want[0])
+        torch.testing.assert_close(got[1], want[1], rtol=2 * HALF[dtype], atol=2.0 ** -24)
+    other = t.masked_fill(t == -100, 0)
+    a = _loss_and_grad(wide[:, :901], other, "mean", ignore_index=0)
+    b = _loss_and_grad(wide[:, :901], other.masked_fill(other == 0, -100), "mean")
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_loss_agrees_with_torch():
+    x, t = _loss_inputs(20, 33, torch.float32, "cpu")
+    torch.testing.assert_close(ops.cross_entropy(x, t), torch.nn.functional.cross_entropy(x, t))
+    x = x[:4].double().requires_grad_()
+    assert torch.autograd.gradcheck(lambda y: ops.cross_entropy(y, t[:4]), x)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_loss_refuses(device):
+    x, t = _loss_inputs(4, 9, torch.float32, device)
+    for args in ((x[0], t), (x, t[:3]), (x, t.float()), (x[None], t[None]), (x[:, :0], t)):
+        with pytest.raises(ValueError):
+            ops.cross_entropy(*args)
+    with pytest.raises(ValueError):
+        ops.cross_entropy(x, t, reduction="max")
+    if device == "cuda":
+        with pytest.raises(ValueError):
+            ops.cross_entropy(x.double(), t)
+        with pytest.raises(ValueError):
+            ops.cross_entropy(x, t.cpu())
+
+
+# ------------------------------------------------------------- gradient norm
+
+def _params(shapes, dtypes, device, std=0.1, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    out = []
+    for i, shape in enumerate(shapes):
+        dtype = dtypes[i % len(dtypes)]
+        p = torch.nn.Parameter(torch.zeros(shape, dtype=dtype, device=device))
+        p.grad = (torch.randn(shape, generator=gen) * std).to(dtype).to(device)
+        out.append(p)
+    return out
+
+
+def _check_clip(params, limit):
+    """Clips, and compares with 64 bits: the factor is rounded to fp32, the
+    product to fp32 and to the gradient's type."""
+    before = [p.grad.detach().double().cpu() for p in params]
+    want = math.sqrt(sum(float(g.square().sum()) for g in before))
+    assert abs(float(ops.grad_norm(params)) - want) <= 2.0 ** -23 * want
+    norm = ops.clip_grad_norm_(params, limit)
+    assert norm.dtype == torch.float32 and norm.dim() == 0
+    assert abs(float(norm) - want) <= 2.0 ** -23 * want
+    factor = min(1.0, limit / (want + 1e-6))
+    for p, g in zip(params, before):
+        got = p.grad.detach().double().cpu()
+        if factor == 1.0:
+            assert torch.equal(got, g)
+            continue
+        tiny = 2.0 ** -25 if p.dtype == torch.float16 else 0.0
+        err = (got - g * factor).abs()
+        assert (err <= (HALF[p.dtype] + 2.0 ** -22) * g.abs() * factor * 1.01 + tiny).all()
+
+
+MIXED = [torch.float32, torch.bfloat16, torch.float16]
+SHAPES = [(1,), (), (7, 3), (0,), (8192,), (8193,), (4095, 5), (3, 1, 2), (100_000,), (2,)]
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("dtypes", [MIXED[:1], MIXED[1:2], MIXED])
+@pytest.mark.parametrize("limit", [0.0, 0.5, 1e6, math.inf])
+def test_clip(limit, dtypes, device):
+    _check_clip(_params(SHAPES, dtypes, device), limit)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_clip_many(device):
+    """More tensors than one launch takes."""
+    _check_clip(_params([(i % 37 + 1,) for i in range(300)], MIXED, device), 0.25)
+
+
+@gpu
+def test_clip_gpu_large():
+    params = _params([(3_000_001,), (5, 700_003)], MIXED[:2], "cuda")
+    _check_clip(params, 1.0)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_clip_strides_and_alignment(device):
+    """Slices of one flat buffer at odd starts, turned and spaced tensors:
+    nothing beside them changes."""
+    for dtype in MIXED:
+        flat = torch.randn(40_000).to(dtype).to(device)
+        keep = flat.clone()
+        cuts = [(1, 8), (9, 9001), (9002, 9003), (9011, 20_000)]
+        params = []
+        for a, b in cuts:
+            p = torch.nn.Parameter(torch.zeros(b - a, dtype=dtype, device=device))
+            p.grad = flat[a:b]
+            params.append(p)
+        p = torch.nn.Parameter(torch.zeros(30, 40, dtype=dtype, device=device))
+        p.grad = torch.randn(40, 30).to(dtype).to(device).t()
+        params.append(p)
+        gaps = torch.randn(50, 20).to(dtype).to(device)
+        was = gaps.clone()
+        p = torch.nn.Parameter(torch.zeros(25, 10, dtype=dtype, device=device))
+        p.grad = gaps[::2, 3:13]
+        params.append(p)
+        _check_clip(params, 0.5)
+        inside = torch.zeros(40_000, dtype=torch.bool)
+        for a, b in cuts:
+            inside[a:b] = True
+        assert torch.equal(flat.cpu()[~inside], keep.cpu()[~inside])
+        assert torch.equal(gaps[1::2], was[1::2]) and torch.equal(gaps[:, 13:], was[:, 13:])
+        assert torch.equal(gaps[:, :3], was[:, :3])
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_clip_range(device):
+    """Squares that 32 bits do not hold."""
+    for std in (1e25, 1e-30):
+        params = _params([(500,)], MIXED[:1], device, std=std)
+        want = float(params[0].grad.double().norm())
+        assert abs(float(ops.grad_norm(params)) / want - 1) < 1e-6
+    before = params[0].grad.clone()
+    ops.clip_grad_norm_(params, 1.0)
+    assert torch.equal(params[0].grad, before)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_clip_not_finite(device):
+    """As torch's: an infinite norm leaves zeros and NaN, a NaN norm NaN."""
+    for bad in (math.inf, math.nan):
+        params = _params([(5,), (9000,)], MIXED[:1], device)
+        params[1].grad[77] = bad
+        twin = [p.grad.clone() for p in params]
+        with pytest.raises(RuntimeError):
+            ops.clip_grad_norm_(iter(params), 1.0, error_if_nonfinite=True)
+        assert all(torch.equal(p.grad, t) or bad != bad for p, t in zip(params, twin))
+        norm = ops.clip_grad_norm_(params, 1.0)
+        other = [torch.nn.Parameter(torch.zeros_like(p)) for p in params]
+        for q, t in zip(other, twin):
+            q.grad = t
+        torch.testing.assert_close(norm, torch.nn.utils.clip_grad_norm_(other, 1.0),
+                                   equal_nan=True)
+        for p, q in zip(params, other):
+            assert torch.equal(torch.isnan(p.grad), torch.isnan(q.grad))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_clip_forms(device):
+    one = torch.nn.Parameter(torch.zeros(3, device=device))
+    assert float(ops.clip_grad_norm_(one, 1.0)) == 0.0     # no gradient
+    assert float(ops.grad_norm([])) == 0.0
+    one.grad = torch.tensor([3.0, 0.0, 4.0], device=device)
+    version = one.grad._version
+    assert float(ops.clip_grad_norm_((p for p in [one]), 1.0)) == 5.0
+    assert one.grad._version > version
+    torch.testing.assert_close(one.grad.cpu(), torch.tensor([0.6, 0.0, 0.8]))
+    one.grad = torch.zeros(3, device=device)
+    assert float(ops.clip_grad_norm_(one, 0.0)) == 0.0
+    none = torch.nn.Parameter(torch.zeros(0, device=device))
+    none.grad = torch.zeros(0, device=device)
+    assert float(ops.clip_grad_norm_(none, 1.0)) == 0.0
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_clip_refuses(device):
+    params = _params([(4,), (5,)], MIXED[:1], device)
+    for limit in (-1.0, math.nan):
+        with pytest.raises(ValueError):
+            ops.clip_grad_norm_(params, limit)
+    wide = torch.nn.Parameter(torch.zeros(4, dtype=torch.float64, device=device))
+    wide.grad = torch.ones_like(wide)
+    with pytest.raises(ValueError):
+        ops.clip_grad_norm_([wide], 1.0)
+    if device == "cuda":
+        with pytest.raises(RuntimeError):
+            ops.clip_grad_norm_([params[0], params[0]], 1.0)
+        spread = torch.nn.Parameter(torch.zeros(4, device=device))
+        spread.grad = torch.ones(1, device=device).expand(4)
+        with pytest.raises(RuntimeError):
+            ops.clip_grad_norm_([spread], 1.0)
+        assert float(ops.grad_norm([spread])) == 2.0
+        host = torch.nn.Parameter(torch.zeros(4))
+        host.grad = torch.ones(4)
+        with pytest.raises(ValueError):
+            ops.clip_grad_norm_([params[0], host], 1.0)
+        assert torch.equal(host.grad, torch.ones(4))
