@@ -206,73 +206,6 @@ def paged_decode_attention(q, k_cache, v_cache, block_tables, seq_lens,
                                             seq_lens, scale)
 
 
-def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
-                     seq_starts: torch.Tensor, scale: Optional[float] = None) -> torch.Tensor:
-    """Causal attention of packed sequences, with gradients for q, k and v.
-
-    q [T, Hq, D], k and v [T, Hk, D] (Hq a multiple of Hk) hold sequences one
-    after another; sequence b has rows seq_starts[b] up to seq_starts[b + 1],
-    which may be none, and each row attends to its own sequence's rows up to
-    itself. Rows in no sequence (a buffer's unused end) get zeros, in the
-    output and in the gradients, whatever they hold. scale defaults to
-    1 / sqrt(D).
-
-    On the GPU: bfloat16, D 64 or 128. q, k and v may be views (slices of a
-    fused projection, say): rows at 16-byte boundaries are read in place,
-    others are copied first. The starts stay on the device and nothing waits
-    for the host, so forward and backward can be captured into a graph.
-    Starts on the host are checked; starts on the device cannot be without
-    waiting for them: where they fall or leave [0, T], every output and
-    gradient is NaN. A value that is not finite reaches no other sequence.
-
-    The training counterpart of prefill_attention, which has no gradients."""
-    from .training import packed_attention as impl
-
-    return impl(q, k, v, seq_starts, scale)
-
-
-def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,
-                  reduction: str = "mean") -> torch.Tensor:
-    """Cross-entropy of logits [N, V] with integer labels [N], with its
-    gradient; fp32 result.
-
-    Rows labelled ignore_index count for nothing: their loss is 0, their
-    gradient zeros, their logits are not read. reduction: "mean" over the
-    labelled rows (NaN if there are none), "sum", or "none" for one loss a
-    row. A label outside the vocabulary makes its row's loss and gradient NaN.
-    Logits of -inf (vocabulary shut off) have probability and gradient 0.
-
-    On the GPU: float32, bfloat16 or float16 logits, in rows of any distance
-    and alignment; the sums are fp32 and over rows fp64."""
-    from .training import cross_entropy as impl
-
-    return impl(logits, targets, ignore_index, reduction)
-
-
-def grad_norm(parameters) -> torch.Tensor:
-    """2-norm of all parameters' gradients together (fp32 scalar on their
-    device); parameters without a gradient are passed over."""
-    from .training import grad_norm as impl
-
-    return impl(parameters)
-
-
-def clip_grad_norm_(parameters, max_norm: float,
-                    error_if_nonfinite: bool = False) -> torch.Tensor:
-    """Scales all parameters' gradients in place by
-    min(1, max_norm / (norm + 1e-6)) and returns their norm before that (fp32
-    scalar on their device).
-
-    On the GPU: any mix of float32, bfloat16 and float16 gradients of any
-    sizes, strides and alignment on one device; two that share memory are
-    refused. The norm is summed in fp64. The host waits for nothing (so it can
-    be captured into a graph) unless error_if_nonfinite is set, which raises
-    for a norm that is not finite and leaves the gradients as they were."""
-    from .training import clip_grad_norm_ as impl
-
-    return impl(parameters, max_norm, error_if_nonfinite)
-
-
 def store_kv(k, v, k_cache, v_cache, slot_mapping):
     if _on_gpu(k):
         _get_ext().store_kv(k.contiguous(), v.contiguous(), k_cache, v_cache,
@@ -373,3 +306,12 @@ def _batch_idx_from_starts(seq_starts: torch.Tensor, T: int) -> torch.Tensor:
     for b in range(len(starts) - 1):
         idx[starts[b]:starts[b + 1]] = b
     return idx.to(seq_starts.device)
+
+
+# training ops: packed attention with gradients, cross-entropy, gradient norm
+from .training import (  # noqa: E402
+    clip_grad_norm_,
+    cross_entropy,
+    grad_norm,
+    packed_attention,
+)

@@ -6,6 +6,7 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <algorithm>
 #include <cmath>
@@ -48,7 +49,26 @@ void launched(int code, const char* what) {
     TORCH_CHECK(code == 0, what, ": the launch failed with HIP error ", code);
 }
 
+// What a backward pass returns: without a gradient of its own, and with an
+// error where somebody asks for one (create_graph).
+std::vector<Tensor> once(std::vector<Tensor> grads, const char* what) {
+    if (!torch::GradMode::is_enabled()) return grads;
+    for (Tensor& g : grads)
+        if (g.defined()) g = g.detach().requires_grad_();
+    const auto error = std::make_shared<torch::autograd::DelayedError>(
+        std::string(what) + " has no second derivative", (int)grads.size());
+    return (*error)(std::move(grads));
+}
+
 // ------------------------------------------------------------ packed attention
+
+// t, or a dense copy where its head rows are not dense at 16-byte boundaries
+Tensor rows16(const Tensor& t) {
+    if (t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+        (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0)
+        return t;
+    return t.clone(at::MemoryFormat::Contiguous);
+}
 
 void check_rows(const Tensor& t, const char* name, const Tensor& like) {
     TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device());
@@ -107,9 +127,10 @@ std::vector<Tensor> packed_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor starts,
     return {out, lse, tiles};
 }
 
-// -> dq, dk, dv
+// -> dq, dk, dv (the last two undefined without `keys`)
 std::vector<Tensor> packed_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out,
-                                    Tensor lse, Tensor tiles, double scale) {
+                                    Tensor lse, Tensor tiles, double scale,
+                                    bool keys) {
     const Sizes s = check_qkv(q, k, v);
     check_rows(dout, "the gradient", q);
     TORCH_CHECK(dout.sizes() == q.sizes(), "the gradient must have the shape of q");
@@ -117,7 +138,11 @@ std::vector<Tensor> packed_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, T
     const c10::cuda::CUDAGuard guard(q.device());
     const auto opt = q.options();
     Tensor dq = torch::empty({s.T, s.Hq, s.D}, opt);
-    Tensor dk = torch::empty({s.T, s.Hk, s.D}, opt), dv = torch::empty_like(dk);
+    Tensor dk, dv;
+    if (keys) {
+        dk = torch::empty({s.T, s.Hk, s.D}, opt);
+        dv = torch::empty_like(dk);
+    }
     Tensor delta = torch::empty_like(lse);
     if (s.T > 0) {
         void* st = stream_of(q);
@@ -128,15 +153,45 @@ std::vector<Tensor> packed_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, T
                      tiles.data_ptr(), (int)max_tiles, lse.data_ptr(), delta.data_ptr(),
                      dq.data_ptr(), s.T, s.Hq, s.Hk, s.D, (float)scale, st),
                  "packed_attention's gradient");
-        launched(launch_packed_attn_dkv(
-                     q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
-                     k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), dout.data_ptr(),
-                     dout.stride(0), dout.stride(1), tiles.data_ptr(), (int)max_tiles,
-                     lse.data_ptr(), delta.data_ptr(), dk.data_ptr(), dv.data_ptr(), s.T, s.Hq,
-                     s.Hk, s.D, (float)scale, st),
-                 "packed_attention's gradient");
+        if (keys)
+            launched(launch_packed_attn_dkv(
+                         q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
+                         k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), dout.data_ptr(),
+                         dout.stride(0), dout.stride(1), tiles.data_ptr(), (int)max_tiles,
+                         lse.data_ptr(), delta.data_ptr(), dk.data_ptr(), dv.data_ptr(), s.T,
+                         s.Hq, s.Hk, s.D, (float)scale, st),
+                     "packed_attention's gradient");
     }
     return {dq, dk, dv};
+}
+
+struct PackedAttention : torch::autograd::Function<PackedAttention> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q0,
+                          const Tensor& k0, const Tensor& v0, const Tensor& starts,
+                          double scale) {
+        const Tensor q = rows16(q0), k = rows16(k0), v = rows16(v0);
+        const auto got = packed_attn_fwd(q, k, v, starts, scale, true);
+        ctx->save_for_backward({q, k, v, got[0], got[1], got[2]});
+        ctx->saved_data["scale"] = scale;
+        return got[0];
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list g) {
+        const auto s = ctx->get_saved_variables();
+        auto d = packed_attn_bwd(rows16(g[0]), s[0], s[1], s[2], s[3], s[4], s[5],
+                                 ctx->saved_data["scale"].toDouble(),
+                                 ctx->needs_input_grad(1) || ctx->needs_input_grad(2));
+        d = once(std::move(d), "packed_attention");
+        return {d[0], d[1], d[2], Tensor(), Tensor()};
+    }
+};
+
+Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v,
+                        const Tensor& starts, double scale) {
+    if (torch::GradMode::is_enabled() &&
+        (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+        return PackedAttention::apply(q, k, v, starts, scale);
+    return packed_attn_fwd(rows16(q), rows16(k), rows16(v), starts, scale, false)[0];
 }
 
 // --------------------------------------------------------------- cross-entropy
@@ -183,7 +238,7 @@ std::vector<Tensor> xent_fwd(Tensor x, Tensor targets, int64_t ignore, int64_t m
 }
 
 Tensor xent_bwd(Tensor gout, Tensor x, Tensor targets, int64_t ignore, Tensor stats,
-                c10::optional<Tensor> factor) {
+                const Tensor& factor) {
     check_logits(x, targets);
     const int kind = kind_of(x, "logits");
     const int N = (int)x.size(0), V = (int)x.size(1);
@@ -203,10 +258,34 @@ Tensor xent_bwd(Tensor gout, Tensor x, Tensor targets, int64_t ignore, Tensor st
         launched(launch_xent_bwd(kind, x.data_ptr(), x.stride(0), targets.data_ptr(), ignore, N,
                                  V, stats.data_ptr(), gout.data_ptr(),
                                  gout.dim() ? gout.stride(0) : 0,
-                                 factor ? factor->data_ptr() : nullptr,
+                                 factor.defined() ? factor.data_ptr() : nullptr,
                                  dx.data_ptr(), V, stream_of(x)),
                  "cross_entropy's gradient");
     return dx;
+}
+
+struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x,
+                          const Tensor& targets, int64_t ignore, int64_t mode) {
+        const auto got = xent_fwd(x, targets, ignore, mode, true);
+        ctx->save_for_backward({x, targets, got[1], mode ? got[3] : Tensor()});
+        ctx->saved_data["ignore"] = ignore;
+        return mode ? got[2] : got[0];
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list g) {
+        const auto s = ctx->get_saved_variables();
+        const auto d = once({xent_bwd(g[0], s[0], s[1], ctx->saved_data["ignore"].toInt(), s[2],
+                                      s[3])},
+                            "cross_entropy");
+        return {d[0], Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor cross_entropy(const Tensor& x, const Tensor& targets, int64_t ignore, int64_t mode) {
+    if (torch::GradMode::is_enabled() && x.requires_grad())
+        return CrossEntropy::apply(x, targets, ignore, mode);
+    return xent_fwd(x, targets, ignore, mode, false)[mode ? 2 : 0];
 }
 
 // --------------------------------------------------------------- gradient norm
@@ -341,10 +420,9 @@ Tensor grad_clip(std::vector<Tensor> grads, double limit, double eps) {
 }  // namespace
 
 void bind_training(pybind11::module_& m) {
-    m.def("packed_attn_fwd", &packed_attn_fwd, "causal attention of packed sequences");
-    m.def("packed_attn_bwd", &packed_attn_bwd, "its gradients");
-    m.def("xent_fwd", &xent_fwd, "cross-entropy of rows with labels");
-    m.def("xent_bwd", &xent_bwd, "its gradient");
+    m.def("packed_attention", &packed_attention,
+          "causal attention of packed sequences, with gradients");
+    m.def("cross_entropy", &cross_entropy, "cross-entropy of rows with labels, with gradient");
     m.def("grad_norm", &grad_norm, "norm of all gradients together");
     m.def("grad_clip", &grad_clip, "norm of all gradients together, and clipping by it");
 }

@@ -1,6 +1,8 @@
-"""Training ops: argument checks, autograd, dispatch to the HIP kernels.
+"""Training ops: packed attention, cross-entropy, gradient norm and clipping.
 
-The public entry points, with their documentation, are in ops/__init__.py.
+On the GPU the kernels of csrc/packed_attn.hip, cross_entropy.hip and
+grad_norm.hip, whose autograd nodes are in csrc/training.cpp; on the CPU the
+references of reference.py. Arguments are checked here for both.
 """
 from __future__ import annotations
 
@@ -8,41 +10,32 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _get_ext, reference
 
 
 # ---------------------------------------------------------- packed attention
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t, or a dense copy where its rows of a head are not dense at 16-byte
-    boundaries."""
-    if (t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0
-            and t.data_ptr() % 16 == 0):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                     seq_starts: torch.Tensor, scale: Optional[float] = None) -> torch.Tensor:
+    """Causal attention of packed sequences, with gradients for q, k and v.
 
+    q [T, Hq, D], k and v [T, Hk, D] (Hq a multiple of Hk) hold sequences one
+    after another; sequence b has rows seq_starts[b] up to seq_starts[b + 1],
+    which may be none, and each row attends to its own sequence's rows up to
+    itself. Rows in no sequence (a buffer's unused end) get zeros, in the
+    output and in the gradients, whatever they hold. scale defaults to
+    1 / sqrt(D).
 
-class _PackedAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, starts, scale):
-        q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        out, lse, tiles = _get_ext().packed_attn_fwd(q, k, v, starts, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, tiles)
-        ctx.scale = scale
-        return out
+    On the GPU: bfloat16, D 64 or 128. q, k and v may be views (slices of a
+    fused projection, say): rows at 16-byte boundaries are read in place,
+    others are copied first. The starts stay on the device and nothing waits
+    for the host, so forward and backward can be captured into a graph.
+    Starts on the host are checked; starts on the device cannot be without
+    waiting for them: where they fall or leave [0, T], every output and
+    gradient is NaN. A value that is not finite reaches no other sequence.
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, k, v, out, lse, tiles = ctx.saved_tensors
-        dq, dk, dv = _get_ext().packed_attn_bwd(_rows16(dout), q, k, v, out, lse,
-                                                tiles, ctx.scale)
-        return dq, dk, dv, None, None
-
-
-def packed_attention(q, k, v, seq_starts, scale: Optional[float] = None):
+    The training counterpart of prefill_attention, which has no gradients."""
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k and v must be [tokens, heads, head dim]")
     if k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
@@ -70,10 +63,7 @@ def packed_attention(q, k, v, seq_starts, scale: Optional[float] = None):
     if q.shape[2] not in (64, 128):
         raise ValueError(f"on the GPU the head dim must be 64 or 128, not {q.shape[2]}")
     starts = seq_starts.to(device=q.device, dtype=torch.int32).contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _PackedAttention.apply(q, k, v, starts, scale)
-    return _get_ext().packed_attn_fwd(_rows16(q), _rows16(k), _rows16(v), starts, scale,
-                                      False)[0]
+    return _get_ext().packed_attention(q, k, v, starts, scale)
 
 
 # ------------------------------------------------------------- cross-entropy
@@ -81,23 +71,19 @@ def packed_attention(q, k, v, seq_starts, scale: Optional[float] = None):
 _MODES = {"none": 0, "mean": 1, "sum": 2}
 
 
-class _CrossEntropy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets, ignore, mode):
-        got = _get_ext().xent_fwd(logits, targets, ignore, mode, True)
-        ctx.save_for_backward(logits, targets, got[1], *got[3:])
-        ctx.ignore = ignore
-        return got[2] if mode else got[0]
+def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,
+                  reduction: str = "mean") -> torch.Tensor:
+    """Cross-entropy of logits [N, V] with integer labels [N], with its
+    gradient; fp32 result.
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gout):
-        logits, targets, stats, *factor = ctx.saved_tensors
-        return (_get_ext().xent_bwd(gout, logits, targets, ctx.ignore, stats,
-                                    factor[0] if factor else None), None, None, None)
+    Rows labelled ignore_index count for nothing: their loss is 0, their
+    gradient zeros, their logits are not read. reduction: "mean" over the
+    labelled rows (NaN if there are none), "sum", or "none" for one loss a
+    row. A label outside the vocabulary makes its row's loss and gradient NaN.
+    Logits of -inf (vocabulary shut off) have probability and gradient 0.
 
-
-def cross_entropy(logits, targets, ignore_index: int = -100, reduction: str = "mean"):
+    On the GPU: float32, bfloat16 or float16 logits, in rows of any distance
+    and alignment; the sums are fp32 and over rows fp64."""
     if logits.dim() != 2 or logits.shape[1] < 1 or targets.shape != logits.shape[:1]:
         raise ValueError(f"logits must be [rows, vocabulary] with one label a row: logits "
                          f"{tuple(logits.shape)}, targets {tuple(targets.shape)}")
@@ -115,11 +101,7 @@ def cross_entropy(logits, targets, ignore_index: int = -100, reduction: str = "m
                          f"not {logits.dtype}")
     if logits.stride(1) != 1:
         logits = logits.contiguous()
-    mode = _MODES[reduction]
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _CrossEntropy.apply(logits, targets, ignore_index, mode)
-    got = _get_ext().xent_fwd(logits, targets, ignore_index, mode, False)
-    return got[2] if mode else got[0]
+    return _get_ext().cross_entropy(logits, targets, ignore_index, _MODES[reduction])
 
 
 # ------------------------------------------------------------- gradient norm
@@ -143,6 +125,8 @@ def _grads(parameters) -> list[torch.Tensor]:
 
 @torch.no_grad()
 def grad_norm(parameters) -> torch.Tensor:
+    """2-norm of all parameters' gradients together (fp32 scalar on their
+    device); parameters without a gradient are passed over."""
     grads = _grads(parameters)
     if not grads:
         return torch.zeros(())
@@ -152,7 +136,17 @@ def grad_norm(parameters) -> torch.Tensor:
 
 
 @torch.no_grad()
-def clip_grad_norm_(parameters, max_norm: float, error_if_nonfinite: bool = False):
+def clip_grad_norm_(parameters, max_norm: float,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Scales all parameters' gradients in place by
+    min(1, max_norm / (norm + 1e-6)) and returns their norm before that (fp32
+    scalar on their device).
+
+    On the GPU: any mix of float32, bfloat16 and float16 gradients of any
+    sizes, strides and alignment on one device; two that share memory are
+    refused. The norm is summed in fp64. The host waits for nothing (so it can
+    be captured into a graph) unless error_if_nonfinite is set, which raises
+    for a norm that is not finite and leaves the gradients as they were."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative: {max_norm}")

@@ -652,3 +652,29 @@ def test_clip_refuses(device):
         with pytest.raises(ValueError):
             ops.clip_grad_norm_([params[0], host], 1.0)
         assert torch.equal(host.grad, torch.ones(4))
+
+
+@gpu
+def test_second_derivatives_refused_gpu():
+    q, k, v, _ = _inputs([20], (2, 1), 64, device="cuda")
+    q.requires_grad_()
+    out = ops.packed_attention(q, k, v, torch.tensor([0, 20], device="cuda"))
+    dq, = torch.autograd.grad(out.float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        dq.float().sum().backward()
+    x, t = _loss_inputs(4, 9, torch.float32, "cuda")
+    dx, = torch.autograd.grad(ops.cross_entropy(x.requires_grad_(), t), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        dx.sum().backward()
+
+
+@gpu
+def test_attention_gpu_part_of_the_gradients():
+    q, k, v, dout = _inputs([90], (4, 2), 64, device="cuda")
+    starts = torch.tensor([0, 90], device="cuda")
+    want = _attend(q, k, v, dout, starts)[1:]
+    for ask in ([0], [1], [2], [0, 2]):
+        parts = [x.detach().requires_grad_(i in ask) for i, x in enumerate((q, k, v))]
+        out = ops.packed_attention(*parts, starts)
+        got = torch.autograd.grad(out, [parts[i] for i in ask], dout)
+        assert all(torch.equal(g, want[i]) for g, i in zip(got, ask))
