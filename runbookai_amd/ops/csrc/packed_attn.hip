@@ -74,63 +74,100 @@ DEVINL bf16x8_t pack8(const f32x16_t& c, int s) {
     return b;
 }
 
-// LDS tile of rows of D bf16, in 16-byte chunks, chunk c of row r at c ^ f(r).
-// f spreads both kinds of reads over all 64 banks: 16 lanes with the same
-// chunk of 16 rows (16 bytes each), and 32 lanes with 64 bytes of 4 rows each
-// (8 bytes each).
+// LDS tile of rows of D bf16, in 16-byte chunks, chunk c of row r at
+// c ^ turn(r).  This spreads both kinds of reads over all 64 banks: 16 lanes
+// with the same chunk of 16 rows (16 bytes each), and 32 lanes with 64 bytes of
+// 4 rows each (8 bytes each).
 template <int D>
-DEVINL unsigned tile_at(unsigned row, unsigned chunk) {
-    const unsigned f = D == 128 ? ((row & 3u) << 2) | ((row >> 2) & 3u)
-                                : (((row >> 1) & 1u) << 2) | ((row >> 2) & 3u);
-    return row * (D * 2) + ((chunk ^ f) << 4);
+DEVINL unsigned turn(unsigned row) {
+    return D == 128 ? ((row & 3u) << 2) | ((row >> 2) & 3u)
+                    : (((row >> 1) & 1u) << 2) | ((row >> 2) & 3u);
 }
 
-// A fragment of rows row0..row0+31, columns 16 s..16 s+15
+// Where a lane's parts of a tile begin.  `turn` and the position in a row only
+// meet in exclusive-ors, so all fragments are one exclusive-or with a constant
+// away from one address for each kind of read: `rows` for a fragment of rows,
+// `cols` for one of the transpose.  The kernels make these anew every step
+// (`fresh`), or the compiler would keep each fragment's address in a register.
 template <int D>
-DEVINL bf16x8_t rows_frag(const char* tile, int row0, int s, int lane) {
-    return *reinterpret_cast<const bf16x8_t*>(
-        tile + tile_at<D>(row0 + (lane & 31), 2 * s + (lane >> 5)));
+struct Lane {
+    unsigned rows, cols;
+    DEVINL explicit Lane(int lane) {
+        const unsigned r = lane & 31, hi = lane >> 5, i = lane & 15;
+        rows = r * (D * 2) + ((hi ^ turn<D>(r)) << 4);
+        const unsigned c = 4 * hi + (i >> 2);
+        cols = c * (D * 2) + (((2 * ((lane >> 4) & 1) + ((i >> 1) & 1)) ^ turn<D>(c)) << 4) +
+               8 * (i & 1);
+    }
+    DEVINL Lane fresh(unsigned tile) const {
+        Lane l = *this;
+        l.rows += tile;
+        l.cols += tile;
+        asm volatile("" : "+v"(l.rows), "+v"(l.cols));
+        return l;
+    }
+};
+
+// A fragment of 32 rows from `tile`, columns 16 s..16 s+15
+template <int D>
+DEVINL bf16x8_t rows_frag(const char* tile, const Lane<D>& l, int s) {
+    return *reinterpret_cast<const bf16x8_t*>(tile + (l.rows ^ (s << 5)));
 }
 
-// A fragment of the tile's transpose: columns 32 db..32 db+31 as its rows, and
-// the rows row0 + k' (k' as above, slice 0) as its columns
+// A fragment of the transpose: columns 32 db..32 db+31 as its rows, and the
+// rows k' (as above, slice 0) from `tile` as its columns
 template <int D>
-DEVINL bf16x8_t cols_frag(char* tile, int row0, int db, int lane) {
-    const int i = lane & 15;
-    const unsigned row = row0 + 4 * (lane >> 5) + (i >> 2);
-    const unsigned chunk = 4 * db + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1);
-    const unsigned half = 8 * (i & 1);
+DEVINL bf16x8_t cols_frag(char* tile, const Lane<D>& l, int db) {
     union { short4_t h[2]; bf16x8_t v; } u;
     u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_short4_t*)(tile + tile_at<D>(row, chunk) + half));
-    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_short4_t*)(tile + tile_at<D>(row + 8, chunk) + half));
+        (lds_short4_t*)(tile + (l.cols ^ (db << 6))));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(   // 8 rows on
+        (lds_short4_t*)(tile + (l.cols ^ (db << 6) ^ 32) + 16 * D));
     return u.v;
 }
 
-// A 64-row tile on its way through registers; rows at or past `end` are zero.
-template <int D, int THREADS>
-struct Stage {
-    static constexpr int N = 64 * D / 8 / THREADS;
-    bf16x8_t x[N];
-    DEVINL void load(const ushort_t* base, long stride, int row0, int end) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int at = (int)threadIdx.x + i * THREADS;
-            const int row = row0 + at / (D / 8);
-            x[i] = bf16x8_t{};
-            if (row < end)
-                x[i] = *reinterpret_cast<const bf16x8_t*>(base + row * stride + (at % (D / 8)) * 8);
-        }
+// Moves N rows from global memory straight into an LDS tile, 16 bytes a lane,
+// by a workgroup of THREADS.  A wave's lanes fill consecutive chunks, so the
+// order of chunks in a row (`turn`) is made by which chunk a lane reads.  A row
+// past `last` is read as row `last` instead: what it holds has P = 0.  Nothing
+// lands in a register, so the compiler need not know of the load; arrived()
+// waits for it.
+template <int D, int N, int THREADS>
+struct Mover {
+    static constexpr int STEP = THREADS / (D / 8);   // rows that the workgroup moves at a time
+    static_assert(STEP % 16 == 0 && N % STEP == 0, "turn(row + STEP) is turn(row)");
+    unsigned row, chunk, off;
+    long pitch;   // bytes from row to row
+    DEVINL explicit Mover(long stride) {
+        row = threadIdx.x / (D / 8);
+        chunk = ((threadIdx.x % (D / 8)) ^ turn<D>(row)) * 16;
+        pitch = stride * 2;
+        off = row * (unsigned)pitch + chunk;
     }
-    DEVINL void store(char* tile) const {
+    DEVINL void move(const ushort_t* base, int row0, int last, char* tile) const {
+        const char* from = reinterpret_cast<const char*>(base) + row0 * pitch;
+        const unsigned to = (unsigned)(unsigned long)(__attribute__((address_space(3))) char*)tile +
+                            (threadIdx.x & ~63u) * 16;
+        const bool whole = row0 + N - 1 <= last;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int at = (int)threadIdx.x + i * THREADS;
-            *reinterpret_cast<bf16x8_t*>(tile + tile_at<D>(at / (D / 8), at % (D / 8))) = x[i];
+        for (int i = 0; i < N / STEP; ++i) {
+            unsigned at = off;
+            const char* src = from + i * STEP * pitch;
+            if (!whole) {
+                src = from;
+                at = (unsigned)min((int)row + i * STEP, last - row0) * (unsigned)pitch + chunk;
+            }
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                         :
+                         : "s"(__builtin_amdgcn_readfirstlane(to + i * STEP * D * 2)), "v"(at),
+                           "s"(src)
+                         : "memory");
         }
     }
 };
+
+// All of the wave's own moves are in LDS; a barrier must follow.
+DEVINL void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // One row's values as a B fragment set: B[k][c] = x[row of lane c][k]
 template <int D>
@@ -253,7 +290,7 @@ packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
 // A workgroup takes a tile of 128 rows and NH heads of one group, a wave 32 of
 // the rows for all NH heads, so that a key or value fragment read from LDS
 // feeds NH products.  64 keys at a time stand in LDS, the next 64 are on their
-// way in registers meanwhile.
+// way there meanwhile.
 template <int D, int NH, bool SAVE>
 __global__ void __launch_bounds__(256, D == 128 && NH == 2 ? 1 : 2)
 packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
@@ -273,14 +310,18 @@ packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
     const bool real = seq1 > seq0;
     const int kv0 = seq0, kv1 = real ? row1 : seq0;
-    const int lane = threadIdx.x & (WAVE - 1), wid = threadIdx.x / WAVE;
+    const int lane = threadIdx.x & (WAVE - 1);
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int hi = lane >> 5;
     const int wrow = row0 + wid * 32;
     const int row = wrow + (lane & 31);
     const bool mine = row < row1;
     const float c2 = scale * LOG2E;
 
-    __shared__ char k_lds[2][64 * D * 2], v_lds[2][64 * D * 2];
+    // two tiles of keys, two of values
+    constexpr int TILE = 64 * D * 2;
+    __shared__ __attribute__((aligned(256))) char lds[4 * TILE];
+    const Lane<D> lanes(lane);
 
     bf16x8_t qf[NH][D / 16];
     f32x16_t acc[NH][D / 32];
@@ -295,23 +336,22 @@ packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     }
     k += hk * kh;
     v += hk * vh;
-    Stage<D, 256> sk, sv;
+    const Mover<D, 64, 256> mk(kt), mv(vt);
     const int steps = (kv1 - kv0 + 63) / 64;
     if (steps > 0) {
-        sk.load(k, kt, kv0, kv1);
-        sv.load(v, vt, kv0, kv1);
-        sk.store(k_lds[0]);
-        sv.store(v_lds[0]);
-        if (steps > 1) {
-            sk.load(k, kt, kv0 + 64, kv1);
-            sv.load(v, vt, kv0 + 64, kv1);
-        }
+        mk.move(k, kv0, kv1 - 1, lds);
+        mv.move(v, kv0, kv1 - 1, lds + 2 * TILE);
+        arrived();
     }
     __syncthreads();
     const int wave_end = min(wrow + 32, row1);   // keys this wave's rows reach
     for (int it = 0; it < steps; ++it) {
-        char* kl = k_lds[it & 1];
-        char* vl = v_lds[it & 1];
+        const Lane<D> at = lanes.fresh((it & 1) * TILE);
+        if (it + 1 < steps) {
+            // the other buffer was last read before the barrier of the step before
+            mk.move(k, kv0 + (it + 1) * 64, kv1 - 1, lds + ((it + 1) & 1) * TILE);
+            mv.move(v, kv0 + (it + 1) * 64, kv1 - 1, lds + (2 + ((it + 1) & 1)) * TILE);
+        }
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) {
             const int key0 = kv0 + it * 64 + sub * 32;
@@ -321,7 +361,7 @@ packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
             for (int n = 0; n < NH; ++n) s[n] = zero16();
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) {
-                const bf16x8_t kf = rows_frag<D>(kl, sub * 32, d, lane);
+                const bf16x8_t kf = rows_frag<D>(lds + sub * (TILE / 2), at, d);
 #pragma unroll
                 for (int n = 0; n < NH; ++n) s[n] = mfma(kf, qf[n][d], s[n]);
             }
@@ -365,21 +405,13 @@ packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int db = 0; db < D / 32; ++db) {
-                    const bf16x8_t vf = cols_frag<D>(vl, sub * 32 + ks * 16, db, lane);
+                    const bf16x8_t vf = cols_frag<D>(lds + 2 * TILE + (2 * sub + ks) * (TILE / 4), at, db);
 #pragma unroll
                     for (int n = 0; n < NH; ++n) acc[n][db] = mfma(vf, pf[n][ks], acc[n][db]);
                 }
         }
-        if (it + 1 < steps) {
-            // the other buffer was last read before the barrier of the step before
-            sk.store(k_lds[(it + 1) & 1]);
-            sv.store(v_lds[(it + 1) & 1]);
-            if (it + 2 < steps) {
-                sk.load(k, kt, kv0 + (it + 2) * 64, kv1);
-                sv.load(v, vt, kv0 + (it + 2) * 64, kv1);
-            }
-            __syncthreads();
-        }
+        arrived();
+        __syncthreads();
     }
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
@@ -415,14 +447,18 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
     const bool real = seq1 > seq0;
     const int kv0 = seq0, kv1 = real ? row1 : seq0;
-    const int lane = threadIdx.x & (WAVE - 1), wid = threadIdx.x / WAVE;
+    const int lane = threadIdx.x & (WAVE - 1);
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int hi = lane >> 5;
     const int wrow = row0 + wid * 32;
     const int row = wrow + (lane & 31);
     const bool mine = row < row1;
     const float c2 = scale * LOG2E;
 
-    __shared__ char k_lds[2][64 * D * 2], v_lds[2][64 * D * 2];
+    // two tiles of keys, two of values
+    constexpr int TILE = 64 * D * 2;
+    __shared__ __attribute__((aligned(256))) char lds[4 * TILE];
+    const Lane<D> lanes(lane);
 
     bf16x8_t qf[NH][D / 16], of[NH][D / 16];
     f32x16_t acc[NH][D / 32];
@@ -431,12 +467,12 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     for (int n = 0; n < NH; ++n) {
         load_row<D>(qf[n], q + row * qt + (h0 + n) * qh, mine, hi);
         load_row<D>(of[n], dout + row * ot + (h0 + n) * oh, mine, hi);
-        const long at = ((long)row * Hq + h0 + n) * D;
+        const long from = ((long)row * Hq + h0 + n) * D;
         float sum = 0.f;
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
             if (!mine) continue;
-            const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(out + at + s * 16 + hi * 8);
+            const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(out + from + s * 16 + hi * 8);
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum = fmaf((float)of[n][s][j], (float)a[j], sum);
         }
@@ -447,25 +483,23 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     }
     k += hk * kh;
     v += hk * vh;
-    Stage<D, 256> sk, sv;
+    const Mover<D, 64, 256> mk(kt), mv(vt);
     const int steps = (kv1 - kv0 + 63) / 64;
     const int wave_end = min(wrow + 32, row1);
     // One pass over the keys.  Of s and dP, `use` makes what the pass is for.
     auto sweep = [&](auto use) {
         if (steps > 0) {
-            sk.load(k, kt, kv0, kv1);
-            sv.load(v, vt, kv0, kv1);
-            sk.store(k_lds[0]);
-            sv.store(v_lds[0]);
-            if (steps > 1) {
-                sk.load(k, kt, kv0 + 64, kv1);
-                sv.load(v, vt, kv0 + 64, kv1);
-            }
+            mk.move(k, kv0, kv1 - 1, lds);
+            mv.move(v, kv0, kv1 - 1, lds + 2 * TILE);
+            arrived();
         }
         __syncthreads();
         for (int it = 0; it < steps; ++it) {
-            char* kl = k_lds[it & 1];
-            char* vl = v_lds[it & 1];
+            const Lane<D> at = lanes.fresh((it & 1) * TILE);
+            if (it + 1 < steps) {
+                mk.move(k, kv0 + (it + 1) * 64, kv1 - 1, lds + ((it + 1) & 1) * TILE);
+                mv.move(v, kv0 + (it + 1) * 64, kv1 - 1, lds + (2 + ((it + 1) & 1)) * TILE);
+            }
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
                 const int key0 = kv0 + it * 64 + sub * 32;
@@ -475,32 +509,25 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
                 for (int n = 0; n < NH; ++n) s[n] = dp[n] = zero16();
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) {
-                    const bf16x8_t kf = rows_frag<D>(kl, sub * 32, d, lane);
-                    const bf16x8_t vf = rows_frag<D>(vl, sub * 32, d, lane);
+                    const bf16x8_t kf = rows_frag<D>(lds + sub * (TILE / 2), at, d);
+                    const bf16x8_t vf = rows_frag<D>(lds + 2 * TILE + sub * (TILE / 2), at, d);
 #pragma unroll
                     for (int n = 0; n < NH; ++n) {
                         s[n] = mfma(kf, qf[n][d], s[n]);
                         dp[n] = mfma(vf, of[n][d], dp[n]);
                     }
                 }
-                use(s, dp, key0, kl, sub);
+                use(s, dp, key0, at, sub);
             }
-            if (it + 1 < steps) {
-                sk.store(k_lds[(it + 1) & 1]);
-                sv.store(v_lds[(it + 1) & 1]);
-                if (it + 2 < steps) {
-                    sk.load(k, kt, kv0 + (it + 2) * 64, kv1);
-                    sv.load(v, vt, kv0 + (it + 2) * 64, kv1);
-                }
-                __syncthreads();
-            }
+            arrived();
+            __syncthreads();
         }
     };
     if (row0 == seq0) {
         float sum[NH];
 #pragma unroll
         for (int n = 0; n < NH; ++n) sum[n] = 0.f;
-        sweep([&](f32x16_t (&s)[NH], f32x16_t (&dp)[NH], int key0, char*, int) {
+        sweep([&](f32x16_t (&s)[NH], f32x16_t (&dp)[NH], int key0, const Lane<D>&, int) {
 #pragma unroll
             for (int n = 0; n < NH; ++n)
 #pragma unroll
@@ -511,12 +538,12 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
         });
 #pragma unroll
         for (int n = 0; n < NH; ++n) dl[n] = sum[n] + __shfl_xor(sum[n], 32, WAVE);
-        __syncthreads();   // before the second sweep writes over the tiles
     }
 #pragma unroll
     for (int n = 0; n < NH; ++n)
         if (mine && hi == 0) delta[(long)(h0 + n) * T + row] = dl[n];
-    sweep([&](f32x16_t (&s)[NH], f32x16_t (&dp)[NH], int key0, char* kl, int sub) {
+    sweep([&](f32x16_t (&s)[NH], f32x16_t (&dp)[NH], int key0,
+              const Lane<D>& at, int sub) {
         const bool inner = key0 + 31 <= wrow;   // every key open to every row
         bf16x8_t df[NH][2];
 #pragma unroll
@@ -534,7 +561,7 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int db = 0; db < D / 32; ++db) {
-                const bf16x8_t kf = cols_frag<D>(kl, sub * 32 + ks * 16, db, lane);
+                const bf16x8_t kf = cols_frag<D>(lds + (2 * sub + ks) * (TILE / 4), at, db);
 #pragma unroll
                 for (int n = 0; n < NH; ++n) acc[n][db] = mfma(kf, df[n][ks], acc[n][db]);
             }
@@ -548,11 +575,12 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
 
 // ------------------------------------------------------------------- dk, dv
 //
-// A workgroup takes a tile of 128 keys of one kv head, a wave 32 of them, whose
-// k and v stay in registers; the queries of all the group's heads that see the
-// tile pass through LDS, 64 at a time.
-template <int D>
-__global__ void __launch_bounds__(256, D == 128 ? 1 : 2)
+// A workgroup takes KS sets of 32 keys of one kv head (a tile or a half of it);
+// the queries of all the group's heads that see them pass through LDS, QB at a
+// time.  A wave keeps k and v of one set in registers; KS waves share the keys,
+// two such teams the queries, and their sums are joined at the end.
+template <int D, int KS, int QB>
+__global__ void __launch_bounds__(KS * 128, D == 128 ? 2 : 3)
 packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
                        const ushort_t* __restrict__ k, long kt, long kh,
                        const ushort_t* __restrict__ v, long vt, long vh,
@@ -561,109 +589,159 @@ packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
                        const float* __restrict__ lse, const float* __restrict__ delta,
                        ushort_t* __restrict__ dk, ushort_t* __restrict__ dv,
                        int T, int Hq, int Hk, float scale) {
-    const int t = blockIdx.x / Hk;
+    constexpr int PARTS = 4 / KS;
+    const int t = blockIdx.x / (Hk * PARTS);
     if (t >= *count) return;
     const int hk = blockIdx.x % Hk;
     const int group = Hq / Hk;
     const int4_t tile = tiles[t];
-    const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
+    const int row0 = tile[0] + blockIdx.x / Hk % PARTS * (KS * 32);
+    const int row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
+    if (row0 >= row1) return;
     const bool real = seq1 > seq0;
-    const int lane = threadIdx.x & (WAVE - 1), wid = threadIdx.x / WAVE;
+    const int lane = threadIdx.x & (WAVE - 1);
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int hi = lane >> 5;
-    const int wkey = row0 + wid * 32;
+    const int team = wid / KS;
+    const int wkey = row0 + wid % KS * 32;
     const int key = wkey + (lane & 31);
     const bool mine = key < row1;
     const float c2 = scale * LOG2E;
 
-    __shared__ char q_lds[2][64 * D * 2], o_lds[2][64 * D * 2];
-    __shared__ float4_t ls_lds[2][16], dl_lds[2][16];
+    // two tiles of queries, two of their outputs' gradients, log-sums, deltas
+    // negated
+    constexpr int TILE = QB * D * 2;
+    struct __attribute__((aligned(256))) Lds {
+        char x[4 * TILE];
+        float ls[2][QB], dl[2][QB];
+    };
+    __shared__ Lds lds;
+    char* const ql = lds.x;
+    char* const ol = lds.x + 2 * TILE;
+    const Lane<D> lanes(lane);
 
     bf16x8_t kf[D / 16], vf[D / 16];
+    f32x16_t ak[D / 32], av[D / 32];
     load_row<D>(kf, k + key * kt + hk * kh, mine, hi);
     load_row<D>(vf, v + key * vt + hk * vh, mine, hi);
-    f32x16_t ak[D / 32], av[D / 32];
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) ak[db] = av[db] = zero16();
 
-    Stage<D, 256> sq, so;
-    float stat = 0.f;   // threads 0..63: a row's log-sum, 64..127: its delta
-    const int per_head = real ? (seq1 - row0 + 63) / 64 : 0;
-    const int steps = per_head * group;
-    auto load = [&](int it) {
-        const int h = hk * group + it / per_head;
-        const int r0 = row0 + it % per_head * 64;
-        sq.load(q + h * qh, qt, r0, seq1);
-        so.load(dout + h * oh, ot, r0, seq1);
-        const int r = r0 + (threadIdx.x & 63);
-        if (threadIdx.x < 128) {
-            // past the sequence: P = exp2(0 - inf) = 0
-            const bool first = threadIdx.x < 64;
-            stat = first ? INFINITY : 0.f;
-            if (r < seq1) stat = (first ? lse : delta)[(long)h * T + r];
+    const Mover<D, QB, KS * 128> mq(qt), mo(ot);
+    // the first QB threads hold a row's log-sum each, the next QB its delta
+    static_assert(QB % 64 == 0 && 2 * QB <= KS * 128, "by wave");
+    constexpr int SW = QB / 64;
+    float stat = 0.f;
+    auto load = [&](int h, int r0, int buf) {
+        mq.move(q + h * qh, r0, seq1 - 1, ql + buf * TILE);
+        mo.move(dout + h * oh, r0, seq1 - 1, ol + buf * TILE);
+        if (wid < 2 * SW) {
+            // past the sequence: P = exp2(s - inf) = 0
+            const int i = wid % SW * 64 + lane;
+            const float* from = (wid < SW ? lse : delta) + (long)h * T + r0;
+            stat = r0 + i < seq1 ? from[i] : wid < SW ? INFINITY : 0.f;
         }
     };
     auto store = [&](int buf) {
-        sq.store(q_lds[buf]);
-        so.store(o_lds[buf]);
-        if (threadIdx.x < 64) reinterpret_cast<float*>(ls_lds[buf])[threadIdx.x] = stat;
-        else if (threadIdx.x < 128) reinterpret_cast<float*>(dl_lds[buf])[threadIdx.x - 64] = stat;
+        if (wid < SW) lds.ls[buf][wid * 64 + lane] = stat;
+        else if (wid < 2 * SW) lds.dl[buf][(wid - SW) * 64 + lane] = -stat;
+        arrived();
     };
-    if (steps > 0) {
-        load(0);
+    int h = hk * group, r0 = row0, left = real ? (seq1 - row0 + QB - 1) / QB * group : 0;
+    if (left > 0) {
+        load(h, r0, 0);
         store(0);
-        if (steps > 1) load(1);
     }
     __syncthreads();
-    for (int it = 0; it < steps; ++it) {
-        const int buf = it & 1;
-        char* ql = q_lds[buf];
-        char* ol = o_lds[buf];
-        const int r0 = row0 + it % per_head * 64;
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-            const int first = r0 + sub * 32;
+    for (int buf = 0; left > 0; buf ^= 1) {
+        const int now = r0;
+        r0 += QB;
+        if (r0 >= seq1) {
+            r0 = row0;
+            ++h;
+        }
+        if (--left > 0) load(h, r0, buf ^ 1);   // last read before the barrier of the step before
+#pragma unroll 1
+        for (int sub = 0; sub < QB / 64; ++sub) {
+            const int in = (team * (QB / 64) + sub) * 32;   // first row in the tile
+            const int first = now + in;
             // queries all before the wave's keys, or past the sequence
             if (first + 31 < wkey || first >= seq1) continue;
-            f32x16_t s = zero16(), dp = zero16();
+            const Lane<D> at = lanes.fresh(buf * TILE + in * (D * 2));
+            f32x16_t s = zero16(), dp;
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-                s = mfma(rows_frag<D>(ql, sub * 32, d, lane), kf[d], s);
-                dp = mfma(rows_frag<D>(ol, sub * 32, d, lane), vf[d], dp);
-            }
-            const bool inner = first >= wkey + 31;
+            for (int d = 0; d < D / 16; ++d)
+                s = mfma(rows_frag<D>(ql, at, d), kf[d], s);
+            // dP - delta, summed onto the deltas
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const float4_t ls = ls_lds[buf][sub * 8 + 2 * g + hi];
-                const float4_t dl = dl_lds[buf][sub * 8 + 2 * g + hi];
+                const float4_t dl = *reinterpret_cast<const float4_t*>(
+                    &lds.dl[buf][in + 8 * g + 4 * hi]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = 4 * g + j;
-                    const float p = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -ls[j]));
-                    const bool open = inner || first + crow(r, hi) >= key;
-                    dp[r] = open ? p * (dp[r] - dl[j]) : 0.f;
-                    s[r] = open ? p : 0.f;
-                }
+                for (int j = 0; j < 4; ++j) dp[4 * g + j] = dl[j];
+            }
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d)
+                dp = mfma(rows_frag<D>(ol, at, d), vf[d], dp);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4_t ls = *reinterpret_cast<const float4_t*>(
+                    &lds.ls[buf][in + 8 * g + 4 * hi]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    s[4 * g + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + j], c2, -ls[j]));
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] *= s[r];
+            if (first < wkey + 31) {   // some do not see some
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (first + crow(r, hi) < key) s[r] = dp[r] = 0.f;
             }
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                const bf16x8_t pf = pack8(s, ks), df = pack8(dp, ks);
+                const bf16x8_t pf = pack8(s, ks);
 #pragma unroll
-                for (int db = 0; db < D / 32; ++db) {
-                    av[db] = mfma(cols_frag<D>(ol, sub * 32 + ks * 16, db, lane), pf, av[db]);
-                    ak[db] = mfma(cols_frag<D>(ql, sub * 32 + ks * 16, db, lane), df, ak[db]);
-                }
+                for (int db = 0; db < D / 32; ++db)
+                    av[db] = mfma(cols_frag<D>(ol + ks * (32 * D), at, db), pf,
+                                  av[db]);
+            }
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const bf16x8_t df = pack8(dp, ks);
+#pragma unroll
+                for (int db = 0; db < D / 32; ++db)
+                    ak[db] = mfma(cols_frag<D>(ql + ks * (32 * D), at, db), df,
+                                  ak[db]);
             }
         }
-        if (it + 1 < steps) {
-            store(buf ^ 1);
-            if (it + 2 < steps) load(it + 2);
-            __syncthreads();
-        }
+        if (left > 0) store(buf ^ 1);
+        __syncthreads();
     }
-    if (mine) {
-        const long at = ((long)key * Hk + hk) * D;
-        store_row<D>(ak, seq1 < 0 ? NAN : scale, dk + at, hi);
-        store_row<D>(av, seq1 < 0 ? NAN : 1.f, dv + at, hi);
+    // the second team's dv to the first, the first team's dk to the second
+    float* join = reinterpret_cast<float*>(lds.x) + wid % KS * 32 * D + lane;
+    auto put = [&](const f32x16_t (&a)[D / 32], float* to) {
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) to[(db * 16 + r) * 64] = a[db][r];
+    };
+    auto add = [&](f32x16_t (&a)[D / 32], const float* from) {
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) a[db][r] += from[(db * 16 + r) * 64];
+    };
+    if (team) put(av, join);
+    else put(ak, join + KS * 32 * D);
+    __syncthreads();
+    const long to = ((long)key * Hk + hk) * D;
+    if (team) {
+        add(ak, join + KS * 32 * D);
+        if (mine) store_row<D>(ak, seq1 < 0 ? NAN : scale, dk + to, hi);
+    } else {
+        add(av, join);
+        if (mine) store_row<D>(av, seq1 < 0 ? NAN : 1.f, dv + to, hi);
     }
 }
 
@@ -709,14 +787,14 @@ void dq_(const void* q, long qt, long qh, const void* k, long kt, long kh,
                        (float*)delta, (ushort_t*)dq, T, Hq, Hk, scale);
 }
 
-template <int D>
+template <int D, int KS, int QB>
 void dkv(const void* q, long qt, long qh, const void* k, long kt, long kh,
          const void* v, long vt, long vh, const void* dout, long ot, long oh,
          const void* tiles, int max_tiles, const void* lse, const void* delta,
          void* dk, void* dv, int T, int Hq, int Hk, float scale, hipStream_t st) {
     const int4_t* a = (const int4_t*)tiles;
-    hipLaunchKernelGGL((packed_attn_dkv_kernel<D>), dim3((unsigned)max_tiles * Hk),
-                       dim3(256), 0, st,
+    hipLaunchKernelGGL((packed_attn_dkv_kernel<D, KS, QB>),
+                       dim3((unsigned)max_tiles * Hk * (4 / KS)), dim3(KS * 128), 0, st,
                        (const ushort_t*)q, qt, qh, (const ushort_t*)k, kt, kh,
                        (const ushort_t*)v, vt, vh, (const ushort_t*)dout, ot, oh,
                        a + max_tiles, (const int*)(a + 2 * (long)max_tiles),
@@ -773,10 +851,10 @@ extern "C" int launch_packed_attn_dkv(const void* q, long qt, long qh, const voi
                                       void* dk, void* dv, int T, int Hq, int Hk, int D,
                                       float scale, void* stream) {
     if (D == 128)
-        dkv<128>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, tiles, max_tiles, lse,
+        dkv<128, 4, 128>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, tiles, max_tiles, lse,
                  delta, dk, dv, T, Hq, Hk, scale, (hipStream_t)stream);
     else
-        dkv<64>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, tiles, max_tiles, lse,
+        dkv<64, 2, 64>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, tiles, max_tiles, lse,
                 delta, dk, dv, T, Hq, Hk, scale, (hipStream_t)stream);
     return (int)hipGetLastError();
 }

@@ -62,22 +62,22 @@ std::vector<Tensor> once(std::vector<Tensor> grads, const char* what) {
 
 // ------------------------------------------------------------ packed attention
 
-// t, or a dense copy where its head rows are not dense at 16-byte boundaries
+// What the kernels take: head rows that are dense, at 16-byte boundaries, and
+// close enough for 32-bit offsets within a tile.
+bool fits(const Tensor& t) {
+    return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+           t.stride(0) < (1L << 23) && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+}
+
 Tensor rows16(const Tensor& t) {
-    if (t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
-        (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0)
-        return t;
-    return t.clone(at::MemoryFormat::Contiguous);
+    return fits(t) ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 void check_rows(const Tensor& t, const char* name, const Tensor& like) {
     TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device());
     TORCH_CHECK(t.scalar_type() == torch::kBFloat16, name, " must be bfloat16");
     TORCH_CHECK(t.dim() == 3, name, " must have 3 dimensions: tokens, heads, head dim");
-    TORCH_CHECK(t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
-                    t.stride(0) >= 0 && t.stride(1) >= 0 &&
-                    (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0,
-                name, " must have dense head rows at 16-byte boundaries");
+    TORCH_CHECK(fits(t), name, " has too many or too wide heads");
 }
 
 long tiles_for(long T, long B) { return T / 128 + B + 2; }
@@ -107,7 +107,7 @@ std::vector<Tensor> packed_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor starts,
                     starts.is_contiguous() && starts.dim() == 1 && starts.numel() >= 1,
                 "seq_starts must be a dense int32 vector on the device of q");
     const long B = starts.numel() - 1, max_tiles = tiles_for(s.T, B);
-    TORCH_CHECK(max_tiles * s.Hq < (1L << 31), "too many sequences");
+    TORCH_CHECK(2 * max_tiles * s.Hq < (1L << 31), "too many sequences");
     const c10::cuda::CUDAGuard guard(q.device());
     const auto opt = q.options();
     Tensor out = torch::empty({s.T, s.Hq, s.D}, opt), lse;
