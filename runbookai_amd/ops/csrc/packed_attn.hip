@@ -68,10 +68,19 @@ DEVINL int crow(int r, int hi) { return (r & 3) + 8 * (r >> 2) + 4 * hi; }
 
 // Registers 8s..8s+7 of a C fragment, rounded, as the B fragment of slice s.
 DEVINL bf16x8_t pack8(const f32x16_t& c, int s) {
-    bf16x8_t b;
+    union { bf16x2_t h[4]; bf16x8_t v; } u;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = (__bf16)c[8 * s + j];
-    return b;
+    for (int j = 0; j < 4; ++j)
+        u.h[j] = __builtin_convertvector((float2_t{c[8 * s + 2 * j], c[8 * s + 2 * j + 1]}),
+                                         bf16x2_t);
+    return u.v;
+}
+
+// x, for a branch that few waves take and that begins with it: keeps the
+// compiler from making selects of the branch that all waves run.
+DEVINL int seldom(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
 }
 
 // LDS tile of rows of D bf16, in 16-byte chunks, chunk c of row r at
@@ -135,6 +144,7 @@ DEVINL bf16x8_t cols_frag(char* tile, const Lane<D>& l, int db) {
 template <int D, int N, int THREADS>
 struct Mover {
     static constexpr int STEP = THREADS / (D / 8);   // rows that the workgroup moves at a time
+    static constexpr int LOADS = N / STEP;           // that each wave issues for a tile
     static_assert(STEP % 16 == 0 && N % STEP == 0, "turn(row + STEP) is turn(row)");
     unsigned row, chunk, off;
     long pitch;   // bytes from row to row
@@ -150,7 +160,7 @@ struct Mover {
                             (threadIdx.x & ~63u) * 16;
         const bool whole = row0 + N - 1 <= last;
 #pragma unroll
-        for (int i = 0; i < N / STEP; ++i) {
+        for (int i = 0; i < LOADS; ++i) {
             unsigned at = off;
             const char* src = from + i * STEP * pitch;
             if (!whole) {
@@ -166,8 +176,22 @@ struct Mover {
     }
 };
 
-// All of the wave's own moves are in LDS; a barrier must follow.
-DEVINL void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// 64 floats, one a lane: `from[i]` of each lane's own i
+DEVINL void move64(const float* from, int i, const float* to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(
+                       (unsigned)(unsigned long)(__attribute__((address_space(3))) const float*)to)),
+                   "v"(i * 4), "s"(from)
+                 : "memory");
+}
+
+// All of the wave's own moves but its last N are in LDS (loads end in the order
+// of their issue); a barrier must follow.
+template <int N = 0>
+DEVINL void arrived() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
 
 // One row's values as a B fragment set: B[k][c] = x[row of lane c][k]
 template <int D>
@@ -177,6 +201,26 @@ DEVINL void load_row(bf16x8_t (&f)[D / 16], const ushort_t* row, bool real, int 
         f[s] = bf16x8_t{};
         if (real) f[s] = *reinterpret_cast<const bf16x8_t*>(row + s * 16 + hi * 8);
     }
+}
+
+// Waits for the loads of f here.  Otherwise the compiler waits at f's first use
+// in the loop, each time round, and with it for the tiles on their way.
+template <int N>
+DEVINL void settle(bf16x8_t (&f)[N]) {
+#pragma unroll
+    for (int s = 0; s < N; ++s) asm volatile("" : "+v"(f[s]));
+}
+
+// x's sum, or maximum, over a lane and its partner in the other half of the wave
+DEVINL float both_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x),
+                                                    false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+DEVINL float both_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x),
+                                                    false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // Writes a transposed accumulator's column (the lane's row) times `factor`.
@@ -287,25 +331,22 @@ packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
 
 // ------------------------------------------------------------------ forward
 //
-// A workgroup takes a tile of 128 rows and NH heads of one group, a wave 32 of
-// the rows for all NH heads, so that a key or value fragment read from LDS
-// feeds NH products.  64 keys at a time stand in LDS, the next 64 are on their
-// way there meanwhile.
-template <int D, int NH, bool SAVE>
-__global__ void __launch_bounds__(256, D == 128 && NH == 2 ? 1 : 2)
+// A workgroup takes a tile of 128 rows of one head, a wave 32 of the rows.  64
+// keys at a time stand in LDS, the next ones are on their way there meanwhile.
+template <int D, bool SAVE>
+__global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
 packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
                        const ushort_t* __restrict__ k, long kt, long kh,
                        const ushort_t* __restrict__ v, long vt, long vh,
                        const int4_t* __restrict__ tiles, const int* __restrict__ count,
-                       ushort_t* __restrict__ out, float* __restrict__ lse, int T, int Hq, int Hk, float scale) {
-    const int per_tile = Hq / NH;
-    const int t = blockIdx.x / per_tile;
+                       ushort_t* __restrict__ out, float* __restrict__ lse, int T, int Hq,
+                       int Hk, float scale) {
+    const int t = blockIdx.x / Hq;
     if (t >= *count) return;
     // the kv head runs fastest: workgroups go round the 8 XCDs in turn, so with
     // 1, 2, 4 or 8n of them an XCD's L2 sees the same heads' keys every time
-    const int which = blockIdx.x % per_tile;
-    const int hk = which % Hk;
-    const int h0 = hk * (Hq / Hk) + which / Hk * NH;
+    const int hk = blockIdx.x % Hk;
+    const int h = hk * (Hq / Hk) + blockIdx.x % Hq / Hk;
     const int4_t tile = tiles[t];
     const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
     const bool real = seq1 > seq0;
@@ -323,126 +364,102 @@ packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     __shared__ __attribute__((aligned(256))) char lds[4 * TILE];
     const Lane<D> lanes(lane);
 
-    bf16x8_t qf[NH][D / 16];
-    f32x16_t acc[NH][D / 32];
-    float m[NH], l[NH];
+    bf16x8_t qf[D / 16];
+    load_row<D>(qf, q + row * qt + h * qh, mine, hi);
+    settle(qf);
+    f32x16_t acc[D / 32];
 #pragma unroll
-    for (int n = 0; n < NH; ++n) {
-        load_row<D>(qf[n], q + row * qt + (h0 + n) * qh, mine, hi);
-#pragma unroll
-        for (int db = 0; db < D / 32; ++db) acc[n][db] = zero16();
-        m[n] = -INFINITY;
-        l[n] = 0.f;
-    }
+    for (int db = 0; db < D / 32; ++db) acc[db] = zero16();
+    float m = -INFINITY, l = 0.f;
     k += hk * kh;
     v += hk * vh;
     const Mover<D, 64, 256> mk(kt), mv(vt);
     const int steps = (kv1 - kv0 + 63) / 64;
-    if (steps > 0) {
-        mk.move(k, kv0, kv1 - 1, lds);
-        mv.move(v, kv0, kv1 - 1, lds + 2 * TILE);
-        arrived();
-    }
+    auto fetch = [&](int it) {
+        mk.move(k, kv0 + it * 64, kv1 - 1, lds + (it & 1) * TILE);
+        mv.move(v, kv0 + it * 64, kv1 - 1, lds + (2 + (it & 1)) * TILE);
+    };
+    if (steps > 0) fetch(0);
+    arrived();
     __syncthreads();
     const int wave_end = min(wrow + 32, row1);   // keys this wave's rows reach
     for (int it = 0; it < steps; ++it) {
+        // into the tiles that were last read before the barrier of the step before
+        if (it + 1 < steps) fetch(it + 1);
         const Lane<D> at = lanes.fresh((it & 1) * TILE);
-        if (it + 1 < steps) {
-            // the other buffer was last read before the barrier of the step before
-            mk.move(k, kv0 + (it + 1) * 64, kv1 - 1, lds + ((it + 1) & 1) * TILE);
-            mv.move(v, kv0 + (it + 1) * 64, kv1 - 1, lds + (2 + ((it + 1) & 1)) * TILE);
-        }
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) {
             const int key0 = kv0 + it * 64 + sub * 32;
             if (key0 >= wave_end) continue;
-            f32x16_t s[NH];
+            f32x16_t s = zero16();
 #pragma unroll
-            for (int n = 0; n < NH; ++n) s[n] = zero16();
+            for (int d = 0; d < D / 16; ++d)
+                s = mfma(rows_frag<D>(lds + sub * (TILE / 2), at, d), qf[d], s);
+            if (key0 + 31 > wrow) {   // not every key open to every row
+                const int open = seldom(row - key0 - 4 * hi);
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-                const bf16x8_t kf = rows_frag<D>(lds + sub * (TILE / 2), at, d);
-#pragma unroll
-                for (int n = 0; n < NH; ++n) s[n] = mfma(kf, qf[n][d], s[n]);
+                for (int r = 0; r < 16; ++r)
+                    if (crow(r, 0) > open) s[r] = -INFINITY;
             }
-            const bool inner = key0 + 31 <= wrow;   // every key open to every row
-            bf16x8_t pf[NH][2];
+            float top = s[0];
 #pragma unroll
-            for (int n = 0; n < NH; ++n) {
-                if (!inner) {
+            for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+            top = both_max(top) * c2;
+            // the sums follow the maximum only when a row's has grown by over
+            // 2^8: until then P stays below 2^8, which costs no bits
+            if (!__all(top <= m + 8.f)) {
+                const float to = fmaxf(m, top);
+                const float f = to == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to);
+                m = to;
+                l *= f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (key0 + crow(r, hi) > row) s[n][r] = -INFINITY;
-                }
-                float top = s[n][0];
+                for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-                for (int r = 1; r < 16; ++r) top = fmaxf(top, s[n][r]);
-                top = fmaxf(top, __shfl_xor(top, 32, WAVE));
-                // the sums follow the maximum only when a row's has grown by
-                // over 2^8: until then P stays below 2^8, which costs no bits
-                if (!__all(top * c2 <= m[n] + 8.f)) {
-                    const float to = fmaxf(m[n], top * c2);
-                    const float f = to == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - to);
-                    m[n] = to;
-                    l[n] *= f;
-#pragma unroll
-                    for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) acc[n][db][r] *= f;
-                }
-                const float base = m[n] == -INFINITY ? 0.f : m[n];
-                float sum = 0.f;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], c2, -base));
-                    sum += s[n][r];
-                }
-                l[n] += sum;
-                pf[n][0] = pack8(s[n], 0);
-                pf[n][1] = pack8(s[n], 1);
+                    for (int r = 0; r < 16; ++r) acc[db][r] *= f;
             }
+            const float base = m == -INFINITY ? 0.f : m;
+            float sum = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
+            for (int r = 0; r < 16; ++r) {
+                s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -base));
+                sum += s[r];
+            }
+            l += sum;
 #pragma unroll
-                for (int db = 0; db < D / 32; ++db) {
-                    const bf16x8_t vf = cols_frag<D>(lds + 2 * TILE + (2 * sub + ks) * (TILE / 4), at, db);
+            for (int ks = 0; ks < 2; ++ks) {
+                const bf16x8_t pf = pack8(s, ks);
 #pragma unroll
-                    for (int n = 0; n < NH; ++n) acc[n][db] = mfma(vf, pf[n][ks], acc[n][db]);
-                }
+                for (int db = 0; db < D / 32; ++db)
+                    acc[db] = mfma(cols_frag<D>(lds + 2 * TILE + (2 * sub + ks) * (TILE / 4), at,
+                                                db), pf, acc[db]);
+            }
         }
         arrived();
         __syncthreads();
     }
-#pragma unroll
-    for (int n = 0; n < NH; ++n) {
-        const float sum = l[n] + __shfl_xor(l[n], 32, WAVE);
-        if (!mine) continue;
-        const long at = ((long)row * Hq + h0 + n) * D;
-        const float f = seq1 < 0 ? NAN : real ? 1.f / sum : 0.f;
-        store_row<D>(acc[n], f, out + at, hi);
-        if (SAVE && hi == 0)
-            lse[(long)(h0 + n) * T + row] = m[n] + __builtin_amdgcn_logf(sum);
-    }
+    l = both_sum(l);
+    if (!mine) return;
+    store_row<D>(acc, seq1 < 0 ? NAN : real ? 1.f / l : 0.f, out + ((long)row * Hq + h) * D, hi);
+    if (SAVE && hi == 0) lse[(long)h * T + row] = m + __builtin_amdgcn_logf(l);
 }
 
 // ----------------------------------------------------------------------- dq
 //
-// The forward kernel's split.  Also writes delta for the kernel below.
-template <int D, int NH>
-__global__ void __launch_bounds__(256, D == 128 && NH == 2 ? 1 : 2)
+// The forward kernel's split.  Also writes -delta for the kernel below.
+template <int D>
+__global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
 packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
                       const ushort_t* __restrict__ k, long kt, long kh,
                       const ushort_t* __restrict__ v, long vt, long vh,
                       const ushort_t* __restrict__ dout, long ot, long oh,
-                      const ushort_t* __restrict__ out, const int4_t* __restrict__ tiles, const int* __restrict__ count,
-                      const float* __restrict__ lse, float* __restrict__ delta,
-                      ushort_t* __restrict__ dq, int T, int Hq, int Hk, float scale) {
-    const int per_tile = Hq / NH;
-    const int t = blockIdx.x / per_tile;
+                      const ushort_t* __restrict__ out, const int4_t* __restrict__ tiles,
+                      const int* __restrict__ count, const float* __restrict__ lse,
+                      float* __restrict__ delta, ushort_t* __restrict__ dq, int T, int Hq,
+                      int Hk, float scale) {
+    const int t = blockIdx.x / Hq;
     if (t >= *count) return;
-    const int which = blockIdx.x % per_tile;
-    const int hk = which % Hk;
-    const int h0 = hk * (Hq / Hk) + which / Hk * NH;
+    const int hk = blockIdx.x % Hk;
+    const int h = hk * (Hq / Hk) + blockIdx.x % Hq / Hk;
     const int4_t tile = tiles[t];
     const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
     const bool real = seq1 > seq0;
@@ -455,67 +472,56 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     const bool mine = row < row1;
     const float c2 = scale * LOG2E;
 
-    // two tiles of keys, two of values
     constexpr int TILE = 64 * D * 2;
     __shared__ __attribute__((aligned(256))) char lds[4 * TILE];
     const Lane<D> lanes(lane);
 
-    bf16x8_t qf[NH][D / 16], of[NH][D / 16];
-    f32x16_t acc[NH][D / 32];
-    float ls[NH], dl[NH];
+    bf16x8_t qf[D / 16], of[D / 16];
+    load_row<D>(qf, q + row * qt + h * qh, mine, hi);
+    load_row<D>(of, dout + row * ot + h * oh, mine, hi);
+    float ls = mine ? lse[(long)h * T + row] : 0.f;
+    float dl = 0.f;
+    {
+        bf16x8_t o[D / 16];
+        load_row<D>(o, out + ((long)row * Hq + h) * D, mine, hi);
 #pragma unroll
-    for (int n = 0; n < NH; ++n) {
-        load_row<D>(qf[n], q + row * qt + (h0 + n) * qh, mine, hi);
-        load_row<D>(of[n], dout + row * ot + (h0 + n) * oh, mine, hi);
-        const long from = ((long)row * Hq + h0 + n) * D;
-        float sum = 0.f;
+        for (int s = 0; s < D / 16; ++s)
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-            if (!mine) continue;
-            const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(out + from + s * 16 + hi * 8);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum = fmaf((float)of[n][s][j], (float)a[j], sum);
-        }
-        dl[n] = sum + __shfl_xor(sum, 32, WAVE);
-        ls[n] = mine ? lse[(long)(h0 + n) * T + row] : 0.f;
-#pragma unroll
-        for (int db = 0; db < D / 32; ++db) acc[n][db] = zero16();
+            for (int j = 0; j < 8; ++j) dl = fmaf((float)of[s][j], (float)o[s][j], dl);
+        dl = both_sum(dl);
     }
+    settle(qf);
+    settle(of);
+    asm volatile("" : "+v"(ls));
+    f32x16_t acc[D / 32];
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) acc[db] = zero16();
     k += hk * kh;
     v += hk * vh;
     const Mover<D, 64, 256> mk(kt), mv(vt);
     const int steps = (kv1 - kv0 + 63) / 64;
+    auto fetch = [&](int it) {
+        mk.move(k, kv0 + it * 64, kv1 - 1, lds + (it & 1) * TILE);
+        mv.move(v, kv0 + it * 64, kv1 - 1, lds + (2 + (it & 1)) * TILE);
+    };
     const int wave_end = min(wrow + 32, row1);
     // One pass over the keys.  Of s and dP, `use` makes what the pass is for.
     auto sweep = [&](auto use) {
-        if (steps > 0) {
-            mk.move(k, kv0, kv1 - 1, lds);
-            mv.move(v, kv0, kv1 - 1, lds + 2 * TILE);
-            arrived();
-        }
+        if (steps > 0) fetch(0);
+        arrived();
         __syncthreads();
         for (int it = 0; it < steps; ++it) {
+            if (it + 1 < steps) fetch(it + 1);
             const Lane<D> at = lanes.fresh((it & 1) * TILE);
-            if (it + 1 < steps) {
-                mk.move(k, kv0 + (it + 1) * 64, kv1 - 1, lds + ((it + 1) & 1) * TILE);
-                mv.move(v, kv0 + (it + 1) * 64, kv1 - 1, lds + (2 + ((it + 1) & 1)) * TILE);
-            }
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
                 const int key0 = kv0 + it * 64 + sub * 32;
                 if (key0 >= wave_end) continue;
-                f32x16_t s[NH], dp[NH];
-#pragma unroll
-                for (int n = 0; n < NH; ++n) s[n] = dp[n] = zero16();
+                f32x16_t s = zero16(), dp = zero16();
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) {
-                    const bf16x8_t kf = rows_frag<D>(lds + sub * (TILE / 2), at, d);
-                    const bf16x8_t vf = rows_frag<D>(lds + 2 * TILE + sub * (TILE / 2), at, d);
-#pragma unroll
-                    for (int n = 0; n < NH; ++n) {
-                        s[n] = mfma(kf, qf[n][d], s[n]);
-                        dp[n] = mfma(vf, of[n][d], dp[n]);
-                    }
+                    s = mfma(rows_frag<D>(lds + sub * (TILE / 2), at, d), qf[d], s);
+                    dp = mfma(rows_frag<D>(lds + 2 * TILE + sub * (TILE / 2), at, d), of[d], dp);
                 }
                 use(s, dp, key0, at, sub);
             }
@@ -524,53 +530,36 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
         }
     };
     if (row0 == seq0) {
-        float sum[NH];
+        float sum = 0.f;
+        sweep([&](f32x16_t& s, f32x16_t& dp, int key0, const Lane<D>&, int) {
 #pragma unroll
-        for (int n = 0; n < NH; ++n) sum[n] = 0.f;
-        sweep([&](f32x16_t (&s)[NH], f32x16_t (&dp)[NH], int key0, const Lane<D>&, int) {
-#pragma unroll
-            for (int n = 0; n < NH; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (key0 + crow(r, hi) <= row)
-                        sum[n] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[n][r], c2, -ls[n])),
-                                      dp[n][r], sum[n]);
+            for (int r = 0; r < 16; ++r)
+                if (crow(r, 0) <= row - key0 - 4 * hi)
+                    sum = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], c2, -ls)), dp[r], sum);
         });
-#pragma unroll
-        for (int n = 0; n < NH; ++n) dl[n] = sum[n] + __shfl_xor(sum[n], 32, WAVE);
+        dl = both_sum(sum);
     }
+    if (mine && hi == 0) delta[(long)h * T + row] = -dl;
+    sweep([&](f32x16_t& s, f32x16_t& dp, int key0, const Lane<D>& at, int sub) {
 #pragma unroll
-    for (int n = 0; n < NH; ++n)
-        if (mine && hi == 0) delta[(long)(h0 + n) * T + row] = dl[n];
-    sweep([&](f32x16_t (&s)[NH], f32x16_t (&dp)[NH], int key0,
-              const Lane<D>& at, int sub) {
-        const bool inner = key0 + 31 <= wrow;   // every key open to every row
-        bf16x8_t df[NH][2];
+        for (int r = 0; r < 16; ++r)
+            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -ls)) * (dp[r] - dl);
+        if (key0 + 31 > wrow) {   // not every key open to every row
+            const int open = seldom(row - key0 - 4 * hi);
 #pragma unroll
-        for (int n = 0; n < NH; ++n) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[n][r], c2, -ls[n]));
-                const float ds = p * (dp[n][r] - dl[n]);
-                s[n][r] = inner || key0 + crow(r, hi) <= row ? ds : 0.f;
-            }
-            df[n][0] = pack8(s[n], 0);
-            df[n][1] = pack8(s[n], 1);
+            for (int r = 0; r < 16; ++r)
+                if (crow(r, 0) > open) s[r] = 0.f;
         }
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+        for (int ks = 0; ks < 2; ++ks) {
+            const bf16x8_t df = pack8(s, ks);
 #pragma unroll
-            for (int db = 0; db < D / 32; ++db) {
-                const bf16x8_t kf = cols_frag<D>(lds + (2 * sub + ks) * (TILE / 4), at, db);
-#pragma unroll
-                for (int n = 0; n < NH; ++n) acc[n][db] = mfma(kf, df[n][ks], acc[n][db]);
-            }
+            for (int db = 0; db < D / 32; ++db)
+                acc[db] = mfma(cols_frag<D>(lds + (2 * sub + ks) * (TILE / 4), at, db), df,
+                               acc[db]);
+        }
     });
-#pragma unroll
-    for (int n = 0; n < NH; ++n) {
-        if (!mine) continue;
-        store_row<D>(acc[n], seq1 < 0 ? NAN : scale, dq + ((long)row * Hq + h0 + n) * D, hi);
-    }
+    if (mine) store_row<D>(acc, seq1 < 0 ? NAN : scale, dq + ((long)row * Hq + h) * D, hi);
 }
 
 // ------------------------------------------------------------------- dk, dv
@@ -579,7 +568,7 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
 // the queries of all the group's heads that see them pass through LDS, QB at a
 // time.  A wave keeps k and v of one set in registers; KS waves share the keys,
 // two such teams the queries, and their sums are joined at the end.
-template <int D, int KS, int QB>
+template <int D, int KS, int QB, int NBUF>
 __global__ void __launch_bounds__(KS * 128, D == 128 ? 2 : 3)
 packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
                        const ushort_t* __restrict__ k, long kt, long kh,
@@ -608,59 +597,61 @@ packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     const bool mine = key < row1;
     const float c2 = scale * LOG2E;
 
-    // two tiles of queries, two of their outputs' gradients, log-sums, deltas
-    // negated
+    // NBUF tiles of queries, as many of their outputs' gradients, and each row's
+    // log-sum and negated delta
     constexpr int TILE = QB * D * 2;
     struct __attribute__((aligned(256))) Lds {
-        char x[4 * TILE];
-        float ls[2][QB], dl[2][QB];
+        char x[2 * NBUF * TILE];
+        float ls[NBUF][QB], dl[NBUF][QB];
     };
     __shared__ Lds lds;
     char* const ql = lds.x;
-    char* const ol = lds.x + 2 * TILE;
+    char* const ol = lds.x + NBUF * TILE;
     const Lane<D> lanes(lane);
 
     bf16x8_t kf[D / 16], vf[D / 16];
     f32x16_t ak[D / 32], av[D / 32];
     load_row<D>(kf, k + key * kt + hk * kh, mine, hi);
     load_row<D>(vf, v + key * vt + hk * vh, mine, hi);
+    settle(kf);
+    settle(vf);
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) ak[db] = av[db] = zero16();
 
     const Mover<D, QB, KS * 128> mq(qt), mo(ot);
-    // the first QB threads hold a row's log-sum each, the next QB its delta
-    static_assert(QB % 64 == 0 && 2 * QB <= KS * 128, "by wave");
-    constexpr int SW = QB / 64;
-    float stat = 0.f;
-    auto load = [&](int h, int r0, int buf) {
+    // each wave also moves 64 rows' log-sums or deltas (where there are more
+    // waves than parts, two move the same)
+    static_assert(QB % 64 == 0 && KS * 2 % (QB / 32) == 0, "by wave");
+    const int part = wid % (QB / 32) / 2;
+    const bool sums = wid % 2 == 0;
+    auto fetch = [&](int h, int r0, int buf) {
         mq.move(q + h * qh, r0, seq1 - 1, ql + buf * TILE);
         mo.move(dout + h * oh, r0, seq1 - 1, ol + buf * TILE);
-        if (wid < 2 * SW) {
-            // past the sequence: P = exp2(s - inf) = 0
-            const int i = wid % SW * 64 + lane;
-            const float* from = (wid < SW ? lse : delta) + (long)h * T + r0;
-            stat = r0 + i < seq1 ? from[i] : wid < SW ? INFINITY : 0.f;
-        }
+        const float* from = (sums ? lse : delta) + (long)h * T;
+        const float* to = (sums ? lds.ls[buf] : lds.dl[buf]) + part * 64;
+        move64(from, min(r0 + part * 64 + lane, seq1 - 1), to);
     };
-    auto store = [&](int buf) {
-        if (wid < SW) lds.ls[buf][wid * 64 + lane] = stat;
-        else if (wid < 2 * SW) lds.dl[buf][(wid - SW) * 64 + lane] = -stat;
-        arrived();
-    };
-    int h = hk * group, r0 = row0, left = real ? (seq1 - row0 + QB - 1) / QB * group : 0;
-    if (left > 0) {
-        load(h, r0, 0);
-        store(0);
-    }
-    __syncthreads();
-    for (int buf = 0; left > 0; buf ^= 1) {
-        const int now = r0;
+    constexpr int AHEAD = NBUF - 1, LEFT = (NBUF - 2) * (2 * mq.LOADS + 1);
+    const int steps = real ? (seq1 - row0 + QB - 1) / QB * group : 0;
+    int h = hk * group, r0 = row0;     // what is fetched next
+    auto next = [&](int buf) {
+        fetch(h, r0, buf);
         r0 += QB;
         if (r0 >= seq1) {
             r0 = row0;
             ++h;
         }
-        if (--left > 0) load(h, r0, buf ^ 1);   // last read before the barrier of the step before
+    };
+#pragma unroll
+    for (int it = 0; it < AHEAD; ++it)
+        if (it < steps) next(it);
+    if (steps >= AHEAD) arrived<LEFT>();
+    else arrived<0>();
+    __syncthreads();
+    int now = row0;   // first row of the step
+    for (int it = 0, buf = 0; it < steps; ++it, buf = buf + 1 < NBUF ? buf + 1 : 0) {
+        const bool more = it + AHEAD < steps;
+        if (more) next(buf ? buf - 1 : NBUF - 1);
 #pragma unroll 1
         for (int sub = 0; sub < QB / 64; ++sub) {
             const int in = (team * (QB / 64) + sub) * 32;   // first row in the tile
@@ -693,10 +684,12 @@ packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) dp[r] *= s[r];
-            if (first < wkey + 31) {   // some do not see some
+            // some do not see some, or are past the sequence
+            if (first < wkey + 31 || first + 31 >= seq1) {
+                const int lo = seldom(key - first - 4 * hi), hi_ = seq1 - first - 4 * hi;
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (first + crow(r, hi) < key) s[r] = dp[r] = 0.f;
+                    if (crow(r, 0) < lo || crow(r, 0) >= hi_) s[r] = dp[r] = 0.f;
             }
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
@@ -715,7 +708,10 @@ packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
                                   ak[db]);
             }
         }
-        if (left > 0) store(buf ^ 1);
+        now += QB;
+        if (now >= seq1) now = row0;
+        if (more) arrived<LEFT>();
+        else arrived<0>();
         __syncthreads();
     }
     // the second team's dv to the first, the first team's dk to the second
@@ -760,40 +756,40 @@ extern "C" int launch_packed_tiles(const void* starts, int B, int T, int max_til
 
 namespace {
 
-template <int D, int NH, bool SAVE>
+template <int D, bool SAVE>
 void fwd(const void* q, long qt, long qh, const void* k, long kt, long kh,
          const void* v, long vt, long vh, const void* tiles, int max_tiles, void* out,
          void* lse, int T, int Hq, int Hk, float scale, hipStream_t st) {
     const int4_t* a = (const int4_t*)tiles;
-    hipLaunchKernelGGL((packed_attn_fwd_kernel<D, NH, SAVE>),
-                       dim3((unsigned)max_tiles * (Hq / NH)), dim3(256), 0, st,
+    hipLaunchKernelGGL((packed_attn_fwd_kernel<D, SAVE>),
+                       dim3((unsigned)max_tiles * Hq), dim3(256), 0, st,
                        (const ushort_t*)q, qt, qh, (const ushort_t*)k, kt, kh,
                        (const ushort_t*)v, vt, vh, a, (const int*)(a + 2 * (long)max_tiles),
                        (ushort_t*)out, (float*)lse, T, Hq, Hk, scale);
 }
 
-template <int D, int NH>
+template <int D>
 void dq_(const void* q, long qt, long qh, const void* k, long kt, long kh,
          const void* v, long vt, long vh, const void* dout, long ot, long oh,
          const void* out, const void* tiles, int max_tiles,
          const void* lse, void* delta, void* dq, int T, int Hq, int Hk, float scale,
          hipStream_t st) {
     const int4_t* a = (const int4_t*)tiles;
-    hipLaunchKernelGGL((packed_attn_dq_kernel<D, NH>),
-                       dim3((unsigned)max_tiles * (Hq / NH)), dim3(256), 0, st,
+    hipLaunchKernelGGL((packed_attn_dq_kernel<D>),
+                       dim3((unsigned)max_tiles * Hq), dim3(256), 0, st,
                        (const ushort_t*)q, qt, qh, (const ushort_t*)k, kt, kh,
                        (const ushort_t*)v, vt, vh, (const ushort_t*)dout, ot, oh,
                        (const ushort_t*)out, a, (const int*)(a + 2 * (long)max_tiles), (const float*)lse,
                        (float*)delta, (ushort_t*)dq, T, Hq, Hk, scale);
 }
 
-template <int D, int KS, int QB>
+template <int D, int KS, int QB, int NBUF>
 void dkv(const void* q, long qt, long qh, const void* k, long kt, long kh,
          const void* v, long vt, long vh, const void* dout, long ot, long oh,
          const void* tiles, int max_tiles, const void* lse, const void* delta,
          void* dk, void* dv, int T, int Hq, int Hk, float scale, hipStream_t st) {
     const int4_t* a = (const int4_t*)tiles;
-    hipLaunchKernelGGL((packed_attn_dkv_kernel<D, KS, QB>),
+    hipLaunchKernelGGL((packed_attn_dkv_kernel<D, KS, QB, NBUF>),
                        dim3((unsigned)max_tiles * Hk * (4 / KS)), dim3(KS * 128), 0, st,
                        (const ushort_t*)q, qt, qh, (const ushort_t*)k, kt, kh,
                        (const ushort_t*)v, vt, vh, (const ushort_t*)dout, ot, oh,
@@ -809,19 +805,15 @@ extern "C" int launch_packed_attn_fwd(const void* q, long qt, long qh, const voi
                                       long kt, long kh, const void* v, long vt, long vh,
                                       const void* tiles, int max_tiles, void* out,
                                       void* lse, int T, int Hq, int Hk, int D, float scale, void* stream) {
-    const bool pair = Hq / Hk % 2 == 0;
-#define FWD(d, n, s)                                                                   \
-    fwd<d, n, s>(q, qt, qh, k, kt, kh, v, vt, vh, tiles, max_tiles, out, lse, \
-                 T, Hq, Hk, scale, (hipStream_t)stream)
+#define FWD(d, s)                                                                          \
+    fwd<d, s>(q, qt, qh, k, kt, kh, v, vt, vh, tiles, max_tiles, out, lse, T, Hq, Hk, scale, \
+              (hipStream_t)stream)
     if (D == 128) {
-        if (lse) FWD(128, 1, true);
-        else FWD(128, 1, false);
-    } else if (pair) {
-        if (lse) FWD(64, 2, true);
-        else FWD(64, 2, false);
+        if (lse) FWD(128, true);
+        else FWD(128, false);
     } else {
-        if (lse) FWD(64, 1, true);
-        else FWD(64, 1, false);
+        if (lse) FWD(64, true);
+        else FWD(64, false);
     }
 #undef FWD
     return (int)hipGetLastError();
@@ -833,14 +825,12 @@ extern "C" int launch_packed_attn_dq(const void* q, long qt, long qh, const void
                                      const void* tiles, int max_tiles,
                                      const void* lse, void* delta, void* dq, int T, int Hq,
                                      int Hk, int D, float scale, void* stream) {
-    const bool pair = Hq / Hk % 2 == 0;
-#define DQ(d, n)                                                                     \
-    dq_<d, n>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, out, tiles,             \
-              max_tiles, lse, delta, dq, T, Hq, Hk, scale, (hipStream_t)stream)
-    if (D == 128) DQ(128, 1);
-    else if (pair) DQ(64, 2);
-    else DQ(64, 1);
-#undef DQ
+    if (D == 128)
+        dq_<128>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, out, tiles, max_tiles, lse,
+                 delta, dq, T, Hq, Hk, scale, (hipStream_t)stream);
+    else
+        dq_<64>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, out, tiles, max_tiles, lse,
+                delta, dq, T, Hq, Hk, scale, (hipStream_t)stream);
     return (int)hipGetLastError();
 }
 
@@ -851,10 +841,10 @@ extern "C" int launch_packed_attn_dkv(const void* q, long qt, long qh, const voi
                                       void* dk, void* dv, int T, int Hq, int Hk, int D,
                                       float scale, void* stream) {
     if (D == 128)
-        dkv<128, 4, 128>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, tiles, max_tiles, lse,
+        dkv<128, 4, 128, 2>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, tiles, max_tiles, lse,
                  delta, dk, dv, T, Hq, Hk, scale, (hipStream_t)stream);
     else
-        dkv<64, 2, 64>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, tiles, max_tiles, lse,
+        dkv<64, 2, 64, 3>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, tiles, max_tiles, lse,
                 delta, dk, dv, T, Hq, Hk, scale, (hipStream_t)stream);
     return (int)hipGetLastError();
 }
