@@ -247,86 +247,80 @@ DEVINL void store_row(const f32x16_t (&acc)[D / 32], float factor, ushort_t* row
 // rows make tiles with end -1, whose outputs are NaN: no start that a caller
 // passes leads a kernel out of its buffers.  `by_query` has the tiles with the
 // most keys first, `by_key` those with the most queries, so that the longest
-// run first and the short ones fill the gaps.  One workgroup: a pass that
+// run first and the short ones fill the gaps; entries that are left over hold
+// no rows.  One workgroup, a wave a sequence and a lane a tile: a pass that
 // counts tiles by their number in the sequence, a scan, a pass that places
 // them.  (The order within one count is free and changes no result.)
 #define BUCKETS 4096
+#define BUILDERS 1024
 
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(BUILDERS)
 packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
-                    int4_t* __restrict__ by_query, int4_t* __restrict__ by_key,
-                    int* __restrict__ count) {
+                    int4_t* __restrict__ by_query, int4_t* __restrict__ by_key) {
     __shared__ int first[BUCKETS], fill_q[BUCKETS], fill_k[BUCKETS];
-    __shared__ int part[512], total, bad;
+    __shared__ int total;
     const int tid = threadIdx.x;
-    const int lane = tid & (WAVE - 1), wid = tid / WAVE;
     int shift = 0;
     while (((T / ROWS) >> shift) >= BUCKETS) ++shift;
     const int used = ((T / ROWS) >> shift) + 1;
-    if (tid == 0) { total = 0; bad = 0; }
-    for (int i = tid; i < used; i += 512) first[i] = fill_q[i] = fill_k[i] = 0;
-    __syncthreads();
-    for (int b = tid; b <= B; b += 512) {
+    for (int i = tid; i < used; i += BUILDERS) first[i] = fill_q[i] = fill_k[i] = 0;
+    bool bad = false;
+    for (int b = tid; b <= B; b += BUILDERS) {
         const int s = starts[b];
-        if (s < 0 || s > T || (b && s < starts[b - 1])) bad = 1;
+        bad |= s < 0 || s > T || (b && s < starts[b - 1]);
     }
-    __syncthreads();
-    const bool wrong = bad != 0;
-    // sequences -1 and B: the rows before the first and behind the last
-    const int lo = wrong ? B : -1;
-    auto range = [&](int b, int& s, int& e) {
-        s = wrong ? 0 : b < 0 ? 0 : starts[b];
-        e = wrong || b == B ? T : starts[b + 1];
+    const bool wrong = __syncthreads_or(bad);
+    // sequence 0 is the rows before the first one, B + 1 those behind the last
+    const int lane = tid & (WAVE - 1), wid = tid / WAVE;
+    constexpr int WAVES = BUILDERS / WAVE;
+    auto each = [&](auto use) {
+        for (int b0 = wid; b0 < B + 2; b0 += BUILDERS) {
+            // 64 sequences' ranges at once, so that their loads overlap
+            const int b = b0 + lane * WAVES;
+            int s = 0, e = b || !wrong ? 0 : T;
+            if (b < B + 2 && !wrong) {
+                s = b ? starts[b - 1] : 0;
+                e = b <= B ? starts[b] : T;
+            }
+            for (int j = 0; j < WAVE && b0 + j * WAVES < B + 2; ++j) {
+                const int sj = __shfl(s, j, WAVE), ej = __shfl(e, j, WAVE);
+                const int n = (ej - sj + ROWS - 1) / ROWS;
+                for (int i = lane; i < n; i += WAVE) use(b0 + j * WAVES, sj, ej, n, i);
+            }
+        }
     };
-    for (int b = lo + wid; b <= B; b += 512 / WAVE) {
-        int s, e;
-        range(b, s, e);
-        const int n = (e - s + ROWS - 1) / ROWS;
-        for (int i = lane; i < n; i += WAVE) atomicAdd(&first[i >> shift], 1);
-    }
+    each([&](int, int, int, int, int i) { atomicAdd(&first[i >> shift], 1); });
     __syncthreads();
     // first[k] = number of tiles in buckets above k
-    constexpr int PER = BUCKETS / 512;
-    int sum = 0;
-    for (int i = 0; i < PER; ++i) {
-        const int k = tid * PER + i;
-        if (k < used) sum += first[k];
-    }
-    part[tid] = sum;
-    __syncthreads();
-    for (int off = 1; off < 512; off <<= 1) {
-        const int v = tid + off < 512 ? part[tid + off] : 0;
-        __syncthreads();
-        part[tid] += v;
-        __syncthreads();
-    }
-    if (tid == 0) total = part[0];
-    int above = part[tid] - sum;
-    for (int i = PER - 1; i >= 0; --i) {
-        const int k = tid * PER + i;
-        if (k < used) {
-            const int n = first[k];
-            first[k] = above;
-            above += n;
+    if (tid < WAVE) {
+        int above = 0;
+        for (int top = used - 1; top >= 0; top -= WAVE) {
+            const int k = top - tid;
+            const int n = k >= 0 ? first[k] : 0;
+            int sum = n;
+#pragma unroll
+            for (int off = 1; off < WAVE; off <<= 1) {
+                const int v = __shfl_up(sum, off, WAVE);
+                if (tid >= off) sum += v;
+            }
+            if (k >= 0) first[k] = above + sum - n;
+            above += __shfl(sum, WAVE - 1, WAVE);
         }
+        if (tid == 0) total = above;
     }
     __syncthreads();
-    for (int b = lo + wid; b <= B; b += 512 / WAVE) {
-        int s, e;
-        range(b, s, e);
-        const int n = (e - s + ROWS - 1) / ROWS;
-        const bool real = !wrong && b >= 0 && b < B;
-        for (int i = lane; i < n; i += WAVE) {
-            const int r0 = s + i * ROWS;
-            const int4_t t = {r0, min(r0 + ROWS, e), real ? s : r0, real ? e : wrong ? -1 : r0};
-            const int kq = i >> shift, kk = (n - 1 - i) >> shift;
-            const int at_q = first[kq] + atomicAdd(&fill_q[kq], 1);
-            const int at_k = first[kk] + atomicAdd(&fill_k[kk], 1);
-            if (at_q < max_tiles) by_query[at_q] = t;
-            if (at_k < max_tiles) by_key[at_k] = t;
-        }
-    }
-    if (tid == 0) *count = min(total, max_tiles);
+    each([&](int b, int s, int e, int n, int i) {
+        const bool real = !wrong && b > 0 && b <= B;
+        const int r0 = s + i * ROWS;
+        const int4_t t = {r0, min(r0 + ROWS, e), real ? s : r0, real ? e : wrong ? -1 : r0};
+        const int kq = i >> shift, kk = (n - 1 - i) >> shift;
+        const int at_q = first[kq] + atomicAdd(&fill_q[kq], 1);
+        const int at_k = first[kk] + atomicAdd(&fill_k[kk], 1);
+        if (at_q < max_tiles) by_query[at_q] = t;
+        if (at_k < max_tiles) by_key[at_k] = t;
+    });
+    for (int i = total + tid; i < max_tiles; i += BUILDERS)
+        by_query[i] = by_key[i] = int4_t{0, 0, 0, 0};
 }
 
 // ------------------------------------------------------------------ forward
@@ -338,17 +332,15 @@ __global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
 packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
                        const ushort_t* __restrict__ k, long kt, long kh,
                        const ushort_t* __restrict__ v, long vt, long vh,
-                       const int4_t* __restrict__ tiles, const int* __restrict__ count,
-                       ushort_t* __restrict__ out, float* __restrict__ lse, int T, int Hq,
-                       int Hk, float scale) {
-    const int t = blockIdx.x / Hq;
-    if (t >= *count) return;
+                       const int4_t* __restrict__ tiles, ushort_t* __restrict__ out,
+                       float* __restrict__ lse, int T, int Hq, int Hk, float scale) {
+    const int4_t tile = tiles[blockIdx.x / Hq];
+    const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
+    if (row0 >= row1) return;
     // the kv head runs fastest: workgroups go round the 8 XCDs in turn, so with
     // 1, 2, 4 or 8n of them an XCD's L2 sees the same heads' keys every time
     const int hk = blockIdx.x % Hk;
     const int h = hk * (Hq / Hk) + blockIdx.x % Hq / Hk;
-    const int4_t tile = tiles[t];
-    const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
     const bool real = seq1 > seq0;
     const int kv0 = seq0, kv1 = real ? row1 : seq0;
     const int lane = threadIdx.x & (WAVE - 1);
@@ -366,7 +358,6 @@ packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
 
     bf16x8_t qf[D / 16];
     load_row<D>(qf, q + row * qt + h * qh, mine, hi);
-    settle(qf);
     f32x16_t acc[D / 32];
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) acc[db] = zero16();
@@ -380,6 +371,7 @@ packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
         mv.move(v, kv0 + it * 64, kv1 - 1, lds + (2 + (it & 1)) * TILE);
     };
     if (steps > 0) fetch(0);
+    settle(qf);
     arrived();
     __syncthreads();
     const int wave_end = min(wrow + 32, row1);   // keys this wave's rows reach
@@ -453,15 +445,13 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
                       const ushort_t* __restrict__ v, long vt, long vh,
                       const ushort_t* __restrict__ dout, long ot, long oh,
                       const ushort_t* __restrict__ out, const int4_t* __restrict__ tiles,
-                      const int* __restrict__ count, const float* __restrict__ lse,
-                      float* __restrict__ delta, ushort_t* __restrict__ dq, int T, int Hq,
-                      int Hk, float scale) {
-    const int t = blockIdx.x / Hq;
-    if (t >= *count) return;
+                      const float* __restrict__ lse, float* __restrict__ delta,
+                      ushort_t* __restrict__ dq, int T, int Hq, int Hk, float scale) {
+    const int4_t tile = tiles[blockIdx.x / Hq];
+    const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
+    if (row0 >= row1) return;
     const int hk = blockIdx.x % Hk;
     const int h = hk * (Hq / Hk) + blockIdx.x % Hq / Hk;
-    const int4_t tile = tiles[t];
-    const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
     const bool real = seq1 > seq0;
     const int kv0 = seq0, kv1 = real ? row1 : seq0;
     const int lane = threadIdx.x & (WAVE - 1);
@@ -476,6 +466,15 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     __shared__ __attribute__((aligned(256))) char lds[4 * TILE];
     const Lane<D> lanes(lane);
 
+    k += hk * kh;
+    v += hk * vh;
+    const Mover<D, 64, 256> mk(kt), mv(vt);
+    const int steps = (kv1 - kv0 + 63) / 64;
+    auto fetch = [&](int it) {
+        mk.move(k, kv0 + it * 64, kv1 - 1, lds + (it & 1) * TILE);
+        mv.move(v, kv0 + it * 64, kv1 - 1, lds + (2 + (it & 1)) * TILE);
+    };
+    if (steps > 0) fetch(0);
     bf16x8_t qf[D / 16], of[D / 16];
     load_row<D>(qf, q + row * qt + h * qh, mine, hi);
     load_row<D>(of, dout + row * ot + h * oh, mine, hi);
@@ -496,19 +495,10 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     f32x16_t acc[D / 32];
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) acc[db] = zero16();
-    k += hk * kh;
-    v += hk * vh;
-    const Mover<D, 64, 256> mk(kt), mv(vt);
-    const int steps = (kv1 - kv0 + 63) / 64;
-    auto fetch = [&](int it) {
-        mk.move(k, kv0 + it * 64, kv1 - 1, lds + (it & 1) * TILE);
-        mv.move(v, kv0 + it * 64, kv1 - 1, lds + (2 + (it & 1)) * TILE);
-    };
     const int wave_end = min(wrow + 32, row1);
     // One pass over the keys.  Of s and dP, `use` makes what the pass is for.
     auto sweep = [&](auto use) {
-        if (steps > 0) fetch(0);
-        arrived();
+        arrived();   // the first tiles
         __syncthreads();
         for (int it = 0; it < steps; ++it) {
             if (it + 1 < steps) fetch(it + 1);
@@ -538,6 +528,7 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
                     sum = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], c2, -ls)), dp[r], sum);
         });
         dl = both_sum(sum);
+        if (steps > 0) fetch(0);
     }
     if (mine && hi == 0) delta[(long)h * T + row] = -dl;
     sweep([&](f32x16_t& s, f32x16_t& dp, int key0, const Lane<D>& at, int sub) {
@@ -574,16 +565,13 @@ packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
                        const ushort_t* __restrict__ k, long kt, long kh,
                        const ushort_t* __restrict__ v, long vt, long vh,
                        const ushort_t* __restrict__ dout, long ot, long oh,
-                       const int4_t* __restrict__ tiles, const int* __restrict__ count,
-                       const float* __restrict__ lse, const float* __restrict__ delta,
-                       ushort_t* __restrict__ dk, ushort_t* __restrict__ dv,
-                       int T, int Hq, int Hk, float scale) {
+                       const int4_t* __restrict__ tiles, const float* __restrict__ lse,
+                       const float* __restrict__ delta, ushort_t* __restrict__ dk,
+                       ushort_t* __restrict__ dv, int T, int Hq, int Hk, float scale) {
     constexpr int PARTS = 4 / KS;
-    const int t = blockIdx.x / (Hk * PARTS);
-    if (t >= *count) return;
     const int hk = blockIdx.x % Hk;
     const int group = Hq / Hk;
-    const int4_t tile = tiles[t];
+    const int4_t tile = tiles[blockIdx.x / (Hk * PARTS)];
     const int row0 = tile[0] + blockIdx.x / Hk % PARTS * (KS * 32);
     const int row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
     if (row0 >= row1) return;
@@ -613,8 +601,6 @@ packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     f32x16_t ak[D / 32], av[D / 32];
     load_row<D>(kf, k + key * kt + hk * kh, mine, hi);
     load_row<D>(vf, v + key * vt + hk * vh, mine, hi);
-    settle(kf);
-    settle(vf);
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) ak[db] = av[db] = zero16();
 
@@ -645,6 +631,8 @@ packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
 #pragma unroll
     for (int it = 0; it < AHEAD; ++it)
         if (it < steps) next(it);
+    settle(kf);
+    settle(vf);
     if (steps >= AHEAD) arrived<LEFT>();
     else arrived<0>();
     __syncthreads();
@@ -743,14 +731,13 @@ packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
 
 // ---------------------------------------------------------------- launchers
 // Each returns the launch's hipError_t.  `tiles` holds max_tiles tiles by
-// query, as many by key, and the count.
+// query and as many by key.
 
 extern "C" int launch_packed_tiles(const void* starts, int B, int T, int max_tiles,
                                    void* tiles, void* stream) {
     int4_t* a = (int4_t*)tiles;
-    hipLaunchKernelGGL(packed_tiles_kernel, dim3(1), dim3(512), 0, (hipStream_t)stream,
-                       (const int*)starts, B, T, max_tiles, a, a + max_tiles,
-                       (int*)(a + 2 * (long)max_tiles));
+    hipLaunchKernelGGL(packed_tiles_kernel, dim3(1), dim3(BUILDERS), 0, (hipStream_t)stream,
+                       (const int*)starts, B, T, max_tiles, a, a + max_tiles);
     return (int)hipGetLastError();
 }
 
@@ -764,7 +751,7 @@ void fwd(const void* q, long qt, long qh, const void* k, long kt, long kh,
     hipLaunchKernelGGL((packed_attn_fwd_kernel<D, SAVE>),
                        dim3((unsigned)max_tiles * Hq), dim3(256), 0, st,
                        (const ushort_t*)q, qt, qh, (const ushort_t*)k, kt, kh,
-                       (const ushort_t*)v, vt, vh, a, (const int*)(a + 2 * (long)max_tiles),
+                       (const ushort_t*)v, vt, vh, a,
                        (ushort_t*)out, (float*)lse, T, Hq, Hk, scale);
 }
 
@@ -779,7 +766,7 @@ void dq_(const void* q, long qt, long qh, const void* k, long kt, long kh,
                        dim3((unsigned)max_tiles * Hq), dim3(256), 0, st,
                        (const ushort_t*)q, qt, qh, (const ushort_t*)k, kt, kh,
                        (const ushort_t*)v, vt, vh, (const ushort_t*)dout, ot, oh,
-                       (const ushort_t*)out, a, (const int*)(a + 2 * (long)max_tiles), (const float*)lse,
+                       (const ushort_t*)out, a, (const float*)lse,
                        (float*)delta, (ushort_t*)dq, T, Hq, Hk, scale);
 }
 
@@ -793,7 +780,7 @@ void dkv(const void* q, long qt, long qh, const void* k, long kt, long kh,
                        dim3((unsigned)max_tiles * Hk * (4 / KS)), dim3(KS * 128), 0, st,
                        (const ushort_t*)q, qt, qh, (const ushort_t*)k, kt, kh,
                        (const ushort_t*)v, vt, vh, (const ushort_t*)dout, ot, oh,
-                       a + max_tiles, (const int*)(a + 2 * (long)max_tiles),
+                       a + max_tiles,
                        (const float*)lse, (const float*)delta, (ushort_t*)dk,
                        (ushort_t*)dv, T, Hq, Hk, scale);
 }

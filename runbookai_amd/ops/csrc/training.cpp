@@ -111,7 +111,7 @@ std::vector<Tensor> packed_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor starts,
     const c10::cuda::CUDAGuard guard(q.device());
     const auto opt = q.options();
     Tensor out = torch::empty({s.T, s.Hq, s.D}, opt), lse;
-    Tensor tiles = torch::empty({8 * max_tiles + 4}, opt.dtype(torch::kInt32));
+    Tensor tiles = torch::empty({8 * max_tiles}, opt.dtype(torch::kInt32));
     if (save) lse = torch::empty({s.Hq, s.T}, opt.dtype(torch::kFloat32));
     if (s.T > 0) {
         void* st = stream_of(q);
@@ -134,7 +134,7 @@ std::vector<Tensor> packed_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, T
     const Sizes s = check_qkv(q, k, v);
     check_rows(dout, "the gradient", q);
     TORCH_CHECK(dout.sizes() == q.sizes(), "the gradient must have the shape of q");
-    const long max_tiles = (tiles.numel() - 4) / 8;
+    const long max_tiles = tiles.numel() / 8;
     const c10::cuda::CUDAGuard guard(q.device());
     const auto opt = q.options();
     Tensor dq = torch::empty({s.T, s.Hq, s.D}, opt);
