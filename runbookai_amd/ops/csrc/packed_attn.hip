@@ -31,16 +31,16 @@
 //
 // Precision: scores, statistics, delta and all sums are fp32; P and dS are
 // rounded to bf16 as operands of a product, which bf16 inputs ask for anyway.
-// delta_i = do_i.o_i is off by about 2^-9 |do| |o| from the roundings in o.
-// Where a row has n open places, |o| falls as 1/sqrt(n) and the error in dq as
-// 1/sqrt(n) of dq's own rounding: nothing, but for the first rows of a
-// sequence, where dP - delta cancels.  The first tile of each sequence
-// therefore takes delta_i = sum_j P_ij dP_ij in fp32, by a sweep of its own
-// over its (at most 128) keys.
+// delta_i = do_i.o_i inherits o's errors, and where dP - delta cancels (rows
+// that attend to few places) they show in dq and dk.  So the forward pass also
+// keeps what o's rounding left over (out_lo, as bf16), which takes the rounding
+// out of delta; and the first tile of each sequence, whose rows have few places
+// to attend to, takes delta_i = sum_j P_ij dP_ij in fp32, by a sweep of its own
+// over its (at most 128) keys.  Of the policy's batch, dq is then 1.45 times as
+// far from exact as its own rounding alone; from the rounded o it was 1.50.
 #include "common.h"
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
@@ -223,17 +223,40 @@ DEVINL float both_max(float x) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// Writes a transposed accumulator's column (the lane's row) times `factor`.
+// Writes a transposed accumulator's column (the lane's row) times `factor`;
+// `rest` (may be null) gets what the rounding to bf16 left over.  A lane and its
+// partner hold 4 elements each of every 8: they swap halves of two groups, so
+// that each writes 16 bytes of one.
 template <int D>
-DEVINL void store_row(const f32x16_t (&acc)[D / 32], float factor, ushort_t* row, int hi) {
+DEVINL void store_row(const f32x16_t (&acc)[D / 32], float factor, ushort_t* row, int hi,
+                      ushort_t* rest, bool mine) {
+    union Pair { bf16x2_t h; unsigned u; };
+    typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
+    auto join = [](Pair a0, Pair a1, Pair b0, Pair b1) {
+        const auto r0 = __builtin_amdgcn_permlane32_swap(a0.u, b0.u, false, false);
+        const auto r1 = __builtin_amdgcn_permlane32_swap(a1.u, b1.u, false, false);
+        return uint4_t{r0[0], r1[0], r0[1], r1[1]};
+    };
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            bf16x4_t x;
+        for (int g = 0; g < 4; g += 2) {
+            Pair x[4], y[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = (__bf16)(acc[db][4 * g + j] * factor);
-            *reinterpret_cast<bf16x4_t*>(row + db * 32 + 8 * g + 4 * hi) = x;
+            for (int i = 0; i < 4; ++i) {
+                const float2_t v = {acc[db][4 * g + 2 * i] * factor,
+                                    acc[db][4 * g + 2 * i + 1] * factor};
+                x[i].h = __builtin_convertvector(v, bf16x2_t);
+                const float2_t left = {v[0] - (float)x[i].h[0], v[1] - (float)x[i].h[1]};
+                y[i].h = __builtin_convertvector(left, bf16x2_t);
+            }
+            const int at = db * 32 + 8 * (g + hi);
+            const uint4_t a = join(x[0], x[1], x[2], x[3]);
+            if (mine) *reinterpret_cast<uint4_t*>(row + at) = a;
+            if (rest) {
+                const uint4_t b = join(y[0], y[1], y[2], y[3]);
+                if (mine) *reinterpret_cast<uint4_t*>(rest + at) = b;
+            }
         }
 }
 
@@ -333,7 +356,8 @@ packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
                        const ushort_t* __restrict__ k, long kt, long kh,
                        const ushort_t* __restrict__ v, long vt, long vh,
                        const int4_t* __restrict__ tiles, ushort_t* __restrict__ out,
-                       float* __restrict__ lse, int T, int Hq, int Hk, float scale) {
+                       ushort_t* __restrict__ out_lo, float* __restrict__ lse, int T, int Hq,
+                       int Hk, float scale) {
     const int4_t tile = tiles[blockIdx.x / Hq];
     const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
     if (row0 >= row1) return;
@@ -430,9 +454,10 @@ packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
         __syncthreads();
     }
     l = both_sum(l);
-    if (!mine) return;
-    store_row<D>(acc, seq1 < 0 ? NAN : real ? 1.f / l : 0.f, out + ((long)row * Hq + h) * D, hi);
-    if (SAVE && hi == 0) lse[(long)h * T + row] = m + __builtin_amdgcn_logf(l);
+    const long to = ((long)row * Hq + h) * D;
+    store_row<D>(acc, seq1 < 0 ? NAN : real ? 1.f / l : 0.f, out + to, hi,
+                 SAVE ? out_lo + to : nullptr, mine);
+    if (SAVE && mine && hi == 0) lse[(long)h * T + row] = m + __builtin_amdgcn_logf(l);
 }
 
 // ----------------------------------------------------------------------- dq
@@ -444,7 +469,8 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
                       const ushort_t* __restrict__ k, long kt, long kh,
                       const ushort_t* __restrict__ v, long vt, long vh,
                       const ushort_t* __restrict__ dout, long ot, long oh,
-                      const ushort_t* __restrict__ out, const int4_t* __restrict__ tiles,
+                      const ushort_t* __restrict__ out, const ushort_t* __restrict__ out_lo,
+                      const int4_t* __restrict__ tiles,
                       const float* __restrict__ lse, float* __restrict__ delta,
                       ushort_t* __restrict__ dq, int T, int Hq, int Hk, float scale) {
     const int4_t tile = tiles[blockIdx.x / Hq];
@@ -481,12 +507,14 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     float ls = mine ? lse[(long)h * T + row] : 0.f;
     float dl = 0.f;
     {
-        bf16x8_t o[D / 16];
+        bf16x8_t o[D / 16], rest[D / 16];
         load_row<D>(o, out + ((long)row * Hq + h) * D, mine, hi);
+        load_row<D>(rest, out_lo + ((long)row * Hq + h) * D, mine, hi);
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) dl = fmaf((float)of[s][j], (float)o[s][j], dl);
+            for (int j = 0; j < 8; ++j)
+                dl = fmaf((float)of[s][j], (float)o[s][j] + (float)rest[s][j], dl);
         dl = both_sum(dl);
     }
     settle(qf);
@@ -550,7 +578,7 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
                                acc[db]);
         }
     });
-    if (mine) store_row<D>(acc, seq1 < 0 ? NAN : scale, dq + ((long)row * Hq + h) * D, hi);
+    store_row<D>(acc, seq1 < 0 ? NAN : scale, dq + ((long)row * Hq + h) * D, hi, nullptr, mine);
 }
 
 // ------------------------------------------------------------------- dk, dv
@@ -722,10 +750,10 @@ packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     const long to = ((long)key * Hk + hk) * D;
     if (team) {
         add(ak, join + KS * 32 * D);
-        if (mine) store_row<D>(ak, seq1 < 0 ? NAN : scale, dk + to, hi);
+        store_row<D>(ak, seq1 < 0 ? NAN : scale, dk + to, hi, nullptr, mine);
     } else {
         add(av, join);
-        if (mine) store_row<D>(av, seq1 < 0 ? NAN : 1.f, dv + to, hi);
+        store_row<D>(av, seq1 < 0 ? NAN : 1.f, dv + to, hi, nullptr, mine);
     }
 }
 
@@ -746,19 +774,19 @@ namespace {
 template <int D, bool SAVE>
 void fwd(const void* q, long qt, long qh, const void* k, long kt, long kh,
          const void* v, long vt, long vh, const void* tiles, int max_tiles, void* out,
-         void* lse, int T, int Hq, int Hk, float scale, hipStream_t st) {
+         void* out_lo, void* lse, int T, int Hq, int Hk, float scale, hipStream_t st) {
     const int4_t* a = (const int4_t*)tiles;
     hipLaunchKernelGGL((packed_attn_fwd_kernel<D, SAVE>),
                        dim3((unsigned)max_tiles * Hq), dim3(256), 0, st,
                        (const ushort_t*)q, qt, qh, (const ushort_t*)k, kt, kh,
                        (const ushort_t*)v, vt, vh, a,
-                       (ushort_t*)out, (float*)lse, T, Hq, Hk, scale);
+                       (ushort_t*)out, (ushort_t*)out_lo, (float*)lse, T, Hq, Hk, scale);
 }
 
 template <int D>
 void dq_(const void* q, long qt, long qh, const void* k, long kt, long kh,
          const void* v, long vt, long vh, const void* dout, long ot, long oh,
-         const void* out, const void* tiles, int max_tiles,
+         const void* out, const void* out_lo, const void* tiles, int max_tiles,
          const void* lse, void* delta, void* dq, int T, int Hq, int Hk, float scale,
          hipStream_t st) {
     const int4_t* a = (const int4_t*)tiles;
@@ -766,7 +794,7 @@ void dq_(const void* q, long qt, long qh, const void* k, long kt, long kh,
                        dim3((unsigned)max_tiles * Hq), dim3(256), 0, st,
                        (const ushort_t*)q, qt, qh, (const ushort_t*)k, kt, kh,
                        (const ushort_t*)v, vt, vh, (const ushort_t*)dout, ot, oh,
-                       (const ushort_t*)out, a, (const float*)lse,
+                       (const ushort_t*)out, (const ushort_t*)out_lo, a, (const float*)lse,
                        (float*)delta, (ushort_t*)dq, T, Hq, Hk, scale);
 }
 
@@ -787,14 +815,14 @@ void dkv(const void* q, long qt, long qh, const void* k, long kt, long kh,
 
 }  // namespace
 
-// lse is null where no backward pass will follow.
+// out_lo and lse are null where no backward pass will follow.
 extern "C" int launch_packed_attn_fwd(const void* q, long qt, long qh, const void* k,
                                       long kt, long kh, const void* v, long vt, long vh,
                                       const void* tiles, int max_tiles, void* out,
-                                      void* lse, int T, int Hq, int Hk, int D, float scale, void* stream) {
+                                      void* out_lo, void* lse, int T, int Hq, int Hk, int D, float scale, void* stream) {
 #define FWD(d, s)                                                                          \
-    fwd<d, s>(q, qt, qh, k, kt, kh, v, vt, vh, tiles, max_tiles, out, lse, T, Hq, Hk, scale, \
-              (hipStream_t)stream)
+    fwd<d, s>(q, qt, qh, k, kt, kh, v, vt, vh, tiles, max_tiles, out, out_lo, lse, T, Hq, Hk, \
+              scale, (hipStream_t)stream)
     if (D == 128) {
         if (lse) FWD(128, true);
         else FWD(128, false);
@@ -809,15 +837,15 @@ extern "C" int launch_packed_attn_fwd(const void* q, long qt, long qh, const voi
 extern "C" int launch_packed_attn_dq(const void* q, long qt, long qh, const void* k,
                                      long kt, long kh, const void* v, long vt, long vh,
                                      const void* dout, long ot, long oh, const void* out,
-                                     const void* tiles, int max_tiles,
+                                     const void* out_lo, const void* tiles, int max_tiles,
                                      const void* lse, void* delta, void* dq, int T, int Hq,
                                      int Hk, int D, float scale, void* stream) {
     if (D == 128)
-        dq_<128>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, out, tiles, max_tiles, lse,
-                 delta, dq, T, Hq, Hk, scale, (hipStream_t)stream);
+        dq_<128>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, out, out_lo, tiles, max_tiles,
+                 lse, delta, dq, T, Hq, Hk, scale, (hipStream_t)stream);
     else
-        dq_<64>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, out, tiles, max_tiles, lse,
-                delta, dq, T, Hq, Hk, scale, (hipStream_t)stream);
+        dq_<64>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, out, out_lo, tiles, max_tiles,
+                lse, delta, dq, T, Hq, Hk, scale, (hipStream_t)stream);
     return (int)hipGetLastError();
 }
 

@@ -18,11 +18,11 @@
 extern "C" {
 int launch_packed_tiles(const void*, int, int, int, void*, void*);
 int launch_packed_attn_fwd(const void*, long, long, const void*, long, long, const void*,
-                           long, long, const void*, int, void*, void*, int, int, int, int,
-                           float, void*);
+                           long, long, const void*, int, void*, void*, void*, int, int, int,
+                           int, float, void*);
 int launch_packed_attn_dq(const void*, long, long, const void*, long, long, const void*,
                           long, long, const void*, long, long, const void*, const void*,
-                          int, const void*, void*, void*, int, int, int, int,
+                          const void*, int, const void*, void*, void*, int, int, int, int,
                           float, void*);
 int launch_packed_attn_dkv(const void*, long, long, const void*, long, long, const void*,
                            long, long, const void*, long, long, const void*, int,
@@ -99,7 +99,7 @@ Sizes check_qkv(const Tensor& q, const Tensor& k, const Tensor& v) {
     return {(int)T, (int)Hq, (int)Hk, (int)D};
 }
 
-// -> out and, with `save`, lse and tiles
+// -> out and, with `save`, what its rounding left over, lse and tiles
 std::vector<Tensor> packed_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor starts, double scale,
                                     bool save) {
     const Sizes s = check_qkv(q, k, v);
@@ -110,9 +110,12 @@ std::vector<Tensor> packed_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor starts,
     TORCH_CHECK(2 * max_tiles * s.Hq < (1L << 31), "too many sequences");
     const c10::cuda::CUDAGuard guard(q.device());
     const auto opt = q.options();
-    Tensor out = torch::empty({s.T, s.Hq, s.D}, opt), lse;
+    Tensor out = torch::empty({s.T, s.Hq, s.D}, opt), rest, lse;
     Tensor tiles = torch::empty({8 * max_tiles}, opt.dtype(torch::kInt32));
-    if (save) lse = torch::empty({s.Hq, s.T}, opt.dtype(torch::kFloat32));
+    if (save) {
+        rest = torch::empty_like(out);
+        lse = torch::empty({s.Hq, s.T}, opt.dtype(torch::kFloat32));
+    }
     if (s.T > 0) {
         void* st = stream_of(q);
         launched(launch_packed_tiles(starts.data_ptr(), (int)B, s.T, (int)max_tiles,
@@ -120,16 +123,17 @@ std::vector<Tensor> packed_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor starts,
         launched(launch_packed_attn_fwd(
                      q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
                      k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), tiles.data_ptr(),
-                     (int)max_tiles, out.data_ptr(), save ? lse.data_ptr() : nullptr, s.T, s.Hq, s.Hk, s.D, (float)scale, st),
+                     (int)max_tiles, out.data_ptr(), save ? rest.data_ptr() : nullptr,
+                     save ? lse.data_ptr() : nullptr, s.T, s.Hq, s.Hk, s.D, (float)scale, st),
                  "packed_attention");
     }
     if (!save) return {out};
-    return {out, lse, tiles};
+    return {out, rest, lse, tiles};
 }
 
 // -> dq, dk, dv (the last two undefined without `keys`)
 std::vector<Tensor> packed_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out,
-                                    Tensor lse, Tensor tiles, double scale,
+                                    Tensor rest, Tensor lse, Tensor tiles, double scale,
                                     bool keys) {
     const Sizes s = check_qkv(q, k, v);
     check_rows(dout, "the gradient", q);
@@ -149,7 +153,7 @@ std::vector<Tensor> packed_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, T
         launched(launch_packed_attn_dq(
                      q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
                      k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), dout.data_ptr(),
-                     dout.stride(0), dout.stride(1), out.data_ptr(),
+                     dout.stride(0), dout.stride(1), out.data_ptr(), rest.data_ptr(),
                      tiles.data_ptr(), (int)max_tiles, lse.data_ptr(), delta.data_ptr(),
                      dq.data_ptr(), s.T, s.Hq, s.Hk, s.D, (float)scale, st),
                  "packed_attention's gradient");
@@ -171,14 +175,14 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
                           double scale) {
         const Tensor q = rows16(q0), k = rows16(k0), v = rows16(v0);
         const auto got = packed_attn_fwd(q, k, v, starts, scale, true);
-        ctx->save_for_backward({q, k, v, got[0], got[1], got[2]});
+        ctx->save_for_backward({q, k, v, got[0], got[1], got[2], got[3]});
         ctx->saved_data["scale"] = scale;
         return got[0];
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                    torch::autograd::variable_list g) {
         const auto s = ctx->get_saved_variables();
-        auto d = packed_attn_bwd(rows16(g[0]), s[0], s[1], s[2], s[3], s[4], s[5],
+        auto d = packed_attn_bwd(rows16(g[0]), s[0], s[1], s[2], s[3], s[4], s[5], s[6],
                                  ctx->saved_data["scale"].toDouble(),
                                  ctx->needs_input_grad(1) || ctx->needs_input_grad(2));
         d = once(std::move(d), "packed_attention");
