@@ -159,9 +159,22 @@ xent_reduce_kernel(const float* __restrict__ loss, const long* __restrict__ targ
                    float* __restrict__ factor) {
     double s = 0.0;
     int n = 0;
-    for (int i = threadIdx.x; i < N; i += 1024) {
-        s += loss[i];
-        n += targets[i] != ignore;
+    for (int i0 = threadIdx.x; i0 < N; i0 += 8 * 1024) {
+        // eight loads on their way at a time, with no branch between them
+        float l[8];
+        long t[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int i = min(i0 + u * 1024, N - 1);
+            l[u] = loss[i];
+            t[u] = targets[i];
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (i0 + u * 1024 < N) {
+                s += l[u];
+                n += t[u] != ignore;
+            }
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
