@@ -16,6 +16,10 @@
 // log-sum near 12 is rounded by 5e-7, which would be in every gradient.
 #include "common.h"
 
+#include <type_traits>
+
+#define XENT_SHORT 8192   // the longest row that a single wave takes
+
 namespace {
 
 template <typename T> struct Elem;
@@ -71,109 +75,127 @@ DEVINL int head_of(const T* row, int V) {
 }  // namespace
 
 // WAVES waves a row, 4 waves a workgroup at least.  A wave a row needs no
-// barrier and keeps its whole row in flight up to V = 4096; long rows take 16.
+// barrier and reads a row of 4096 in two steps; long rows take 16 (4 a row read
+// 128256 bf16 at 5.0 TB/s, 16 at 5.4).  A workgroup leaves one sum and count of
+// its rows (`sums` not null) to add up.
 template <typename T, int WAVES>
 __global__ void __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64)
 xent_fwd_kernel(const T* __restrict__ x, long stride, const long* __restrict__ targets,
                 long ignore, int N, int V, float* __restrict__ loss,
-                float2_t* __restrict__ stats) {
+                float2_t* __restrict__ stats, double* __restrict__ sums,
+                int* __restrict__ counts) {
     constexpr int VEC = Elem<T>::VEC, LANES = WAVES * 64;
     constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1;
     constexpr int U = 4;
-    const int row = blockIdx.x * ROWS + (ROWS > 1 ? (int)threadIdx.x / LANES : 0);
-    if (ROWS > 1 && row >= N) return;   // a whole wave; there is no barrier then
     const int tid = threadIdx.x % LANES;
-    const long t = targets[row];
-    if (t == ignore) {
-        if (tid == 0) loss[row] = 0.f;
-        return;
-    }
-    const T* r = x + row * stride;
-    float m = -INFINITY, l = 0.f;
-    auto one = [&](float v) {
-        if (v > m) {
-            l *= __builtin_amdgcn_exp2f((m - v) * L2E);
-            m = v;
+    const long row = (long)blockIdx.x * ROWS + threadIdx.x / LANES;
+    const long t = row < N ? targets[row] : ignore;
+    double sum = 0.0;   // of a row's first thread
+    int labels = 0;
+    if (row < N && t == ignore && tid == 0) loss[row] = 0.f;
+    if (row < N && t != ignore) {   // the whole workgroup, where it has a barrier
+        const T* r = x + row * stride;
+        float m = -INFINITY, l = 0.f;
+        auto one = [&](float v) {
+            if (v > m) {
+                l *= __builtin_amdgcn_exp2f((m - v) * L2E);
+                m = v;
+            }
+            l += __builtin_amdgcn_exp2f((v - (m == -INFINITY ? 0.f : m)) * L2E);
+        };
+        const int head = head_of(r, V);
+        const int vecs = (V - head) / VEC;
+        const Vec<T>* body = reinterpret_cast<const Vec<T>*>(r + head);
+        // U vectors on their way at a time, all of them real but in the last step
+        auto step = [&](int i0, auto whole) {
+            Vec<T> v[U];
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                v[u] = body[whole ? i0 + u * LANES : min(i0 + u * LANES, vecs - 1)];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (whole || i0 + u * LANES < vecs)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) top = fmaxf(top, Elem<T>::get(v[u][j]));
+            if (top > m) {
+                l *= __builtin_amdgcn_exp2f((m - top) * L2E);
+                m = top;
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (whole || i0 + u * LANES < vecs)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j)
+                        l += __builtin_amdgcn_exp2f((Elem<T>::get(v[u][j]) - base) * L2E);
+        };
+        int i0 = 0;
+        for (; i0 + U * LANES <= vecs; i0 += U * LANES) step(i0 + tid, std::true_type{});
+        if (i0 < vecs) step(i0 + tid, std::false_type{});
+        // the rest: fewer than VEC elements at each end
+        const int tail = head + vecs * VEC;
+        if (tid < head) one(Elem<T>::get(r[tid]));
+        if (tail + tid < V) one(Elem<T>::get(r[tail + tid]));
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) {
+            const float m2 = __shfl_xor(m, off, WAVE), l2 = __shfl_xor(l, off, WAVE);
+            join(m, l, m2, l2);
         }
-        l += __builtin_amdgcn_exp2f((v - (m == -INFINITY ? 0.f : m)) * L2E);
-    };
-    const int head = head_of(r, V);
-    const int vecs = (V - head) / VEC;
-    const Vec<T>* body = reinterpret_cast<const Vec<T>*>(r + head);
-    for (int i0 = tid; i0 < vecs; i0 += U * LANES) {
-        Vec<T> v[U];
-        float top = -INFINITY;
+        if (WAVES > 1) {
+            __shared__ float ms[WAVES], lsum[WAVES];
+            if ((tid & 63) == 0) { ms[tid >> 6] = m; lsum[tid >> 6] = l; }
+            __syncthreads();
+            m = ms[0];
+            l = lsum[0];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * LANES;
-            if (i < vecs) v[u] = body[i];
+            for (int w = 1; w < WAVES; ++w) join(m, l, ms[w], lsum[w]);
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i0 + u * LANES < vecs)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) top = fmaxf(top, Elem<T>::get(v[u][j]));
-        if (top > m) {
-            l *= __builtin_amdgcn_exp2f((m - top) * L2E);
-            m = top;
+        if (tid == 0) {
+            // a label that is no place of the row: no value, and no read
+            const bool in = t >= 0 && t < V;
+            const float x = in ? __logf(l) + (m - Elem<T>::get(r[in ? t : 0])) : NAN;
+            loss[row] = x;
+            if (stats) stats[row] = float2_t{m, in ? 1.f / l : NAN};
+            sum += x;
+            ++labels;
         }
-        const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i0 + u * LANES < vecs)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    l += __builtin_amdgcn_exp2f((Elem<T>::get(v[u][j]) - base) * L2E);
     }
-    // the rest: fewer than VEC elements at each end
-    const int tail = head + vecs * VEC;
-    if (tid < head) one(Elem<T>::get(r[tid]));
-    if (tail + tid < V) one(Elem<T>::get(r[tail + tid]));
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const float m2 = __shfl_xor(m, off, WAVE), l2 = __shfl_xor(l, off, WAVE);
-        join(m, l, m2, l2);
-    }
-    if (WAVES > 1) {
-        __shared__ float ms[WAVES], lsum[WAVES];
-        if ((tid & 63) == 0) { ms[tid >> 6] = m; lsum[tid >> 6] = l; }
+    if (sums) {
+        __shared__ double ss[ROWS];
+        __shared__ int ns[ROWS];
+        if (tid == 0) { ss[threadIdx.x / LANES] = sum; ns[threadIdx.x / LANES] = labels; }
         __syncthreads();
-        m = ms[0];
-        l = lsum[0];
-#pragma unroll
-        for (int w = 1; w < WAVES; ++w) join(m, l, ms[w], lsum[w]);
-    }
-    if (tid == 0) {
-        // a label that is no place of the row: no value, and no read
-        const bool in = t >= 0 && t < V;
-        loss[row] = in ? __logf(l) + (m - Elem<T>::get(r[in ? t : 0])) : NAN;
-        if (stats) stats[row] = float2_t{m, in ? 1.f / l : NAN};
+        if (threadIdx.x == 0) {
+            for (int i = 1; i < ROWS; ++i) { sum += ss[i]; labels += ns[i]; }
+            sums[blockIdx.x] = sum;
+            counts[blockIdx.x] = labels;
+        }
     }
 }
 
-// Sum of the rows' losses, or their mean over the labels (NaN where there is
-// none), and the factor 1, or 1 / number of labels.
+// The rows' loss, or its mean over the labels (NaN where there is none), from
+// the workgroups' sums, and the factor 1, or 1 / number of labels.
 __global__ void __launch_bounds__(1024)
-xent_reduce_kernel(const float* __restrict__ loss, const long* __restrict__ targets,
-                   long ignore, int N, int mean, float* __restrict__ result,
-                   float* __restrict__ factor) {
+xent_reduce_kernel(const double* __restrict__ sums, const int* __restrict__ counts, int parts,
+                   int mean, float* __restrict__ result, float* __restrict__ factor) {
     double s = 0.0;
     int n = 0;
-    for (int i0 = threadIdx.x; i0 < N; i0 += 8 * 1024) {
-        // eight loads on their way at a time, with no branch between them
-        float l[8];
-        long t[8];
+    for (int i0 = threadIdx.x; i0 < parts; i0 += 8 * 1024) {
+        // eight on their way at a time, with no branch between them
+        double x[8];
+        int c[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const int i = min(i0 + u * 1024, N - 1);
-            l[u] = loss[i];
-            t[u] = targets[i];
+            const int i = min(i0 + u * 1024, parts - 1);
+            x[u] = sums[i];
+            c[u] = counts[i];
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            if (i0 + u * 1024 < N) {
-                s += l[u];
-                n += t[u] != ignore;
+            if (i0 + u * 1024 < parts) {
+                s += x[u];
+                n += c[u];
             }
     }
 #pragma unroll
@@ -226,17 +248,15 @@ xent_bwd_kernel(const T* __restrict__ x, long stride, const long* __restrict__ t
         return Elem<T>::put((exp_neg<T>(v - m) * inv - (j == t ? 1.f : 0.f)) * g);
     };
     const Vec<T>* body = reinterpret_cast<const Vec<T>*>(r + head);
-    for (int i0 = tid; i0 < vecs; i0 += U * LANES) {
+    auto step = [&](int i0, auto whole) {
         Vec<T> v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * LANES;
-            if (i < vecs) v[u] = body[i];
-        }
+        for (int u = 0; u < U; ++u)
+            v[u] = body[whole ? i0 + u * LANES : min(i0 + u * LANES, vecs - 1)];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * LANES;
-            if (i < vecs) {
+            if (whole || i < vecs) {
                 Vec<T> w;
                 const int j0 = head + i * VEC;
 #pragma unroll
@@ -244,7 +264,10 @@ xent_bwd_kernel(const T* __restrict__ x, long stride, const long* __restrict__ t
                 out[i] = w;
             }
         }
-    }
+    };
+    int i0 = 0;
+    for (; i0 + U * LANES <= vecs; i0 += U * LANES) step(i0 + tid, std::true_type{});
+    if (i0 < vecs) step(i0 + tid, std::false_type{});
     if (tid < head) d[tid] = one(tid, Elem<T>::get(r[tid]));
     if (tail + tid < V) d[tail + tid] = one(tail + tid, Elem<T>::get(r[tail + tid]));
 }
@@ -254,20 +277,23 @@ xent_bwd_kernel(const T* __restrict__ x, long stride, const long* __restrict__ t
 
 namespace {
 
+template <int WAVES> constexpr int rows_of = WAVES < 4 ? 4 / WAVES : 1;
+
 template <typename T, int WAVES>
 void fwd(const void* x, long stride, const void* targets, long ignore, int N, int V,
-         void* loss, void* stats, hipStream_t st) {
-    constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1;
+         void* loss, void* stats, void* sums, void* counts, hipStream_t st) {
+    constexpr int ROWS = rows_of<WAVES>;
     hipLaunchKernelGGL((xent_fwd_kernel<T, WAVES>), dim3((N + ROWS - 1) / ROWS),
                        dim3(ROWS * WAVES * 64), 0, st, (const T*)x, stride,
-                       (const long*)targets, ignore, N, V, (float*)loss, (float2_t*)stats);
+                       (const long*)targets, ignore, N, V, (float*)loss, (float2_t*)stats,
+                       (double*)sums, (int*)counts);
 }
 
 template <typename T, int WAVES>
 void bwd(const void* x, long stride, const void* targets, long ignore, int N, int V,
          const void* stats, const void* gout, long gstride, const void* factor, void* dx,
          long dstride, hipStream_t st) {
-    constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1;
+    constexpr int ROWS = rows_of<WAVES>;
     hipLaunchKernelGGL((xent_bwd_kernel<T, WAVES>), dim3((N + ROWS - 1) / ROWS),
                        dim3(ROWS * WAVES * 64), 0, st, (const T*)x, stride,
                        (const long*)targets, ignore, N, V, (const float2_t*)stats,
@@ -276,13 +302,21 @@ void bwd(const void* x, long stride, const void* targets, long ignore, int N, in
 
 }  // namespace
 
+// How many sums and counts the forward kernel leaves.
+extern "C" int xent_parts(int N, int V) {
+    const int rows = V <= XENT_SHORT ? rows_of<1> : rows_of<16>;
+    return (N + rows - 1) / rows;
+}
+
 extern "C" int launch_xent_fwd(int kind, const void* x, long stride, const void* targets,
-                               long ignore, int N, int V, void* loss, void* stats,
-                               void* stream) {
+                               long ignore, int N, int V, void* loss, void* stats, void* sums,
+                               void* counts, void* stream) {
     const hipStream_t st = (hipStream_t)stream;
-#define FWD(T)                                                                    \
-    if (V <= 8192) fwd<T, 1>(x, stride, targets, ignore, N, V, loss, stats, st);  \
-    else fwd<T, 16>(x, stride, targets, ignore, N, V, loss, stats, st)
+#define FWD(T)                                                                             \
+    if (V <= XENT_SHORT)                                                                   \
+        fwd<T, 1>(x, stride, targets, ignore, N, V, loss, stats, sums, counts, st);        \
+    else                                                                                   \
+        fwd<T, 16>(x, stride, targets, ignore, N, V, loss, stats, sums, counts, st)
     if (kind == 0) { FWD(float); }
     else if (kind == 1) { FWD(__bf16); }
     else { FWD(_Float16); }
@@ -290,11 +324,11 @@ extern "C" int launch_xent_fwd(int kind, const void* x, long stride, const void*
     return (int)hipGetLastError();
 }
 
-extern "C" int launch_xent_reduce(const void* loss, const void* targets, long ignore, int N,
-                                  int mean, void* result, void* factor, void* stream) {
+extern "C" int launch_xent_reduce(const void* sums, const void* counts, int parts, int mean,
+                                  void* result, void* factor, void* stream) {
     hipLaunchKernelGGL(xent_reduce_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream,
-                       (const float*)loss, (const long*)targets, ignore, N, mean,
-                       (float*)result, (float*)factor);
+                       (const double*)sums, (const int*)counts, parts, mean, (float*)result,
+                       (float*)factor);
     return (int)hipGetLastError();
 }
 
@@ -304,7 +338,7 @@ extern "C" int launch_xent_bwd(int kind, const void* x, long stride, const void*
                                long dstride, void* stream) {
     const hipStream_t st = (hipStream_t)stream;
 #define BWD(T)                                                                          \
-    if (V <= 8192)                                                                      \
+    if (V <= XENT_SHORT)                                                                      \
         bwd<T, 1>(x, stride, targets, ignore, N, V, stats, gout, gstride, factor, dx,   \
                   dstride, st);                                                         \
     else                                                                                \

@@ -28,8 +28,10 @@ int launch_packed_attn_dkv(const void*, long, long, const void*, long, long, con
                            long, long, const void*, long, long, const void*, int,
                            const void*, const void*, void*, void*, int, int, int, int, float,
                            void*);
-int launch_xent_fwd(int, const void*, long, const void*, long, int, int, void*, void*, void*);
-int launch_xent_reduce(const void*, const void*, long, int, int, void*, void*, void*);
+int launch_xent_fwd(int, const void*, long, const void*, long, int, int, void*, void*, void*,
+                    void*, void*);
+int xent_parts(int, int);
+int launch_xent_reduce(const void*, const void*, int, int, void*, void*, void*);
 int launch_xent_bwd(int, const void*, long, const void*, long, int, int, const void*,
                     const void*, long, const void*, void*, long, void*);
 int launch_grad_sums(const GradTable*, int, void*, void*);
@@ -205,7 +207,7 @@ int kind_of(const Tensor& t, const char* name) {
         case torch::kFloat32: return 0;
         case torch::kBFloat16: return 1;
         case torch::kFloat16: return 2;
-        default: TORCH_CHECK(false, name, " must be float32, bfloat16 or float16");
+        default: TORCH_CHECK_VALUE(false, name, " must be float32, bfloat16 or float16");
     }
 }
 
@@ -229,15 +231,24 @@ std::vector<Tensor> xent_fwd(Tensor x, Tensor targets, int64_t ignore, int64_t m
     const c10::cuda::CUDAGuard guard(x.device());
     const auto opt = x.options().dtype(torch::kFloat32);
     Tensor loss = torch::empty({N}, opt), stats = torch::empty({save ? N : 0, 2}, opt);
+    Tensor sums;   // of each workgroup of the kernel, and its counts behind them
+    double* at = nullptr;
+    const long parts = N > 0 ? xent_parts(N, V) : 1;
+    if (mode) {
+        sums = N > 0 ? torch::empty({2 * parts}, opt.dtype(torch::kFloat64))
+                     : torch::zeros({2 * parts}, opt.dtype(torch::kFloat64));
+        at = sums.data_ptr<double>();
+    }
     void* st = stream_of(x);
     if (N > 0)
         launched(launch_xent_fwd(kind, x.data_ptr(), x.stride(0), targets.data_ptr(), ignore, N,
-                                 V, loss.data_ptr(), save ? stats.data_ptr() : nullptr, st),
+                                 V, loss.data_ptr(), save ? stats.data_ptr() : nullptr, at,
+                                 mode ? at + parts : nullptr, st),
                  "cross_entropy");
     if (!mode) return {loss, stats};
     Tensor result = torch::empty({}, opt), factor = torch::empty({}, opt);
-    launched(launch_xent_reduce(loss.data_ptr(), targets.data_ptr(), ignore, N, mode == 1,
-                                result.data_ptr(), factor.data_ptr(), st), "cross_entropy");
+    launched(launch_xent_reduce(at, at + parts, (int)parts, mode == 1, result.data_ptr(),
+                                factor.data_ptr(), st), "cross_entropy");
     return {loss, stats, result, factor};
 }
 
@@ -322,15 +333,15 @@ Grads collect(const std::vector<Tensor>& grads, bool write) {
     std::vector<std::pair<uintptr_t, uintptr_t>> spans;
     for (size_t i = 0; i < grads.size(); ++i) {
         const Tensor& t = grads[i];
-        TORCH_CHECK(t.layout() == torch::kStrided && t.is_cuda() &&
-                        t.device() == grads[0].device(),
-                    "gradients must be dense and on one GPU");
+        TORCH_CHECK_VALUE(t.layout() == torch::kStrided && t.is_cuda() &&
+                              t.device() == grads[0].device(),
+                          "gradients must be dense and on one device");
         kind_of(t, "gradients");
         if (t.numel() == 0) continue;
         Tensor d = t;
         if (!t.is_non_overlapping_and_dense()) {
-            TORCH_CHECK(!write || apart(t),
-                        "a gradient must not share memory between its elements");
+            TORCH_CHECK_VALUE(!write || apart(t),
+                              "a gradient must not share memory between its elements");
             d = t.clone(at::MemoryFormat::Contiguous);
             g.copied.push_back((long)i);
         }
@@ -344,8 +355,8 @@ Grads collect(const std::vector<Tensor>& grads, bool write) {
     }
     std::sort(spans.begin(), spans.end());
     for (size_t i = 1; i < spans.size(); ++i)
-        TORCH_CHECK(spans[i].first >= spans[i - 1].second,
-                    "two of the gradients share memory");
+        TORCH_CHECK_VALUE(spans[i].first >= spans[i - 1].second,
+                          "two of the gradients share memory");
     for (const Tensor& d : g.at) {
         const long size = d.element_size();
         const auto p = reinterpret_cast<uintptr_t>(d.data_ptr());
@@ -384,6 +395,7 @@ Tensor sums_of(const Grads& g, const Tensor& like, void* st) {
 
 Tensor grad_norm(std::vector<Tensor> grads) {
     TORCH_CHECK(!grads.empty(), "no gradients");
+    const at::NoGradGuard no_grad;
     const Grads g = collect(grads, false);
     const c10::cuda::CUDAGuard guard(grads[0].device());
     void* st = stream_of(grads[0]);
@@ -396,6 +408,7 @@ Tensor grad_norm(std::vector<Tensor> grads) {
 
 Tensor grad_clip(std::vector<Tensor> grads, double limit, double eps) {
     TORCH_CHECK(!grads.empty(), "no gradients");
+    const at::NoGradGuard no_grad;
     const Grads g = collect(grads, true);
     const c10::cuda::CUDAGuard guard(grads[0].device());
     void* st = stream_of(grads[0]);

@@ -62,7 +62,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         raise ValueError(f"on the GPU q, k and v must be bfloat16, not {q.dtype}")
     if q.shape[2] not in (64, 128):
         raise ValueError(f"on the GPU the head dim must be 64 or 128, not {q.shape[2]}")
-    starts = seq_starts.to(device=q.device, dtype=torch.int32).contiguous()
+    starts = seq_starts
+    if starts.dtype != torch.int32 or starts.device != q.device or not starts.is_contiguous():
+        starts = starts.to(device=q.device, dtype=torch.int32).contiguous()
     return _get_ext().packed_attention(q, k, v, starts, scale)
 
 
@@ -93,7 +95,8 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int
         raise ValueError("logits and targets must be on one device")
     if reduction not in _MODES:
         raise ValueError(f"reduction must be one of {sorted(_MODES)}, not {reduction!r}")
-    targets = targets.long().contiguous()
+    if targets.dtype != torch.int64 or not targets.is_contiguous():
+        targets = targets.long().contiguous()
     if not logits.is_cuda:
         return reference.cross_entropy(logits, targets, ignore_index, reduction)
     if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
@@ -111,8 +114,12 @@ _EPS = 1e-6   # in the divisor, so that a norm of zero divides
 
 def _grads(parameters) -> list[torch.Tensor]:
     if isinstance(parameters, torch.Tensor):
-        parameters = [parameters]
-    grads = [p.grad for p in parameters if p.grad is not None]
+        parameters = (parameters,)
+    return [g for g in [p.grad for p in parameters] if g is not None]
+
+
+def _check_host(grads: list[torch.Tensor]) -> None:
+    """What the kernels' bindings check of gradients on the GPU."""
     for g in grads:
         if g.layout != torch.strided or g.dtype not in (torch.float32, torch.bfloat16,
                                                         torch.float16):
@@ -120,22 +127,21 @@ def _grads(parameters) -> list[torch.Tensor]:
                              f"not {g.layout} {g.dtype}")
         if g.device != grads[0].device:
             raise ValueError("gradients must be on one device")
-    return grads
 
 
-@torch.no_grad()
 def grad_norm(parameters) -> torch.Tensor:
     """2-norm of all parameters' gradients together (fp32 scalar on their
     device); parameters without a gradient are passed over."""
     grads = _grads(parameters)
     if not grads:
         return torch.zeros(())
-    if not grads[0].is_cuda:
+    if grads[0].is_cuda:
+        return _get_ext().grad_norm(grads)
+    _check_host(grads)
+    with torch.no_grad():
         return reference.grad_norm(grads)
-    return _get_ext().grad_norm(grads)
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scales all parameters' gradients in place by
@@ -160,6 +166,8 @@ def clip_grad_norm_(parameters, max_norm: float,
     grads = _grads(parameters)
     if not grads:
         return torch.zeros(())
-    if not grads[0].is_cuda:
+    if grads[0].is_cuda:
+        return _get_ext().grad_clip(grads, max_norm, _EPS)
+    _check_host(grads)
+    with torch.no_grad():
         return reference.grad_clip(grads, max_norm, _EPS)
-    return _get_ext().grad_clip(grads, max_norm, _EPS)
