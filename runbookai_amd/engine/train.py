@@ -21,6 +21,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .. import ops
 from .llama import CONFIGS, LlamaConfig, LlamaModel
 
 # served policy architecture: small enough to train on one MI355X in
@@ -92,7 +93,23 @@ class TrainableLayer(nn.Module):
         attn = F.scaled_dot_product_attention(
             q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2),
             is_causal=True, scale=1.0 / math.sqrt(d))
-        h = h + self.o_proj(attn.transpose(1, 2).reshape(B, T, hq * d))
+        return self._after(h, attn.transpose(1, 2).reshape(B, T, hq * d))
+
+    def forward_packed(self, h: torch.Tensor, cos, sin, seq_starts) -> torch.Tensor:
+        """h [T, H]: sequences one after another; cos/sin [T, D/2] of each
+        row's place in its sequence."""
+        cfg = self.cfg
+        T = h.shape[0]
+        d, hq, hk = cfg.head_dim, cfg.num_heads, cfg.num_kv_heads
+        qkv = self.qkv(self.input_norm(h))
+        q, k, v = qkv.split([hq * d, hk * d, hk * d], dim=-1)
+        q = _rope_interleaved(q.view(1, T, hq, d), cos, sin)[0]
+        k = _rope_interleaved(k.view(1, T, hk, d), cos, sin)[0]
+        attn = ops.packed_attention(q, k, v.view(T, hk, d), seq_starts, scale=1.0 / math.sqrt(d))
+        return self._after(h, attn.reshape(T, hq * d))
+
+    def _after(self, h: torch.Tensor, attn: torch.Tensor) -> torch.Tensor:
+        h = h + self.o_proj(attn)
         x = self.post_norm(h)
         gate, up = self.gate_up(x).chunk(2, dim=-1)
         h = h + self.down(F.silu(gate) * up)
@@ -127,6 +144,49 @@ class TrainableLlama(nn.Module):
         for layer in self.layers:
             h = layer(h, cos, sin)
         return self.lm_head(self.final_norm(h))
+
+    def forward_packed(self, ids: torch.Tensor, seq_starts: torch.Tensor) -> torch.Tensor:
+        """ids [T]: sequences one after another, of rows seq_starts[b] up to
+        seq_starts[b + 1], each as if it came alone -> logits [T, vocab].
+        Rows in no sequence are computed but attend to nothing. On the GPU
+        attention is the HIP kernel pair of ops.packed_attention, which takes
+        bfloat16: run it under autocast or with a bfloat16 model. seq_starts
+        belongs on the host; one on the device is waited for."""
+        starts = seq_starts.tolist()
+        if ids.dim() != 1 or not starts or starts[0] < 0 or starts[-1] > ids.shape[0] \
+                or starts != sorted(starts):
+            raise ValueError(f"seq_starts must rise within the {ids.numel()} rows of ids")
+        longest = max([b - a for a, b in zip(starts[:-1], starts[1:])], default=0)
+        if longest > self.cfg.max_seq_len:
+            raise ValueError(f"a sequence of {longest} tokens is longer than the model's "
+                             f"{self.cfg.max_seq_len}")
+        place = torch.zeros(ids.shape[0], dtype=torch.long)
+        for a, b in zip(starts[:-1], starts[1:]):
+            place[a:b] = torch.arange(b - a)
+        h = self.embed(ids)
+        place = place.to(h.device)
+        cos = self.rope_cos[place]
+        sin = self.rope_sin[place]
+        on_device = torch.tensor(starts, dtype=torch.int32, device=h.device)
+        for layer in self.layers:
+            h = layer.forward_packed(h, cos, sin, on_device)
+        return self.lm_head(self.final_norm(h))
+
+
+def pack_samples(samples) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Samples (ids, first answer position) -> (ids [T], seq_starts [B+1],
+    targets [T]) of one packed batch: each row's target is the next token
+    where that is part of the answer, -100 elsewhere."""
+    ids: list[int] = []
+    targets: list[int] = []
+    starts = [0]
+    for tokens, answer in samples:
+        ids += tokens
+        targets += [t if i + 1 >= answer else -100 for i, t in enumerate(tokens[1:])]
+        targets += [-100] * bool(tokens)
+        starts.append(len(ids))
+    return (torch.tensor(ids, dtype=torch.long), torch.tensor(starts, dtype=torch.int32),
+            torch.tensor(targets, dtype=torch.long))
 
 
 def to_inference_model(model: TrainableLlama, device: str = "cpu",

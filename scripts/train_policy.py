@@ -14,8 +14,12 @@ Pipeline (all offline, no network):
   5. --eval: run the held-out eval fixture cases (redis/gateway/kafka/tls)
      through the served checkpoint + reference scorer -> pass_rate.
 
+With --packed, step 3 packs whole samples into batches without padding and
+runs the training ops (packed attention, cross-entropy that skips unlabelled
+rows, gradient clipping) instead of padded batches through the library's.
+
 Usage:  python scripts/train_policy.py --cases 400 --steps 1200 \
-            --out gpurun_out/policy_ckpt --eval
+            --out gpurun_out/policy_ckpt --eval [--packed]
 """
 from __future__ import annotations
 
@@ -107,7 +111,26 @@ def batches(samples, batch_tokens: int, rng: random.Random):
         yield ids, mask
 
 
+def packed_batches(samples, batch_tokens: int, rng: random.Random):
+    """Batches of whole samples in random order, one after another without
+    padding, of at most batch_tokens tokens (or one sample)."""
+    from runbookai_amd.engine.train import pack_samples
+
+    order = list(range(len(samples)))
+    rng.shuffle(order)
+    cur, total = [], 0
+    for i in order:
+        if cur and total + len(samples[i][0]) > batch_tokens:
+            yield pack_samples(cur)
+            cur, total = [], 0
+        cur.append(samples[i])
+        total += len(samples[i][0])
+    if cur:
+        yield pack_samples(cur)
+
+
 def run_training(args):
+    from runbookai_amd import ops
     from runbookai_amd.engine.bpe_tokenizer import BpeTokenizer
     from runbookai_amd.engine.train import CONFIGS, TrainableLlama, export_trained
 
@@ -153,25 +176,35 @@ def run_training(args):
             lt[m.reshape(-1)], tgt.reshape(-1)[m.reshape(-1)])
         return loss
 
+    def packed_loss_of(ids, starts, targets):
+        with torch.autocast(device_type="cuda", dtype=torch.bfloat16,
+                            enabled=(dev == "cuda")):
+            logits = model.forward_packed(ids.to(dev), starts)
+        return ops.cross_entropy(logits, targets.to(dev))
+
+    batched, loss_fn, clip = batches, loss_of, torch.nn.utils.clip_grad_norm_
+    if args.packed:
+        batched, loss_fn, clip = packed_batches, packed_loss_of, ops.clip_grad_norm_
+
     while step < args.steps:
-        for ids, mask in batches(train_s, args.batch_tokens, rng):
+        for batch in batched(train_s, args.batch_tokens, rng):
             if step >= args.steps:
                 break
             lr = args.lr * 0.5 * (1 + math.cos(math.pi * step / args.steps))
             for g in opt.param_groups:
                 g["lr"] = lr
-            loss = loss_of(ids, mask)
+            loss = loss_fn(*batch)
             opt.zero_grad(set_to_none=True)
             loss.backward()
-            torch.nn.utils.clip_grad_norm_(model.parameters(), 1.0)
+            clip(model.parameters(), 1.0)
             opt.step()
             losses.append(float(loss))
             step += 1
             if step % 100 == 0 or step == args.steps:
                 with torch.no_grad():
-                    vl = [float(loss_of(i, m))
-                          for i, m in list(batches(val_s, args.batch_tokens,
-                                                   random.Random(0)))[:4]]
+                    vl = [float(loss_fn(*b))
+                          for b in list(batched(val_s, args.batch_tokens,
+                                                random.Random(0)))[:4]]
                 print(f"[train] step {step}/{args.steps} "
                       f"loss {sum(losses[-100:])/len(losses[-100:]):.3f} "
                       f"val {sum(vl)/len(vl):.3f} "
@@ -278,6 +311,8 @@ def main():
     p.add_argument("--config", default="policy-small")
     p.add_argument("--max-len", type=int, default=1536)
     p.add_argument("--batch-tokens", type=int, default=65536)
+    p.add_argument("--packed", action="store_true",
+                   help="packed batches through the HIP training ops")
     p.add_argument("--lr", type=float, default=6e-4)
     p.add_argument("--out", default="gpurun_out/policy_ckpt")
     p.add_argument("--eval", action="store_true")

@@ -678,3 +678,122 @@ def test_attention_gpu_part_of_the_gradients():
         out = ops.packed_attention(*parts, starts)
         got = torch.autograd.grad(out, [parts[i] for i in ask], dout)
         assert all(torch.equal(g, want[i]) for g, i in zip(got, ask))
+
+
+# -------------------------------------------------------------- all together
+
+def test_pack_samples():
+    from runbookai_amd.engine.train import pack_samples
+
+    ids, starts, targets = pack_samples([([5, 6, 7, 8], 2), ([], 0), ([9], 0), ([1, 2], 1)])
+    assert ids.tolist() == [5, 6, 7, 8, 9, 1, 2]
+    assert starts.tolist() == [0, 4, 4, 5, 7]
+    assert targets.tolist() == [-100, 7, 8, -100, -100, 2, -100]
+
+
+def test_packed_model_agrees_with_padded():
+    """Logits and gradients of a packed batch are those of each sequence by
+    itself; both in fp32, whose sums differ in order only."""
+    from runbookai_amd.engine.train import CONFIGS, TrainableLlama, pack_samples
+
+    torch.manual_seed(0)
+    model = TrainableLlama(CONFIGS["tiny"])
+    gen = torch.Generator().manual_seed(1)
+    samples = [(torch.randint(0, 4096, (n,), generator=gen).tolist(), n // 2) for n in (7, 1, 12)]
+    ids, starts, targets = pack_samples(samples)
+    ops.cross_entropy(model.forward_packed(ids, starts), targets).backward()
+    packed = {n: p.grad.clone() for n, p in model.named_parameters()}
+    model.zero_grad()
+    logits, labels = [], []
+    for tokens, answer in samples:
+        logits.append(model(torch.tensor(tokens)[None])[0])
+        t = torch.tensor(tokens[1:] + [-100])
+        t[:max(0, answer - 1)] = -100
+        labels.append(t)
+    torch.testing.assert_close(model.forward_packed(ids, starts), torch.cat(logits),
+                               rtol=1e-4, atol=1e-5)
+    torch.nn.functional.cross_entropy(torch.cat(logits), torch.cat(labels)).backward()
+    for n, p in model.named_parameters():
+        torch.testing.assert_close(packed[n], p.grad, rtol=1e-3, atol=1e-6, msg=n)
+
+
+def test_packed_model_refuses():
+    from runbookai_amd.engine.train import CONFIGS, TrainableLlama
+
+    model = TrainableLlama(CONFIGS["tiny"])
+    ids = torch.zeros(10, dtype=torch.long)
+    for starts in ([0, 11], [0, 4, 3], [-1, 10], []):
+        with pytest.raises(ValueError):
+            model.forward_packed(ids, torch.tensor(starts, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        model.forward_packed(ids[None], torch.tensor([0, 10]))
+    with pytest.raises(ValueError):
+        model.forward_packed(torch.zeros(5000, dtype=torch.long), torch.tensor([0, 5000]))
+    assert model.forward_packed(ids[:0], torch.tensor([0])).shape == (0, 4096)
+
+
+def test_packed_training_script_runs(tmp_path):
+    import subprocess
+    import sys
+
+    proc = subprocess.run(
+        [sys.executable, "scripts/train_policy.py", "--cases", "4", "--steps", "2", "--out",
+         str(tmp_path), "--max-len", "768", "--batch-tokens", "2048", "--packed"],
+        capture_output=True, text=True, timeout=600)
+    assert proc.returncode == 0, proc.stderr[-1500:]
+    assert (tmp_path / "model.safetensors").exists()
+
+
+@gpu
+def test_training_step_gpu():
+    """Attention, loss and clipping as a step runs them; each stage is held to
+    64 bits on what the stage before gave it."""
+    lens, hq, hk, d, vocab = [150, 0, 1, 200], 4, 2, 64, 1000
+    q, k, v, _ = _inputs(lens, (hq, hk), d, pad=9, device="cuda")
+    starts = _starts(lens)
+    T = q.shape[0]
+    gen = torch.Generator().manual_seed(5)
+    w = torch.nn.Parameter((torch.randn(vocab, hq * d, generator=gen) * 0.05).cuda())
+    targets = torch.randint(0, vocab, (T,), generator=gen).cuda()
+    targets[::3] = -100
+    targets[starts[-1]:] = -100
+    parts = [torch.nn.Parameter(x) for x in (q, k, v)]
+    out = ops.packed_attention(*parts, torch.tensor(starts, device="cuda"))
+    out.retain_grad()
+    logits = out.reshape(T, -1).float() @ w.t()
+    logits.retain_grad()
+    loss = ops.cross_entropy(logits, targets)
+    loss.backward()
+    one = torch.ones((), device="cuda")
+    _check_loss((loss.detach(), logits.grad), loss_oracle(logits, targets, "mean", one),
+                torch.float32, one)
+    want, tol = attention_oracle(q, k, v, out.grad, starts, 1 / math.sqrt(d))
+    _within([out.detach()] + [p.grad for p in parts], want, tol)
+    _check_clip(parts + [w], 0.01)
+
+
+@gpu
+def test_packed_model_gpu():
+    """The policy's forward and backward pass under autocast, against fp32 on
+    the host. A row passes some 16 roundings to bf16 on its way to a logit."""
+    from runbookai_amd.engine.train import CONFIGS, TrainableLlama, pack_samples
+
+    torch.manual_seed(0)
+    model = TrainableLlama(CONFIGS["tiny"])
+    gen = torch.Generator().manual_seed(1)
+    samples = [(torch.randint(0, 4096, (n,), generator=gen).tolist(), n // 3)
+               for n in (200, 3, 1, 333, 64)]
+    ids, starts, targets = pack_samples(samples)
+    want = model.forward_packed(ids, starts)
+    want_loss = ops.cross_entropy(want, targets)
+    model = model.cuda()
+    with torch.autocast(device_type="cuda", dtype=torch.bfloat16):
+        got = model.forward_packed(ids.cuda(), starts)
+    loss = ops.cross_entropy(got, targets.cuda())
+    slack = 16 * H * float(want.detach().abs().max())
+    assert (got.detach().float().cpu() - want.detach()).abs().max() <= slack
+    assert abs(float(loss.detach()) - float(want_loss.detach())) <= slack
+    loss.backward()
+    norm = ops.clip_grad_norm_(model.parameters(), 0.5, error_if_nonfinite=True)
+    assert float(norm) > 0
+    assert float(ops.grad_norm(model.parameters())) <= 0.5 * (1 + 1e-5)
