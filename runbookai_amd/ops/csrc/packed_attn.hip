@@ -146,32 +146,36 @@ struct Mover {
     static constexpr int STEP = THREADS / (D / 8);   // rows that the workgroup moves at a time
     static constexpr int LOADS = N / STEP;           // that each wave issues for a tile
     static_assert(STEP % 16 == 0 && N % STEP == 0, "turn(row + STEP) is turn(row)");
-    unsigned row, chunk, off;
+    int row;
+    unsigned chunk, off, wave;
     long pitch;   // bytes from row to row
     DEVINL explicit Mover(long stride) {
         row = threadIdx.x / (D / 8);
         chunk = ((threadIdx.x % (D / 8)) ^ turn<D>(row)) * 16;
         pitch = stride * 2;
         off = row * (unsigned)pitch + chunk;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE) * (WAVE * 16);
+    }
+    DEVINL static void issue(unsigned to, unsigned at, const char* from) {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :
+                     : "s"(to), "v"(at), "s"(from)
+                     : "memory");
     }
     DEVINL void move(const ushort_t* base, int row0, int last, char* tile) const {
         const char* from = reinterpret_cast<const char*>(base) + row0 * pitch;
-        const unsigned to = (unsigned)(unsigned long)(__attribute__((address_space(3))) char*)tile +
-                            (threadIdx.x & ~63u) * 16;
-        const bool whole = row0 + N - 1 <= last;
+        const unsigned to =
+            (unsigned)(unsigned long)(__attribute__((address_space(3))) char*)tile + wave;
+        if (row0 + N - 1 <= last) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            unsigned at = off;
-            const char* src = from + i * STEP * pitch;
-            if (!whole) {
-                src = from;
-                at = (unsigned)min((int)row + i * STEP, last - row0) * (unsigned)pitch + chunk;
-            }
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                         :
-                         : "s"(__builtin_amdgcn_readfirstlane(to + i * STEP * D * 2)), "v"(at),
-                           "s"(src)
-                         : "memory");
+            for (int i = 0; i < LOADS; ++i)
+                issue(to + i * STEP * D * 2, off, from + i * STEP * pitch);
+        } else {
+            const int r = seldom(row);
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i)
+                issue(to + i * STEP * D * 2,
+                      __umul24(min(r + i * STEP, last - row0), (unsigned)pitch) + chunk, from);
         }
     }
 };
