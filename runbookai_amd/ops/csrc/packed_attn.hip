@@ -40,6 +40,8 @@
 // far from exact as its own rounding alone; from the rounded o it was 1.50.
 #include "common.h"
 
+#include "packed_attn.h"
+
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
@@ -47,7 +49,7 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef int int4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4_t lds_short4_t;
 
-#define ROWS 128        // rows of a tile, of queries or of keys
+#define ROWS PACKED_ROWS
 #define LOG2E 1.4426950408889634f
 
 namespace {
@@ -291,23 +293,31 @@ packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
     while (((T / ROWS) >> shift) >= BUCKETS) ++shift;
     const int used = ((T / ROWS) >> shift) + 1;
     for (int i = tid; i < used; i += BUILDERS) first[i] = fill_q[i] = fill_k[i] = 0;
-    bool bad = false;
-    for (int b = tid; b <= B; b += BUILDERS) {
-        const int s = starts[b];
-        bad |= s < 0 || s > T || (b && s < starts[b - 1]);
-    }
-    const bool wrong = __syncthreads_or(bad);
-    // sequence 0 is the rows before the first one, B + 1 those behind the last
+    // sequence 0 is the rows before the first one, B + 1 those behind the last;
+    // a wave's lanes load 64 ranges at once, so that the loads overlap
     const int lane = tid & (WAVE - 1), wid = tid / WAVE;
     constexpr int WAVES = BUILDERS / WAVE;
+    auto range = [&](int b, int& s, int& e) {
+        s = b > 0 && b < B + 2 ? starts[b - 1] : 0;
+        e = b <= B ? starts[b] : b < B + 2 ? T : 0;
+    };
+    const int mine = wid + lane * WAVES;
+    int s0, e0;
+    range(mine, s0, e0);   // all there are, up to 1022 sequences
+    bool bad = s0 < 0 || e0 > T || e0 < s0;
+    for (int b = mine + BUILDERS; b < B + 2; b += BUILDERS) {
+        int s, e;
+        range(b, s, e);
+        bad |= s < 0 || e > T || e < s;
+    }
+    const bool wrong = __syncthreads_or(bad);
     auto each = [&](auto use) {
         for (int b0 = wid; b0 < B + 2; b0 += BUILDERS) {
-            // 64 sequences' ranges at once, so that their loads overlap
-            const int b = b0 + lane * WAVES;
-            int s = 0, e = b || !wrong ? 0 : T;
-            if (b < B + 2 && !wrong) {
-                s = b ? starts[b - 1] : 0;
-                e = b <= B ? starts[b] : T;
+            int s = s0, e = e0;
+            if (b0 != wid) range(b0 + lane * WAVES, s, e);
+            if (wrong) {
+                s = 0;
+                e = b0 + lane == 0 ? T : 0;
             }
             for (int j = 0; j < WAVE && b0 + j * WAVES < B + 2; ++j) {
                 const int sj = __shfl(s, j, WAVE), ej = __shfl(e, j, WAVE);
@@ -350,20 +360,48 @@ packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
         by_query[i] = by_key[i] = int4_t{0, 0, 0, 0};
 }
 
+// Without a table (tiles null): tile `p` in the order of the sequences, found by
+// every wave for itself, a lane a sequence.  For up to PACKED_FEW sequences and so few
+// workgroups that all run at once, when the order does not matter: it saves a
+// launch that is 3 us on its way and 3 us of host time.
+DEVINL int4_t find_tile(const int* __restrict__ starts, int B, int T, int p) {
+    const int b = threadIdx.x & (WAVE - 1);
+    int s = b > 0 && b < B + 2 ? starts[b - 1] : 0;
+    int e = b <= B ? starts[b] : b < B + 2 ? T : 0;
+    const bool wrong = __any(s < 0 || e > T || e < s);
+    if (wrong) {
+        s = 0;
+        e = b == 0 ? T : 0;
+    }
+    const int n = (e - s + ROWS - 1) / ROWS;
+    int upto = n;
+#pragma unroll
+    for (int off = 1; off < WAVE; off <<= 1) {
+        const int v = __shfl_up(upto, off, WAVE);
+        if (b >= off) upto += v;
+    }
+    const int seq = __popcll(__ballot(upto <= p));   // those that end before it
+    if (seq == WAVE) return int4_t{0, 0, 0, 0};
+    s = __builtin_amdgcn_readlane(s, seq);
+    e = __builtin_amdgcn_readlane(e, seq);
+    const int r0 = s + (p - __builtin_amdgcn_readlane(upto - n, seq)) * ROWS;
+    const bool real = !wrong && seq > 0 && seq <= B;
+    return int4_t{r0, min(r0 + ROWS, e), real ? s : r0, real ? e : wrong ? -1 : r0};
+}
+
 // ------------------------------------------------------------------ forward
 //
 // A workgroup takes a tile of 128 rows of one head, a wave 32 of the rows.  64
 // keys at a time stand in LDS, the next ones are on their way there meanwhile.
 template <int D, bool SAVE>
 __global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
-packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
-                       const ushort_t* __restrict__ k, long kt, long kh,
-                       const ushort_t* __restrict__ v, long vt, long vh,
-                       const int4_t* __restrict__ tiles, ushort_t* __restrict__ out,
-                       ushort_t* __restrict__ out_lo, float* __restrict__ lse, int T, int Hq,
-                       int Hk, float scale) {
-    const int4_t tile = tiles[blockIdx.x / Hq];
+packed_attn_fwd_kernel(const PackedArgs a) {
+    const int T = a.T, Hq = a.Hq, Hk = a.Hk;
+    const int4_t* tiles = (const int4_t*)a.tiles;
+    const int4_t tile = tiles ? tiles[blockIdx.x / Hq] : find_tile(a.starts, a.B, T, blockIdx.x / Hq);
     const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
+    if (SAVE && !tiles && blockIdx.x == 0)   // for the backward pass, which runs later
+        for (int i = threadIdx.x; i <= a.B; i += 256) a.kept_starts[i] = a.starts[i];
     if (row0 >= row1) return;
     // the kv head runs fastest: workgroups go round the 8 XCDs in turn, so with
     // 1, 2, 4 or 8n of them an XCD's L2 sees the same heads' keys every time
@@ -377,7 +415,7 @@ packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     const int wrow = row0 + wid * 32;
     const int row = wrow + (lane & 31);
     const bool mine = row < row1;
-    const float c2 = scale * LOG2E;
+    const float c2 = a.scale * LOG2E;
 
     // two tiles of keys, two of values
     constexpr int TILE = 64 * D * 2;
@@ -385,14 +423,13 @@ packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     const Lane<D> lanes(lane);
 
     bf16x8_t qf[D / 16];
-    load_row<D>(qf, q + row * qt + h * qh, mine, hi);
+    load_row<D>(qf, a.q + row * a.qt + h * a.qh, mine, hi);
     f32x16_t acc[D / 32];
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) acc[db] = zero16();
     float m = -INFINITY, l = 0.f;
-    k += hk * kh;
-    v += hk * vh;
-    const Mover<D, 64, 256> mk(kt), mv(vt);
+    const ushort_t *k = a.k + hk * a.kh, *v = a.v + hk * a.vh;
+    const Mover<D, 64, 256> mk(a.kt), mv(a.vt);
     const int steps = (kv1 - kv0 + 63) / 64;
     auto fetch = [&](int it) {
         mk.move(k, kv0 + it * 64, kv1 - 1, lds + (it & 1) * TILE);
@@ -459,9 +496,9 @@ packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     }
     l = both_sum(l);
     const long to = ((long)row * Hq + h) * D;
-    store_row<D>(acc, seq1 < 0 ? NAN : real ? 1.f / l : 0.f, out + to, hi,
-                 SAVE ? out_lo + to : nullptr, mine);
-    if (SAVE && mine && hi == 0) lse[(long)h * T + row] = m + __builtin_amdgcn_logf(l);
+    store_row<D>(acc, seq1 < 0 ? NAN : real ? 1.f / l : 0.f, a.out + to, hi,
+                 SAVE ? a.out_lo + to : nullptr, mine);
+    if (SAVE && mine && hi == 0) a.lse[(long)h * T + row] = m + __builtin_amdgcn_logf(l);
 }
 
 // ----------------------------------------------------------------------- dq
@@ -469,15 +506,10 @@ packed_attn_fwd_kernel(const ushort_t* __restrict__ q, long qt, long qh,
 // The forward kernel's split.  Also writes -delta for the kernel below.
 template <int D>
 __global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
-packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
-                      const ushort_t* __restrict__ k, long kt, long kh,
-                      const ushort_t* __restrict__ v, long vt, long vh,
-                      const ushort_t* __restrict__ dout, long ot, long oh,
-                      const ushort_t* __restrict__ out, const ushort_t* __restrict__ out_lo,
-                      const int4_t* __restrict__ tiles,
-                      const float* __restrict__ lse, float* __restrict__ delta,
-                      ushort_t* __restrict__ dq, int T, int Hq, int Hk, float scale) {
-    const int4_t tile = tiles[blockIdx.x / Hq];
+packed_attn_dq_kernel(const PackedArgs a) {
+    const int T = a.T, Hq = a.Hq, Hk = a.Hk;
+    const int4_t* tiles = (const int4_t*)a.tiles;
+    const int4_t tile = tiles ? tiles[blockIdx.x / Hq] : find_tile(a.starts, a.B, T, blockIdx.x / Hq);
     const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
     if (row0 >= row1) return;
     const int hk = blockIdx.x % Hk;
@@ -490,15 +522,14 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     const int wrow = row0 + wid * 32;
     const int row = wrow + (lane & 31);
     const bool mine = row < row1;
-    const float c2 = scale * LOG2E;
+    const float c2 = a.scale * LOG2E;
 
     constexpr int TILE = 64 * D * 2;
     __shared__ __attribute__((aligned(256))) char lds[4 * TILE];
     const Lane<D> lanes(lane);
 
-    k += hk * kh;
-    v += hk * vh;
-    const Mover<D, 64, 256> mk(kt), mv(vt);
+    const ushort_t *k = a.k + hk * a.kh, *v = a.v + hk * a.vh;
+    const Mover<D, 64, 256> mk(a.kt), mv(a.vt);
     const int steps = (kv1 - kv0 + 63) / 64;
     auto fetch = [&](int it) {
         mk.move(k, kv0 + it * 64, kv1 - 1, lds + (it & 1) * TILE);
@@ -506,14 +537,14 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     };
     if (steps > 0) fetch(0);
     bf16x8_t qf[D / 16], of[D / 16];
-    load_row<D>(qf, q + row * qt + h * qh, mine, hi);
-    load_row<D>(of, dout + row * ot + h * oh, mine, hi);
-    float ls = mine ? lse[(long)h * T + row] : 0.f;
+    load_row<D>(qf, a.q + row * a.qt + h * a.qh, mine, hi);
+    load_row<D>(of, a.dout + row * a.ot + h * a.oh, mine, hi);
+    float ls = mine ? a.lse[(long)h * T + row] : 0.f;
     float dl = 0.f;
     {
         bf16x8_t o[D / 16], rest[D / 16];
-        load_row<D>(o, out + ((long)row * Hq + h) * D, mine, hi);
-        load_row<D>(rest, out_lo + ((long)row * Hq + h) * D, mine, hi);
+        load_row<D>(o, a.out + ((long)row * Hq + h) * D, mine, hi);
+        load_row<D>(rest, a.out_lo + ((long)row * Hq + h) * D, mine, hi);
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
 #pragma unroll
@@ -562,7 +593,7 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
         dl = both_sum(sum);
         if (steps > 0) fetch(0);
     }
-    if (mine && hi == 0) delta[(long)h * T + row] = -dl;
+    if (mine && hi == 0) a.delta[(long)h * T + row] = -dl;
     sweep([&](f32x16_t& s, f32x16_t& dp, int key0, const Lane<D>& at, int sub) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -582,7 +613,7 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
                                acc[db]);
         }
     });
-    store_row<D>(acc, seq1 < 0 ? NAN : scale, dq + ((long)row * Hq + h) * D, hi, nullptr, mine);
+    store_row<D>(acc, seq1 < 0 ? NAN : a.scale, a.dq + ((long)row * Hq + h) * D, hi, nullptr, mine);
 }
 
 // ------------------------------------------------------------------- dk, dv
@@ -593,17 +624,14 @@ packed_attn_dq_kernel(const ushort_t* __restrict__ q, long qt, long qh,
 // two such teams the queries, and their sums are joined at the end.
 template <int D, int KS, int QB, int NBUF>
 __global__ void __launch_bounds__(KS * 128, D == 128 ? 2 : 3)
-packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
-                       const ushort_t* __restrict__ k, long kt, long kh,
-                       const ushort_t* __restrict__ v, long vt, long vh,
-                       const ushort_t* __restrict__ dout, long ot, long oh,
-                       const int4_t* __restrict__ tiles, const float* __restrict__ lse,
-                       const float* __restrict__ delta, ushort_t* __restrict__ dk,
-                       ushort_t* __restrict__ dv, int T, int Hq, int Hk, float scale) {
+packed_attn_dkv_kernel(const PackedArgs a) {
+    const int T = a.T, Hq = a.Hq, Hk = a.Hk;
+    const int4_t* tiles = a.tiles ? (const int4_t*)a.tiles + a.max_tiles : nullptr;
     constexpr int PARTS = 4 / KS;
     const int hk = blockIdx.x % Hk;
     const int group = Hq / Hk;
-    const int4_t tile = tiles[blockIdx.x / (Hk * PARTS)];
+    const int at_tile = blockIdx.x / (Hk * PARTS);
+    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile);
     const int row0 = tile[0] + blockIdx.x / Hk % PARTS * (KS * 32);
     const int row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
     if (row0 >= row1) return;
@@ -615,7 +643,7 @@ packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     const int wkey = row0 + wid % KS * 32;
     const int key = wkey + (lane & 31);
     const bool mine = key < row1;
-    const float c2 = scale * LOG2E;
+    const float c2 = a.scale * LOG2E;
 
     // NBUF tiles of queries, as many of their outputs' gradients, and each row's
     // log-sum and negated delta
@@ -631,21 +659,21 @@ packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
 
     bf16x8_t kf[D / 16], vf[D / 16];
     f32x16_t ak[D / 32], av[D / 32];
-    load_row<D>(kf, k + key * kt + hk * kh, mine, hi);
-    load_row<D>(vf, v + key * vt + hk * vh, mine, hi);
+    load_row<D>(kf, a.k + key * a.kt + hk * a.kh, mine, hi);
+    load_row<D>(vf, a.v + key * a.vt + hk * a.vh, mine, hi);
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) ak[db] = av[db] = zero16();
 
-    const Mover<D, QB, KS * 128> mq(qt), mo(ot);
+    const Mover<D, QB, KS * 128> mq(a.qt), mo(a.ot);
     // each wave also moves 64 rows' log-sums or deltas (where there are more
     // waves than parts, two move the same)
     static_assert(QB % 64 == 0 && KS * 2 % (QB / 32) == 0, "by wave");
     const int part = wid % (QB / 32) / 2;
     const bool sums = wid % 2 == 0;
     auto fetch = [&](int h, int r0, int buf) {
-        mq.move(q + h * qh, r0, seq1 - 1, ql + buf * TILE);
-        mo.move(dout + h * oh, r0, seq1 - 1, ol + buf * TILE);
-        const float* from = (sums ? lse : delta) + (long)h * T;
+        mq.move(a.q + h * a.qh, r0, seq1 - 1, ql + buf * TILE);
+        mo.move(a.dout + h * a.oh, r0, seq1 - 1, ol + buf * TILE);
+        const float* from = (sums ? a.lse : a.delta) + (long)h * T;
         const float* to = (sums ? lds.ls[buf] : lds.dl[buf]) + part * 64;
         move64(from, min(r0 + part * 64 + lane, seq1 - 1), to);
     };
@@ -754,116 +782,57 @@ packed_attn_dkv_kernel(const ushort_t* __restrict__ q, long qt, long qh,
     const long to = ((long)key * Hk + hk) * D;
     if (team) {
         add(ak, join + KS * 32 * D);
-        store_row<D>(ak, seq1 < 0 ? NAN : scale, dk + to, hi, nullptr, mine);
+        store_row<D>(ak, seq1 < 0 ? NAN : a.scale, a.dk + to, hi, nullptr, mine);
     } else {
         add(av, join);
-        store_row<D>(av, seq1 < 0 ? NAN : 1.f, dv + to, hi, nullptr, mine);
+        store_row<D>(av, seq1 < 0 ? NAN : 1.f, a.dv + to, hi, nullptr, mine);
     }
 }
 
 // ---------------------------------------------------------------- launchers
-// Each returns the launch's hipError_t.  `tiles` holds max_tiles tiles by
-// query and as many by key.
+// Each returns the launch's hipError_t.
 
-extern "C" int launch_packed_tiles(const void* starts, int B, int T, int max_tiles,
-                                   void* tiles, void* stream) {
-    int4_t* a = (int4_t*)tiles;
+extern "C" int launch_packed_tiles(const PackedArgs* a, void* stream) {
+    int4_t* tiles = (int4_t*)a->tiles;
     hipLaunchKernelGGL(packed_tiles_kernel, dim3(1), dim3(BUILDERS), 0, (hipStream_t)stream,
-                       (const int*)starts, B, T, max_tiles, a, a + max_tiles);
+                       a->starts, a->B, a->T, a->max_tiles, tiles, tiles + a->max_tiles);
+    return (int)hipGetLastError();
+}
+
+extern "C" int launch_packed_attn_fwd(const PackedArgs* a, void* stream) {
+    const dim3 grid((unsigned)a->max_tiles * a->Hq), block(256);
+    const hipStream_t st = (hipStream_t)stream;
+    if (a->D == 128) {
+        if (a->lse) hipLaunchKernelGGL((packed_attn_fwd_kernel<128, true>), grid, block, 0, st, *a);
+        else hipLaunchKernelGGL((packed_attn_fwd_kernel<128, false>), grid, block, 0, st, *a);
+    } else {
+        if (a->lse) hipLaunchKernelGGL((packed_attn_fwd_kernel<64, true>), grid, block, 0, st, *a);
+        else hipLaunchKernelGGL((packed_attn_fwd_kernel<64, false>), grid, block, 0, st, *a);
+    }
+    return (int)hipGetLastError();
+}
+
+extern "C" int launch_packed_attn_dq(const PackedArgs* a, void* stream) {
+    const dim3 grid((unsigned)a->max_tiles * a->Hq), block(256);
+    const hipStream_t st = (hipStream_t)stream;
+    if (a->D == 128) hipLaunchKernelGGL((packed_attn_dq_kernel<128>), grid, block, 0, st, *a);
+    else hipLaunchKernelGGL((packed_attn_dq_kernel<64>), grid, block, 0, st, *a);
     return (int)hipGetLastError();
 }
 
 namespace {
 
-template <int D, bool SAVE>
-void fwd(const void* q, long qt, long qh, const void* k, long kt, long kh,
-         const void* v, long vt, long vh, const void* tiles, int max_tiles, void* out,
-         void* out_lo, void* lse, int T, int Hq, int Hk, float scale, hipStream_t st) {
-    const int4_t* a = (const int4_t*)tiles;
-    hipLaunchKernelGGL((packed_attn_fwd_kernel<D, SAVE>),
-                       dim3((unsigned)max_tiles * Hq), dim3(256), 0, st,
-                       (const ushort_t*)q, qt, qh, (const ushort_t*)k, kt, kh,
-                       (const ushort_t*)v, vt, vh, a,
-                       (ushort_t*)out, (ushort_t*)out_lo, (float*)lse, T, Hq, Hk, scale);
-}
-
-template <int D>
-void dq_(const void* q, long qt, long qh, const void* k, long kt, long kh,
-         const void* v, long vt, long vh, const void* dout, long ot, long oh,
-         const void* out, const void* out_lo, const void* tiles, int max_tiles,
-         const void* lse, void* delta, void* dq, int T, int Hq, int Hk, float scale,
-         hipStream_t st) {
-    const int4_t* a = (const int4_t*)tiles;
-    hipLaunchKernelGGL((packed_attn_dq_kernel<D>),
-                       dim3((unsigned)max_tiles * Hq), dim3(256), 0, st,
-                       (const ushort_t*)q, qt, qh, (const ushort_t*)k, kt, kh,
-                       (const ushort_t*)v, vt, vh, (const ushort_t*)dout, ot, oh,
-                       (const ushort_t*)out, (const ushort_t*)out_lo, a, (const float*)lse,
-                       (float*)delta, (ushort_t*)dq, T, Hq, Hk, scale);
-}
-
 template <int D, int KS, int QB, int NBUF>
-void dkv(const void* q, long qt, long qh, const void* k, long kt, long kh,
-         const void* v, long vt, long vh, const void* dout, long ot, long oh,
-         const void* tiles, int max_tiles, const void* lse, const void* delta,
-         void* dk, void* dv, int T, int Hq, int Hk, float scale, hipStream_t st) {
-    const int4_t* a = (const int4_t*)tiles;
+void dkv(const PackedArgs* a, hipStream_t st) {
     hipLaunchKernelGGL((packed_attn_dkv_kernel<D, KS, QB, NBUF>),
-                       dim3((unsigned)max_tiles * Hk * (4 / KS)), dim3(KS * 128), 0, st,
-                       (const ushort_t*)q, qt, qh, (const ushort_t*)k, kt, kh,
-                       (const ushort_t*)v, vt, vh, (const ushort_t*)dout, ot, oh,
-                       a + max_tiles,
-                       (const float*)lse, (const float*)delta, (ushort_t*)dk,
-                       (ushort_t*)dv, T, Hq, Hk, scale);
+                       dim3((unsigned)a->max_tiles * a->Hk * (4 / KS)), dim3(KS * 128), 0, st,
+                       *a);
 }
 
 }  // namespace
 
-// out_lo and lse are null where no backward pass will follow.
-extern "C" int launch_packed_attn_fwd(const void* q, long qt, long qh, const void* k,
-                                      long kt, long kh, const void* v, long vt, long vh,
-                                      const void* tiles, int max_tiles, void* out,
-                                      void* out_lo, void* lse, int T, int Hq, int Hk, int D, float scale, void* stream) {
-#define FWD(d, s)                                                                          \
-    fwd<d, s>(q, qt, qh, k, kt, kh, v, vt, vh, tiles, max_tiles, out, out_lo, lse, T, Hq, Hk, \
-              scale, (hipStream_t)stream)
-    if (D == 128) {
-        if (lse) FWD(128, true);
-        else FWD(128, false);
-    } else {
-        if (lse) FWD(64, true);
-        else FWD(64, false);
-    }
-#undef FWD
-    return (int)hipGetLastError();
-}
-
-extern "C" int launch_packed_attn_dq(const void* q, long qt, long qh, const void* k,
-                                     long kt, long kh, const void* v, long vt, long vh,
-                                     const void* dout, long ot, long oh, const void* out,
-                                     const void* out_lo, const void* tiles, int max_tiles,
-                                     const void* lse, void* delta, void* dq, int T, int Hq,
-                                     int Hk, int D, float scale, void* stream) {
-    if (D == 128)
-        dq_<128>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, out, out_lo, tiles, max_tiles,
-                 lse, delta, dq, T, Hq, Hk, scale, (hipStream_t)stream);
-    else
-        dq_<64>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, out, out_lo, tiles, max_tiles,
-                lse, delta, dq, T, Hq, Hk, scale, (hipStream_t)stream);
-    return (int)hipGetLastError();
-}
-
-extern "C" int launch_packed_attn_dkv(const void* q, long qt, long qh, const void* k,
-                                      long kt, long kh, const void* v, long vt, long vh,
-                                      const void* dout, long ot, long oh, const void* tiles,
-                                      int max_tiles, const void* lse, const void* delta,
-                                      void* dk, void* dv, int T, int Hq, int Hk, int D,
-                                      float scale, void* stream) {
-    if (D == 128)
-        dkv<128, 4, 128, 2>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, tiles, max_tiles, lse,
-                 delta, dk, dv, T, Hq, Hk, scale, (hipStream_t)stream);
-    else
-        dkv<64, 2, 64, 3>(q, qt, qh, k, kt, kh, v, vt, vh, dout, ot, oh, tiles, max_tiles, lse,
-                delta, dk, dv, T, Hq, Hk, scale, (hipStream_t)stream);
+extern "C" int launch_packed_attn_dkv(const PackedArgs* a, void* stream) {
+    if (a->D == 128) dkv<128, 4, 128, 2>(a, (hipStream_t)stream);
+    else dkv<64, 2, 64, 3>(a, (hipStream_t)stream);
     return (int)hipGetLastError();
 }

@@ -14,20 +14,13 @@
 #include <vector>
 
 #include "grad_norm.h"
+#include "packed_attn.h"
 
 extern "C" {
-int launch_packed_tiles(const void*, int, int, int, void*, void*);
-int launch_packed_attn_fwd(const void*, long, long, const void*, long, long, const void*,
-                           long, long, const void*, int, void*, void*, void*, int, int, int,
-                           int, float, void*);
-int launch_packed_attn_dq(const void*, long, long, const void*, long, long, const void*,
-                          long, long, const void*, long, long, const void*, const void*,
-                          const void*, int, const void*, void*, void*, int, int, int, int,
-                          float, void*);
-int launch_packed_attn_dkv(const void*, long, long, const void*, long, long, const void*,
-                           long, long, const void*, long, long, const void*, int,
-                           const void*, const void*, void*, void*, int, int, int, int, float,
-                           void*);
+int launch_packed_tiles(const PackedArgs*, void*);
+int launch_packed_attn_fwd(const PackedArgs*, void*);
+int launch_packed_attn_dq(const PackedArgs*, void*);
+int launch_packed_attn_dkv(const PackedArgs*, void*);
 int launch_xent_fwd(int, const void*, long, const void*, long, int, int, void*, void*, void*,
                     void*, void*);
 int xent_parts(int, int);
@@ -82,11 +75,10 @@ void check_rows(const Tensor& t, const char* name, const Tensor& like) {
     TORCH_CHECK(fits(t), name, " has too many or too wide heads");
 }
 
-long tiles_for(long T, long B) { return T / 128 + B + 2; }
+unsigned short* bf16(const Tensor& t) { return (unsigned short*)t.data_ptr(); }
 
-struct Sizes { int T, Hq, Hk, D; };
-
-Sizes check_qkv(const Tensor& q, const Tensor& k, const Tensor& v) {
+// The arguments that both passes have
+PackedArgs packed_args(const Tensor& q, const Tensor& k, const Tensor& v, double scale) {
     check_rows(q, "q", q);
     check_rows(k, "k", q);
     check_rows(v, "v", q);
@@ -98,75 +90,98 @@ Sizes check_qkv(const Tensor& q, const Tensor& k, const Tensor& v) {
     TORCH_CHECK(Hk > 0 && Hq > 0 && Hq % Hk == 0,
                 "query heads must be a multiple of key/value heads");
     TORCH_CHECK(T < (1L << 30), "at most 2^30 tokens");
-    return {(int)T, (int)Hq, (int)Hk, (int)D};
+    PackedArgs a = {};
+    a.q = bf16(q); a.qt = q.stride(0); a.qh = q.stride(1);
+    a.k = bf16(k); a.kt = k.stride(0); a.kh = k.stride(1);
+    a.v = bf16(v); a.vt = v.stride(0); a.vh = v.stride(1);
+    a.T = (int)T; a.Hq = (int)Hq; a.Hk = (int)Hk; a.D = (int)D;
+    a.scale = (float)scale;
+    return a;
 }
 
-// -> out and, with `save`, what its rounding left over, lse and tiles
-std::vector<Tensor> packed_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor starts, double scale,
-                                    bool save) {
-    const Sizes s = check_qkv(q, k, v);
+// Sets where the tiles are: `where` holds a table of tiles or, for few
+// sequences in few tiles, just their starts (a workgroup of 128 rows for each
+// head: up to 512 run at once whatever the head dim).
+void packed_tiles(PackedArgs& a, const Tensor& where, long B) {
+    const long most = a.T / PACKED_ROWS + B + 2;
+    TORCH_CHECK(2 * most * a.Hq < (1L << 31), "too many sequences");
+    a.B = (int)B;
+    a.max_tiles = (int)most;
+    if (B <= PACKED_FEW && most * a.Hq <= 512) a.starts = where.data_ptr<int>();
+    else a.tiles = where.data_ptr();
+}
+
+bool by_table(const PackedArgs& a) { return a.tiles != nullptr; }
+
+// -> out and, with `save`, what its rounding left over, lse and where the tiles are
+std::vector<Tensor> packed_attn_fwd(const Tensor& q, const Tensor& k, const Tensor& v,
+                                    const Tensor& starts, double scale, bool save) {
+    PackedArgs a = packed_args(q, k, v, scale);
     TORCH_CHECK(starts.device() == q.device() && starts.scalar_type() == torch::kInt32 &&
                     starts.is_contiguous() && starts.dim() == 1 && starts.numel() >= 1,
                 "seq_starts must be a dense int32 vector on the device of q");
-    const long B = starts.numel() - 1, max_tiles = tiles_for(s.T, B);
-    TORCH_CHECK(2 * max_tiles * s.Hq < (1L << 31), "too many sequences");
     const c10::cuda::CUDAGuard guard(q.device());
     const auto opt = q.options();
-    Tensor out = torch::empty({s.T, s.Hq, s.D}, opt), rest, lse;
-    Tensor tiles = torch::empty({8 * max_tiles}, opt.dtype(torch::kInt32));
+    const Tensor out = torch::empty({a.T, a.Hq, a.D}, opt);
+    Tensor rest, lse, where;
+    packed_tiles(a, starts, starts.numel() - 1);
+    a.out = bf16(out);
+    if (by_table(a)) where = torch::empty({8 * (long)a.max_tiles}, opt.dtype(torch::kInt32));
     if (save) {
         rest = torch::empty_like(out);
-        lse = torch::empty({s.Hq, s.T}, opt.dtype(torch::kFloat32));
+        lse = torch::empty({a.Hq, a.T}, opt.dtype(torch::kFloat32));
+        a.out_lo = bf16(rest);
+        a.lse = lse.data_ptr<float>();
+        if (!by_table(a)) {
+            where = torch::empty_like(starts);
+            a.kept_starts = where.data_ptr<int>();
+        }
     }
-    if (s.T > 0) {
+    if (a.T > 0) {
         void* st = stream_of(q);
-        launched(launch_packed_tiles(starts.data_ptr(), (int)B, s.T, (int)max_tiles,
-                                     tiles.data_ptr(), st), "packed_attention");
-        launched(launch_packed_attn_fwd(
-                     q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
-                     k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), tiles.data_ptr(),
-                     (int)max_tiles, out.data_ptr(), save ? rest.data_ptr() : nullptr,
-                     save ? lse.data_ptr() : nullptr, s.T, s.Hq, s.Hk, s.D, (float)scale, st),
-                 "packed_attention");
+        if (by_table(a)) {
+            a.starts = starts.data_ptr<int>();
+            a.tiles = where.data_ptr();
+            launched(launch_packed_tiles(&a, st), "packed_attention");
+        }
+        launched(launch_packed_attn_fwd(&a, st), "packed_attention");
     }
     if (!save) return {out};
-    return {out, rest, lse, tiles};
+    return {out, rest, lse, where};
 }
 
 // -> dq, dk, dv (the last two undefined without `keys`)
-std::vector<Tensor> packed_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out,
-                                    Tensor rest, Tensor lse, Tensor tiles, double scale,
+std::vector<Tensor> packed_attn_bwd(const Tensor& dout, const Tensor& q, const Tensor& k,
+                                    const Tensor& v, const Tensor& out, const Tensor& rest,
+                                    const Tensor& lse, const Tensor& where, long B, double scale,
                                     bool keys) {
-    const Sizes s = check_qkv(q, k, v);
+    PackedArgs a = packed_args(q, k, v, scale);
     check_rows(dout, "the gradient", q);
     TORCH_CHECK(dout.sizes() == q.sizes(), "the gradient must have the shape of q");
-    const long max_tiles = tiles.numel() / 8;
     const c10::cuda::CUDAGuard guard(q.device());
     const auto opt = q.options();
-    Tensor dq = torch::empty({s.T, s.Hq, s.D}, opt);
+    const Tensor dq = torch::empty({a.T, a.Hq, a.D}, opt);
     Tensor dk, dv;
     if (keys) {
-        dk = torch::empty({s.T, s.Hk, s.D}, opt);
+        dk = torch::empty({a.T, a.Hk, a.D}, opt);
         dv = torch::empty_like(dk);
     }
-    Tensor delta = torch::empty_like(lse);
-    if (s.T > 0) {
+    if (a.T > 0) {
+        const Tensor delta = torch::empty_like(lse);
+        packed_tiles(a, where, B);
+        a.out = bf16(out);
+        a.out_lo = bf16(rest);
+        a.lse = lse.data_ptr<float>();
+        a.dout = bf16(dout); a.ot = dout.stride(0); a.oh = dout.stride(1);
+        a.delta = delta.data_ptr<float>();
+        a.dq = bf16(dq);
         void* st = stream_of(q);
-        launched(launch_packed_attn_dq(
-                     q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
-                     k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), dout.data_ptr(),
-                     dout.stride(0), dout.stride(1), out.data_ptr(), rest.data_ptr(),
-                     tiles.data_ptr(), (int)max_tiles, lse.data_ptr(), delta.data_ptr(),
-                     dq.data_ptr(), s.T, s.Hq, s.Hk, s.D, (float)scale, st),
-                 "packed_attention's gradient");
-        if (keys)
-            launched(launch_packed_attn_dkv(
-                         q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
-                         k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), dout.data_ptr(),
-                         dout.stride(0), dout.stride(1), tiles.data_ptr(), (int)max_tiles,
-                         lse.data_ptr(), delta.data_ptr(), dk.data_ptr(), dv.data_ptr(), s.T,
-                         s.Hq, s.Hk, s.D, (float)scale, st),
-                     "packed_attention's gradient");
+        launched(launch_packed_attn_dq(&a, st), "packed_attention's gradient");
+        if (keys) {
+            a.dk = bf16(dk);
+            a.dv = bf16(dv);
+            launched(launch_packed_attn_dkv(&a, st), "packed_attention's gradient");
+        }
     }
     return {dq, dk, dv};
 }
@@ -179,12 +194,14 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
         const auto got = packed_attn_fwd(q, k, v, starts, scale, true);
         ctx->save_for_backward({q, k, v, got[0], got[1], got[2], got[3]});
         ctx->saved_data["scale"] = scale;
+        ctx->saved_data["sequences"] = starts.numel() - 1;
         return got[0];
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                    torch::autograd::variable_list g) {
         const auto s = ctx->get_saved_variables();
         auto d = packed_attn_bwd(rows16(g[0]), s[0], s[1], s[2], s[3], s[4], s[5], s[6],
+                                 ctx->saved_data["sequences"].toInt(),
                                  ctx->saved_data["scale"].toDouble(),
                                  ctx->needs_input_grad(1) || ctx->needs_input_grad(2));
         d = once(std::move(d), "packed_attention");
