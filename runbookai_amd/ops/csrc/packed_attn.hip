@@ -393,13 +393,18 @@ DEVINL int4_t find_tile(const int* __restrict__ starts, int B, int T, int p) {
 //
 // A workgroup takes a tile of 128 rows of one head, a wave 32 of the rows.  64
 // keys at a time stand in LDS, the next ones are on their way there meanwhile.
-template <int D, bool SAVE>
+// With two TEAMS it takes half a tile, and each team half of the keys, whose
+// sums are joined at the end: for grids that leave CUs idle, where a wave's own
+// chain of steps is what takes the time.
+template <int D, int TEAMS, bool SAVE>
 __global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
 packed_attn_fwd_kernel(const PackedArgs a) {
     const int T = a.T, Hq = a.Hq, Hk = a.Hk;
     const int4_t* tiles = (const int4_t*)a.tiles;
-    const int4_t tile = tiles ? tiles[blockIdx.x / Hq] : find_tile(a.starts, a.B, T, blockIdx.x / Hq);
-    const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
+    const int at_tile = blockIdx.x / (Hq * TEAMS);
+    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile);
+    const int row0 = tile[0] + blockIdx.x / Hq % TEAMS * (ROWS / TEAMS);
+    const int row1 = min(tile[1], row0 + ROWS / TEAMS), seq0 = tile[2], seq1 = tile[3];
     if (SAVE && !tiles && blockIdx.x == 0)   // for the backward pass, which runs later
         for (int i = threadIdx.x; i <= a.B; i += 256) a.kept_starts[i] = a.starts[i];
     if (row0 >= row1) return;
@@ -412,7 +417,9 @@ packed_attn_fwd_kernel(const PackedArgs a) {
     const int lane = threadIdx.x & (WAVE - 1);
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int hi = lane >> 5;
-    const int wrow = row0 + wid * 32;
+    constexpr int SETS = 4 / TEAMS;   // of 32 rows
+    const int team = wid / SETS;
+    const int wrow = row0 + wid % SETS * 32;
     const int row = wrow + (lane & 31);
     const bool mine = row < row1;
     const float c2 = a.scale * LOG2E;
@@ -447,7 +454,7 @@ packed_attn_fwd_kernel(const PackedArgs a) {
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) {
             const int key0 = kv0 + it * 64 + sub * 32;
-            if (key0 >= wave_end) continue;
+            if (key0 >= wave_end || (TEAMS > 1 && sub != team)) continue;
             f32x16_t s = zero16();
 #pragma unroll
             for (int d = 0; d < D / 16; ++d)
@@ -494,6 +501,25 @@ packed_attn_fwd_kernel(const PackedArgs a) {
         arrived();
         __syncthreads();
     }
+    if (TEAMS > 1) {
+        // the second team's rows to the first
+        float* join = reinterpret_cast<float*>(lds) + wid % SETS * (D / 2 + 2) * 64 + lane;
+        if (team) {
+            join[0] = m;
+            join[64] = l;
+#pragma unroll
+            for (int i = 0; i < D / 2; ++i) join[(2 + i) * 64] = acc[i / 16][i % 16];
+        }
+        __syncthreads();
+        if (team) return;
+        const float m2 = join[0], to = fmaxf(m, m2), base = to == -INFINITY ? 0.f : to;
+        const float f = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+        m = to;
+        l = l * f + join[64] * f2;
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i)
+            acc[i / 16][i % 16] = acc[i / 16][i % 16] * f + join[(2 + i) * 64] * f2;
+    }
     l = both_sum(l);
     const long to = ((long)row * Hq + h) * D;
     store_row<D>(acc, seq1 < 0 ? NAN : real ? 1.f / l : 0.f, a.out + to, hi,
@@ -504,13 +530,15 @@ packed_attn_fwd_kernel(const PackedArgs a) {
 // ----------------------------------------------------------------------- dq
 //
 // The forward kernel's split.  Also writes -delta for the kernel below.
-template <int D>
+template <int D, int TEAMS>
 __global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
 packed_attn_dq_kernel(const PackedArgs a) {
     const int T = a.T, Hq = a.Hq, Hk = a.Hk;
     const int4_t* tiles = (const int4_t*)a.tiles;
-    const int4_t tile = tiles ? tiles[blockIdx.x / Hq] : find_tile(a.starts, a.B, T, blockIdx.x / Hq);
-    const int row0 = tile[0], row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
+    const int at_tile = blockIdx.x / (Hq * TEAMS);
+    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile);
+    const int row0 = tile[0] + blockIdx.x / Hq % TEAMS * (ROWS / TEAMS);
+    const int row1 = min(tile[1], row0 + ROWS / TEAMS), seq0 = tile[2], seq1 = tile[3];
     if (row0 >= row1) return;
     const int hk = blockIdx.x % Hk;
     const int h = hk * (Hq / Hk) + blockIdx.x % Hq / Hk;
@@ -519,7 +547,9 @@ packed_attn_dq_kernel(const PackedArgs a) {
     const int lane = threadIdx.x & (WAVE - 1);
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int hi = lane >> 5;
-    const int wrow = row0 + wid * 32;
+    constexpr int SETS = 4 / TEAMS;   // of 32 rows
+    const int team = wid / SETS;
+    const int wrow = row0 + wid % SETS * 32;
     const int row = wrow + (lane & 31);
     const bool mine = row < row1;
     const float c2 = a.scale * LOG2E;
@@ -569,7 +599,7 @@ packed_attn_dq_kernel(const PackedArgs a) {
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
                 const int key0 = kv0 + it * 64 + sub * 32;
-                if (key0 >= wave_end) continue;
+                if (key0 >= wave_end || (TEAMS > 1 && sub != team)) continue;
                 f32x16_t s = zero16(), dp = zero16();
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) {
@@ -582,7 +612,8 @@ packed_attn_dq_kernel(const PackedArgs a) {
             __syncthreads();
         }
     };
-    if (row0 == seq0) {
+    float* join = reinterpret_cast<float*>(lds) + wid % SETS * (D / 2) * 64 + lane;
+    if (tile[0] == seq0) {
         float sum = 0.f;
         sweep([&](f32x16_t& s, f32x16_t& dp, int key0, const Lane<D>&, int) {
 #pragma unroll
@@ -590,10 +621,17 @@ packed_attn_dq_kernel(const PackedArgs a) {
                 if (crow(r, 0) <= row - key0 - 4 * hi)
                     sum = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], c2, -ls)), dp[r], sum);
         });
+        if (TEAMS > 1) {
+            // each team's sum to the other
+            join[team * SETS * (D / 2) * 64] = sum;
+            __syncthreads();
+            sum += join[(1 - team) * SETS * (D / 2) * 64];
+            __syncthreads();
+        }
         dl = both_sum(sum);
         if (steps > 0) fetch(0);
     }
-    if (mine && hi == 0) a.delta[(long)h * T + row] = -dl;
+    if (mine && hi == 0 && team == 0) a.delta[(long)h * T + row] = -dl;
     sweep([&](f32x16_t& s, f32x16_t& dp, int key0, const Lane<D>& at, int sub) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -613,6 +651,15 @@ packed_attn_dq_kernel(const PackedArgs a) {
                                acc[db]);
         }
     });
+    if (TEAMS > 1) {
+        if (team)
+#pragma unroll
+            for (int i = 0; i < D / 2; ++i) join[i * 64] = acc[i / 16][i % 16];
+        __syncthreads();
+        if (team) return;
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i) acc[i / 16][i % 16] += join[i * 64];
+    }
     store_row<D>(acc, seq1 < 0 ? NAN : a.scale, a.dq + ((long)row * Hq + h) * D, hi, nullptr, mine);
 }
 
@@ -621,9 +668,10 @@ packed_attn_dq_kernel(const PackedArgs a) {
 // A workgroup takes KS sets of 32 keys of one kv head (a tile or a half of it);
 // the queries of all the group's heads that see them pass through LDS, QB at a
 // time.  A wave keeps k and v of one set in registers; KS waves share the keys,
-// two such teams the queries, and their sums are joined at the end.
-template <int D, int KS, int QB, int NBUF>
-__global__ void __launch_bounds__(KS * 128, D == 128 ? 2 : 3)
+// TEAMS of them the queries, and their sums are joined at the end.  (TEAMS 4,
+// with half the keys or twice the waves, is for grids that leave CUs idle.)
+template <int D, int KS, int TEAMS, int QB, int NBUF>
+__global__ void __launch_bounds__(KS * TEAMS * 64, D == 128 || KS * TEAMS > 4 ? 2 : 3)
 packed_attn_dkv_kernel(const PackedArgs a) {
     const int T = a.T, Hq = a.Hq, Hk = a.Hk;
     const int4_t* tiles = a.tiles ? (const int4_t*)a.tiles + a.max_tiles : nullptr;
@@ -664,10 +712,10 @@ packed_attn_dkv_kernel(const PackedArgs a) {
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) ak[db] = av[db] = zero16();
 
-    const Mover<D, QB, KS * 128> mq(a.qt), mo(a.ot);
+    const Mover<D, QB, KS * TEAMS * 64> mq(a.qt), mo(a.ot);
     // each wave also moves 64 rows' log-sums or deltas (where there are more
     // waves than parts, two move the same)
-    static_assert(QB % 64 == 0 && KS * 2 % (QB / 32) == 0, "by wave");
+    static_assert(QB % 64 == 0 && KS * TEAMS % (QB / 32) == 0, "by wave");
     const int part = wid % (QB / 32) / 2;
     const bool sums = wid % 2 == 0;
     auto fetch = [&](int h, int r0, int buf) {
@@ -701,8 +749,8 @@ packed_attn_dkv_kernel(const PackedArgs a) {
         const bool more = it + AHEAD < steps;
         if (more) next(buf ? buf - 1 : NBUF - 1);
 #pragma unroll 1
-        for (int sub = 0; sub < QB / 64; ++sub) {
-            const int in = (team * (QB / 64) + sub) * 32;   // first row in the tile
+        for (int sub = 0; sub < QB / 32 / TEAMS; ++sub) {
+            const int in = (team * (QB / 32 / TEAMS) + sub) * 32;   // first row in the tile
             const int first = now + in;
             // queries all before the wave's keys, or past the sequence
             if (first + 31 < wkey || first >= seq1) continue;
@@ -762,31 +810,29 @@ packed_attn_dkv_kernel(const PackedArgs a) {
         else arrived<0>();
         __syncthreads();
     }
-    // the second team's dv to the first, the first team's dk to the second
-    float* join = reinterpret_cast<float*>(lds.x) + wid % KS * 32 * D + lane;
-    auto put = [&](const f32x16_t (&a)[D / 32], float* to) {
+    // the other teams' dv to the first, then their dk to the second
+    auto joined = [&](f32x16_t (&x)[D / 32], int to) {
+        float* join = reinterpret_cast<float*>(lds.x) + wid % KS * 32 * D + lane;
+        static_assert((TEAMS - 1) * KS * 32 * D * 4 <= 2 * NBUF * TILE, "fits the tiles");
+        if (team != to) {
+            join += (team < to ? team : team - 1) * KS * 32 * D;
 #pragma unroll
-        for (int db = 0; db < D / 32; ++db)
+            for (int i = 0; i < D / 2; ++i) join[i * 64] = x[i / 16][i % 16];
+        }
+        __syncthreads();
+        if (team == to)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) to[(db * 16 + r) * 64] = a[db][r];
+            for (int other = 0; other < TEAMS - 1; ++other)
+#pragma unroll
+                for (int i = 0; i < D / 2; ++i)
+                    x[i / 16][i % 16] += join[other * KS * 32 * D + i * 64];
     };
-    auto add = [&](f32x16_t (&a)[D / 32], const float* from) {
-#pragma unroll
-        for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) a[db][r] += from[(db * 16 + r) * 64];
-    };
-    if (team) put(av, join);
-    else put(ak, join + KS * 32 * D);
-    __syncthreads();
     const long to = ((long)key * Hk + hk) * D;
-    if (team) {
-        add(ak, join + KS * 32 * D);
-        store_row<D>(ak, seq1 < 0 ? NAN : a.scale, a.dk + to, hi, nullptr, mine);
-    } else {
-        add(av, join);
-        store_row<D>(av, seq1 < 0 ? NAN : 1.f, a.dv + to, hi, nullptr, mine);
-    }
+    joined(av, 0);
+    if (team == 0) store_row<D>(av, seq1 < 0 ? NAN : 1.f, a.dv + to, hi, nullptr, mine);
+    __syncthreads();
+    joined(ak, 1);
+    if (team == 1) store_row<D>(ak, seq1 < 0 ? NAN : a.scale, a.dk + to, hi, nullptr, mine);
 }
 
 // ---------------------------------------------------------------- launchers
@@ -799,40 +845,55 @@ extern "C" int launch_packed_tiles(const PackedArgs* a, void* stream) {
     return (int)hipGetLastError();
 }
 
+namespace {
+
+template <int D, int TEAMS>
+void fwd(const PackedArgs* a, hipStream_t st) {
+    const dim3 grid((unsigned)a->max_tiles * a->Hq * TEAMS), block(256);
+    if (a->lse)
+        hipLaunchKernelGGL((packed_attn_fwd_kernel<D, TEAMS, true>), grid, block, 0, st, *a);
+    else hipLaunchKernelGGL((packed_attn_fwd_kernel<D, TEAMS, false>), grid, block, 0, st, *a);
+}
+
+template <int D, int TEAMS>
+void dq_(const PackedArgs* a, hipStream_t st) {
+    hipLaunchKernelGGL((packed_attn_dq_kernel<D, TEAMS>),
+                       dim3((unsigned)a->max_tiles * a->Hq * TEAMS), dim3(256), 0, st, *a);
+}
+
+template <int D, int KS, int TEAMS, int QB, int NBUF>
+void dkv(const PackedArgs* a, hipStream_t st) {
+    hipLaunchKernelGGL((packed_attn_dkv_kernel<D, KS, TEAMS, QB, NBUF>),
+                       dim3((unsigned)a->max_tiles * a->Hk * (4 / KS)), dim3(KS * TEAMS * 64), 0,
+                       st, *a);
+}
+
+// Whether workgroups of 128 rows leave CUs idle: then more waves take a tile.
+// (7 sequences of up to 1023 tokens, 8/4 heads of 64, 200 workgroups:
+// FIGURES)
+bool sparse(const PackedArgs* a, int heads) { return a->max_tiles * heads <= 256; }
+
+}  // namespace
+
 extern "C" int launch_packed_attn_fwd(const PackedArgs* a, void* stream) {
-    const dim3 grid((unsigned)a->max_tiles * a->Hq), block(256);
     const hipStream_t st = (hipStream_t)stream;
-    if (a->D == 128) {
-        if (a->lse) hipLaunchKernelGGL((packed_attn_fwd_kernel<128, true>), grid, block, 0, st, *a);
-        else hipLaunchKernelGGL((packed_attn_fwd_kernel<128, false>), grid, block, 0, st, *a);
-    } else {
-        if (a->lse) hipLaunchKernelGGL((packed_attn_fwd_kernel<64, true>), grid, block, 0, st, *a);
-        else hipLaunchKernelGGL((packed_attn_fwd_kernel<64, false>), grid, block, 0, st, *a);
-    }
+    const bool few = sparse(a, a->Hq);
+    if (a->D == 128) few ? fwd<128, 2>(a, st) : fwd<128, 1>(a, st);
+    else few ? fwd<64, 2>(a, st) : fwd<64, 1>(a, st);
     return (int)hipGetLastError();
 }
 
 extern "C" int launch_packed_attn_dq(const PackedArgs* a, void* stream) {
-    const dim3 grid((unsigned)a->max_tiles * a->Hq), block(256);
     const hipStream_t st = (hipStream_t)stream;
-    if (a->D == 128) hipLaunchKernelGGL((packed_attn_dq_kernel<128>), grid, block, 0, st, *a);
-    else hipLaunchKernelGGL((packed_attn_dq_kernel<64>), grid, block, 0, st, *a);
+    const bool few = sparse(a, a->Hq);
+    if (a->D == 128) few ? dq_<128, 2>(a, st) : dq_<128, 1>(a, st);
+    else few ? dq_<64, 2>(a, st) : dq_<64, 1>(a, st);
     return (int)hipGetLastError();
 }
 
-namespace {
-
-template <int D, int KS, int QB, int NBUF>
-void dkv(const PackedArgs* a, hipStream_t st) {
-    hipLaunchKernelGGL((packed_attn_dkv_kernel<D, KS, QB, NBUF>),
-                       dim3((unsigned)a->max_tiles * a->Hk * (4 / KS)), dim3(KS * 128), 0, st,
-                       *a);
-}
-
-}  // namespace
-
 extern "C" int launch_packed_attn_dkv(const PackedArgs* a, void* stream) {
-    if (a->D == 128) dkv<128, 4, 128, 2>(a, (hipStream_t)stream);
-    else dkv<64, 2, 64, 3>(a, (hipStream_t)stream);
+    const hipStream_t st = (hipStream_t)stream;
+    if (a->D == 128) sparse(a, a->Hk) ? dkv<128, 2, 4, 128, 2>(a, st) : dkv<128, 4, 2, 128, 2>(a, st);
+    else sparse(a, 2 * a->Hk) ? dkv<64, 2, 4, 128, 2>(a, st) : dkv<64, 2, 2, 64, 3>(a, st);
     return (int)hipGetLastError();
 }

@@ -166,6 +166,24 @@ def test_attention_gpu(lens, heads, d):
 
 @gpu
 @pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens,heads", [
+    ([257, 3, 640], (32, 8)),      # enough workgroups for one wave set a tile
+    ([257, 3, 640], (64, 64)),     # and for dk, dv
+    ([900, 130, 77], (64, 8)),     # more than run at once: a table of tiles
+    ([9] * 100, (4, 2)),           # more sequences than a wave looks through
+    ([128] * 70, (6, 3)),
+])
+def test_attention_gpu_large_grids(lens, heads, d):
+    q, k, v, dout = _inputs(lens, heads, d, pad=5, device="cuda")
+    starts = _starts(lens)
+    got = _attend(q, k, v, dout, torch.tensor(starts, dtype=torch.int32, device="cuda"))
+    want, tol = attention_oracle(q, k, v, dout, starts, 1.0 / math.sqrt(d))
+    _within(got, want, tol)
+    assert all(not x[starts[-1]:].any() for x in got)
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
 def test_attention_gpu_sharp_scores(d):
     """Scores far apart: the running maximum grows many times, and most
     probabilities underflow."""
