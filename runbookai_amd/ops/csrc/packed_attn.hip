@@ -868,10 +868,18 @@ void dkv(const PackedArgs* a, hipStream_t st) {
                        st, *a);
 }
 
-// Whether workgroups of 128 rows leave CUs idle: then more waves take a tile.
-// (7 sequences of up to 1023 tokens, 8/4 heads of 64, 200 workgroups:
-// FIGURES)
-bool sparse(const PackedArgs* a, int heads) { return a->max_tiles * heads <= 256; }
+// Whether the usual split leaves CUs with a workgroup or two less than fit: then
+// more waves take a tile.  With and without (us; 8/4 heads of 64, 32/8 of 128):
+//   workgroups           forward     dq          dk/dv
+//   88   1024, 8/4       14.5 19.2   17.0 22.1   24.3 32.1
+//   328  3 x 1536, 8/4   26.4 32.5   31.4 37.5   36.8 49.6
+//   448  6 x 1024, 8/4   23.4 27.5   28.3 32.5   41.1 41.8
+//   736  1916, 32/8      33.6 33.4   47.4 43.7
+//   152  2048, 32/8                              147 221
+//   592  8 x 1024, 32/8                          229 151
+bool sparse(const PackedArgs* a, int heads, int fit = 2) {
+    return a->max_tiles * heads <= 256 * fit;
+}
 
 }  // namespace
 
@@ -893,7 +901,8 @@ extern "C" int launch_packed_attn_dq(const PackedArgs* a, void* stream) {
 
 extern "C" int launch_packed_attn_dkv(const PackedArgs* a, void* stream) {
     const hipStream_t st = (hipStream_t)stream;
-    if (a->D == 128) sparse(a, a->Hk) ? dkv<128, 2, 4, 128, 2>(a, st) : dkv<128, 4, 2, 128, 2>(a, st);
+    if (a->D == 128)   // one workgroup a CU
+        sparse(a, a->Hk, 1) ? dkv<128, 2, 4, 128, 2>(a, st) : dkv<128, 4, 2, 128, 2>(a, st);
     else sparse(a, 2 * a->Hk) ? dkv<64, 2, 4, 128, 2>(a, st) : dkv<64, 2, 2, 64, 3>(a, st);
     return (int)hipGetLastError();
 }
