@@ -88,7 +88,8 @@ xent_fwd_kernel(const T* __restrict__ x, long stride, const long* __restrict__ t
     constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1;
     constexpr int U = 4;
     const int tid = threadIdx.x % LANES;
-    const long row = (long)blockIdx.x * ROWS + threadIdx.x / LANES;
+    const long part = (long)blockIdx.y * gridDim.x + blockIdx.x;
+    const long row = part * ROWS + threadIdx.x / LANES;
     const long t = row < N ? targets[row] : ignore;
     double sum = 0.0;   // of a row's first thread
     int labels = 0;
@@ -166,10 +167,10 @@ xent_fwd_kernel(const T* __restrict__ x, long stride, const long* __restrict__ t
         __shared__ int ns[ROWS];
         if (tid == 0) { ss[threadIdx.x / LANES] = sum; ns[threadIdx.x / LANES] = labels; }
         __syncthreads();
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0 && part * ROWS < N) {
             for (int i = 1; i < ROWS; ++i) { sum += ss[i]; labels += ns[i]; }
-            sums[blockIdx.x] = sum;
-            counts[blockIdx.x] = labels;
+            sums[part] = sum;
+            counts[part] = labels;
         }
     }
 }
@@ -225,7 +226,7 @@ xent_bwd_kernel(const T* __restrict__ x, long stride, const long* __restrict__ t
     constexpr int VEC = Elem<T>::VEC, LANES = WAVES * 64;
     constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1;
     constexpr int U = 4;
-    const int row = blockIdx.x * ROWS + (ROWS > 1 ? (int)threadIdx.x / LANES : 0);
+    const long row = ((long)blockIdx.y * gridDim.x + blockIdx.x) * ROWS + threadIdx.x / LANES;
     if (row >= N) return;
     const int tid = threadIdx.x % LANES;
     const long t = targets[row];
@@ -279,11 +280,18 @@ namespace {
 
 template <int WAVES> constexpr int rows_of = WAVES < 4 ? 4 / WAVES : 1;
 
+// A launch's threads along x are counted in 32 bits: more workgroups go along y.
+template <int WAVES>
+dim3 grid_of(int N) {
+    const int blocks = (N - 1) / rows_of<WAVES> + 1, most = 1 << 21;
+    return blocks <= most ? dim3(blocks) : dim3(most, (blocks - 1) / most + 1);
+}
+
 template <typename T, int WAVES>
 void fwd(const void* x, long stride, const void* targets, long ignore, int N, int V,
          void* loss, void* stats, void* sums, void* counts, hipStream_t st) {
     constexpr int ROWS = rows_of<WAVES>;
-    hipLaunchKernelGGL((xent_fwd_kernel<T, WAVES>), dim3((N + ROWS - 1) / ROWS),
+    hipLaunchKernelGGL((xent_fwd_kernel<T, WAVES>), grid_of<WAVES>(N),
                        dim3(ROWS * WAVES * 64), 0, st, (const T*)x, stride,
                        (const long*)targets, ignore, N, V, (float*)loss, (float2_t*)stats,
                        (double*)sums, (int*)counts);
@@ -294,7 +302,7 @@ void bwd(const void* x, long stride, const void* targets, long ignore, int N, in
          const void* stats, const void* gout, long gstride, const void* factor, void* dx,
          long dstride, hipStream_t st) {
     constexpr int ROWS = rows_of<WAVES>;
-    hipLaunchKernelGGL((xent_bwd_kernel<T, WAVES>), dim3((N + ROWS - 1) / ROWS),
+    hipLaunchKernelGGL((xent_bwd_kernel<T, WAVES>), grid_of<WAVES>(N),
                        dim3(ROWS * WAVES * 64), 0, st, (const T*)x, stride,
                        (const long*)targets, ignore, N, V, (const float2_t*)stats,
                        (const float*)gout, gstride, (const float*)factor, (T*)dx, dstride);
@@ -305,7 +313,7 @@ void bwd(const void* x, long stride, const void* targets, long ignore, int N, in
 // How many sums and counts the forward kernel leaves.
 extern "C" int xent_parts(int N, int V) {
     const int rows = V <= XENT_SHORT ? rows_of<1> : rows_of<16>;
-    return (N + rows - 1) / rows;
+    return (N - 1) / rows + 1;
 }
 
 extern "C" int launch_xent_fwd(int kind, const void* x, long stride, const void* targets,

@@ -162,7 +162,7 @@ struct Mover {
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                      :
                      : "s"(to), "v"(at), "s"(from)
-                     : "memory");
+                     : "memory", "m0");
     }
     DEVINL void move(const ushort_t* base, int row0, int last, char* tile) const {
         const char* from = reinterpret_cast<const char*>(base) + row0 * pitch;
@@ -189,7 +189,7 @@ DEVINL void move64(const float* from, int i, const float* to) {
                  : "s"(__builtin_amdgcn_readfirstlane(
                        (unsigned)(unsigned long)(__attribute__((address_space(3))) const float*)to)),
                    "v"(i * 4), "s"(from)
-                 : "memory");
+                 : "memory", "m0");
 }
 
 // All of the wave's own moves but its last N are in LDS (loads end in the order

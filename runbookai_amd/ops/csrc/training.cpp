@@ -55,6 +55,25 @@ std::vector<Tensor> once(std::vector<Tensor> grads, const char* what) {
     return (*error)(std::move(grads));
 }
 
+// Scratch memory of several parts in one allocation: each part's offset, and
+// the size of all.
+struct Parts {
+    size_t size = 0;
+    size_t add(size_t bytes) {
+        const size_t at = size;
+        size += (bytes + 255) / 256 * 256;
+        return at;
+    }
+    Tensor make(const Tensor& like) const {
+        return torch::empty({(long)size}, like.options().dtype(torch::kUInt8));
+    }
+};
+
+template <typename T>
+T* part(const Tensor& t, size_t at) {
+    return reinterpret_cast<T*>(static_cast<char*>(t.data_ptr()) + at);
+}
+
 // ------------------------------------------------------------ packed attention
 
 // What the kernels take: head rows that are dense, at 16-byte boundaries, and
@@ -99,21 +118,31 @@ PackedArgs packed_args(const Tensor& q, const Tensor& k, const Tensor& v, double
     return a;
 }
 
-// Sets where the tiles are: `where` holds a table of tiles or, for few
-// sequences in few tiles, just their starts (a workgroup of 128 rows for each
-// head: up to 512 run at once whatever the head dim).
-void packed_tiles(PackedArgs& a, const Tensor& where, long B) {
+// Where the tiles come from: a table or, for few sequences in few tiles, just
+// the starts (a workgroup of 128 rows for each head: up to 512 run at once
+// whatever the head dim).  -> whether by a table
+bool plan_tiles(PackedArgs& a, long B) {
     const long most = a.T / PACKED_ROWS + B + 2;
-    TORCH_CHECK(2 * most * a.Hq < (1L << 31), "too many sequences");
+    // a launch's threads are counted in 32 bits
+    TORCH_CHECK(most * a.Hq * 512 < (1L << 32), "too many rows and sequences for one call");
     a.B = (int)B;
     a.max_tiles = (int)most;
-    if (B <= PACKED_FEW && most * a.Hq <= 512) a.starts = where.data_ptr<int>();
-    else a.tiles = where.data_ptr();
+    return B > PACKED_FEW || most * a.Hq > 512;
 }
 
-bool by_table(const PackedArgs& a) { return a.tiles != nullptr; }
+// What the forward pass keeps for the backward one, and the table of tiles.
+struct Kept {
+    Parts parts;
+    size_t tiles, rest = 0, lse = 0;
+    Kept(const PackedArgs& a, bool table, bool save)
+        : tiles(parts.add(table ? 32 * (size_t)a.max_tiles : save ? 4 * ((size_t)a.B + 1) : 0)) {
+        if (!save) return;
+        rest = parts.add(2 * (size_t)a.T * a.Hq * a.D);
+        lse = parts.add(4 * (size_t)a.T * a.Hq);
+    }
+};
 
-// -> out and, with `save`, what its rounding left over, lse and where the tiles are
+// -> out and, with `save`, what the backward pass needs
 std::vector<Tensor> packed_attn_fwd(const Tensor& q, const Tensor& k, const Tensor& v,
                                     const Tensor& starts, double scale, bool save) {
     PackedArgs a = packed_args(q, k, v, scale);
@@ -121,40 +150,31 @@ std::vector<Tensor> packed_attn_fwd(const Tensor& q, const Tensor& k, const Tens
                     starts.is_contiguous() && starts.dim() == 1 && starts.numel() >= 1,
                 "seq_starts must be a dense int32 vector on the device of q");
     const c10::cuda::CUDAGuard guard(q.device());
-    const auto opt = q.options();
-    const Tensor out = torch::empty({a.T, a.Hq, a.D}, opt);
-    Tensor rest, lse, where;
-    packed_tiles(a, starts, starts.numel() - 1);
+    const Tensor out = torch::empty({a.T, a.Hq, a.D}, q.options());
+    const bool table = plan_tiles(a, starts.numel() - 1);
+    const Kept at(a, table, save);
+    Tensor kept;
+    if (at.parts.size) kept = at.parts.make(q);
+    a.starts = starts.data_ptr<int>();
     a.out = bf16(out);
-    if (by_table(a)) where = torch::empty({8 * (long)a.max_tiles}, opt.dtype(torch::kInt32));
+    if (table) a.tiles = part<void>(kept, at.tiles);
     if (save) {
-        rest = torch::empty_like(out);
-        lse = torch::empty({a.Hq, a.T}, opt.dtype(torch::kFloat32));
-        a.out_lo = bf16(rest);
-        a.lse = lse.data_ptr<float>();
-        if (!by_table(a)) {
-            where = torch::empty_like(starts);
-            a.kept_starts = where.data_ptr<int>();
-        }
+        a.out_lo = part<unsigned short>(kept, at.rest);
+        a.lse = part<float>(kept, at.lse);
+        if (!table) a.kept_starts = part<int>(kept, at.tiles);
     }
     if (a.T > 0) {
         void* st = stream_of(q);
-        if (by_table(a)) {
-            a.starts = starts.data_ptr<int>();
-            a.tiles = where.data_ptr();
-            launched(launch_packed_tiles(&a, st), "packed_attention");
-        }
+        if (table) launched(launch_packed_tiles(&a, st), "packed_attention");
         launched(launch_packed_attn_fwd(&a, st), "packed_attention");
     }
-    if (!save) return {out};
-    return {out, rest, lse, where};
+    return {out, kept};
 }
 
 // -> dq, dk, dv (the last two undefined without `keys`)
 std::vector<Tensor> packed_attn_bwd(const Tensor& dout, const Tensor& q, const Tensor& k,
-                                    const Tensor& v, const Tensor& out, const Tensor& rest,
-                                    const Tensor& lse, const Tensor& where, long B, double scale,
-                                    bool keys) {
+                                    const Tensor& v, const Tensor& out, const Tensor& kept,
+                                    long B, double scale, bool keys) {
     PackedArgs a = packed_args(q, k, v, scale);
     check_rows(dout, "the gradient", q);
     TORCH_CHECK(dout.sizes() == q.sizes(), "the gradient must have the shape of q");
@@ -164,14 +184,17 @@ std::vector<Tensor> packed_attn_bwd(const Tensor& dout, const Tensor& q, const T
     Tensor dk, dv;
     if (keys) {
         dk = torch::empty({a.T, a.Hk, a.D}, opt);
-        dv = torch::empty_like(dk);
+        dv = torch::empty({a.T, a.Hk, a.D}, opt);
     }
     if (a.T > 0) {
-        const Tensor delta = torch::empty_like(lse);
-        packed_tiles(a, where, B);
+        const Tensor delta = torch::empty({a.Hq, a.T}, opt.dtype(torch::kFloat32));
+        const bool table = plan_tiles(a, B);
+        const Kept at(a, table, true);
+        if (table) a.tiles = part<void>(kept, at.tiles);
+        else a.starts = part<int>(kept, at.tiles);
         a.out = bf16(out);
-        a.out_lo = bf16(rest);
-        a.lse = lse.data_ptr<float>();
+        a.out_lo = part<unsigned short>(kept, at.rest);
+        a.lse = part<float>(kept, at.lse);
         a.dout = bf16(dout); a.ot = dout.stride(0); a.oh = dout.stride(1);
         a.delta = delta.data_ptr<float>();
         a.dq = bf16(dq);
@@ -192,7 +215,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
                           double scale) {
         const Tensor q = rows16(q0), k = rows16(k0), v = rows16(v0);
         const auto got = packed_attn_fwd(q, k, v, starts, scale, true);
-        ctx->save_for_backward({q, k, v, got[0], got[1], got[2], got[3]});
+        ctx->save_for_backward({q, k, v, got[0], got[1]});
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["sequences"] = starts.numel() - 1;
         return got[0];
@@ -200,7 +223,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                    torch::autograd::variable_list g) {
         const auto s = ctx->get_saved_variables();
-        auto d = packed_attn_bwd(rows16(g[0]), s[0], s[1], s[2], s[3], s[4], s[5], s[6],
+        auto d = packed_attn_bwd(rows16(g[0]), s[0], s[1], s[2], s[3], s[4],
                                  ctx->saved_data["sequences"].toInt(),
                                  ctx->saved_data["scale"].toDouble(),
                                  ctx->needs_input_grad(1) || ctx->needs_input_grad(2));
@@ -239,38 +262,50 @@ void check_logits(const Tensor& x, const Tensor& targets) {
                 "targets must be a dense int64 vector with one label a row, beside the logits");
 }
 
-// -> loss of each row, stats and, unless mode is 0, their mean (1) or sum (2) and
-// the factor that this puts before a row's gradient
-std::vector<Tensor> xent_fwd(Tensor x, Tensor targets, int64_t ignore, int64_t mode, bool save) {
+// What the loss leaves: of every row its maximum and 1 / sum, the factor before
+// a row's gradient, and what is needed on the way to a sum of rows.
+struct Losses {
+    Parts parts;
+    size_t stats, factor, rows = 0, sums = 0, counts = 0;
+    Losses(long N, long workgroups, bool mode, bool save)
+        : stats(parts.add(save ? 8 * N : 0)), factor(parts.add(mode ? 4 : 0)) {
+        if (!mode) return;
+        rows = parts.add(4 * N);
+        sums = parts.add(8 * workgroups);
+        counts = parts.add(4 * workgroups);
+    }
+};
+
+// mode 0: the loss of each row, 1: their mean, 2: their sum -> it and what the
+// backward pass needs
+std::vector<Tensor> xent_fwd(const Tensor& x, const Tensor& targets, int64_t ignore,
+                             int64_t mode, bool save) {
     check_logits(x, targets);
     const int kind = kind_of(x, "logits");
     const int N = (int)x.size(0), V = (int)x.size(1);
     const c10::cuda::CUDAGuard guard(x.device());
     const auto opt = x.options().dtype(torch::kFloat32);
-    Tensor loss = torch::empty({N}, opt), stats = torch::empty({save ? N : 0, 2}, opt);
-    Tensor sums;   // of each workgroup of the kernel, and its counts behind them
-    double* at = nullptr;
-    const long parts = N > 0 ? xent_parts(N, V) : 1;
-    if (mode) {
-        sums = N > 0 ? torch::empty({2 * parts}, opt.dtype(torch::kFloat64))
-                     : torch::zeros({2 * parts}, opt.dtype(torch::kFloat64));
-        at = sums.data_ptr<double>();
-    }
+    const Tensor result = mode ? torch::empty({}, opt) : torch::empty({N}, opt);
+    const int parts = N > 0 ? xent_parts(N, V) : 0;
+    const Losses at(N, parts, mode != 0, save);
+    Tensor kept;
+    if (at.parts.size) kept = at.parts.make(x);
+    double* sums = mode ? part<double>(kept, at.sums) : nullptr;
+    int* counts = mode ? part<int>(kept, at.counts) : nullptr;
     void* st = stream_of(x);
     if (N > 0)
         launched(launch_xent_fwd(kind, x.data_ptr(), x.stride(0), targets.data_ptr(), ignore, N,
-                                 V, loss.data_ptr(), save ? stats.data_ptr() : nullptr, at,
-                                 mode ? at + parts : nullptr, st),
+                                 V, mode ? part<void>(kept, at.rows) : result.data_ptr(),
+                                 save ? part<void>(kept, at.stats) : nullptr, sums, counts, st),
                  "cross_entropy");
-    if (!mode) return {loss, stats};
-    Tensor result = torch::empty({}, opt), factor = torch::empty({}, opt);
-    launched(launch_xent_reduce(at, at + parts, (int)parts, mode == 1, result.data_ptr(),
-                                factor.data_ptr(), st), "cross_entropy");
-    return {loss, stats, result, factor};
+    if (mode)
+        launched(launch_xent_reduce(sums, counts, parts, mode == 1, result.data_ptr(),
+                                    part<void>(kept, at.factor), st), "cross_entropy");
+    return {result, kept};
 }
 
-Tensor xent_bwd(Tensor gout, Tensor x, Tensor targets, int64_t ignore, Tensor stats,
-                const Tensor& factor) {
+Tensor xent_bwd(const Tensor& gout, Tensor x, const Tensor& targets, int64_t ignore, int64_t mode,
+                const Tensor& kept) {
     check_logits(x, targets);
     const int kind = kind_of(x, "logits");
     const int N = (int)x.size(0), V = (int)x.size(1);
@@ -286,12 +321,13 @@ Tensor xent_bwd(Tensor gout, Tensor x, Tensor targets, int64_t ignore, Tensor st
     };
     if (!off(x) || (N > 1 && (x.stride(0) - V) * size % 16 != 0))
         x = x.clone(at::MemoryFormat::Contiguous);
+    const Losses at(N, N > 0 ? xent_parts(N, V) : 0, mode != 0, true);
     if (N > 0)
         launched(launch_xent_bwd(kind, x.data_ptr(), x.stride(0), targets.data_ptr(), ignore, N,
-                                 V, stats.data_ptr(), gout.data_ptr(),
+                                 V, part<void>(kept, at.stats), gout.data_ptr(),
                                  gout.dim() ? gout.stride(0) : 0,
-                                 factor.defined() ? factor.data_ptr() : nullptr,
-                                 dx.data_ptr(), V, stream_of(x)),
+                                 mode ? part<void>(kept, at.factor) : nullptr, dx.data_ptr(), V,
+                                 stream_of(x)),
                  "cross_entropy's gradient");
     return dx;
 }
@@ -300,15 +336,16 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x,
                           const Tensor& targets, int64_t ignore, int64_t mode) {
         const auto got = xent_fwd(x, targets, ignore, mode, true);
-        ctx->save_for_backward({x, targets, got[1], mode ? got[3] : Tensor()});
+        ctx->save_for_backward({x, targets, got[1]});
         ctx->saved_data["ignore"] = ignore;
-        return mode ? got[2] : got[0];
+        ctx->saved_data["mode"] = mode;
+        return got[0];
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                    torch::autograd::variable_list g) {
         const auto s = ctx->get_saved_variables();
-        const auto d = once({xent_bwd(g[0], s[0], s[1], ctx->saved_data["ignore"].toInt(), s[2],
-                                      s[3])},
+        const auto d = once({xent_bwd(g[0], s[0], s[1], ctx->saved_data["ignore"].toInt(),
+                                      ctx->saved_data["mode"].toInt(), s[2])},
                             "cross_entropy");
         return {d[0], Tensor(), Tensor(), Tensor()};
     }
@@ -317,7 +354,7 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
 Tensor cross_entropy(const Tensor& x, const Tensor& targets, int64_t ignore, int64_t mode) {
     if (torch::GradMode::is_enabled() && x.requires_grad())
         return CrossEntropy::apply(x, targets, ignore, mode);
-    return xent_fwd(x, targets, ignore, mode, false)[mode ? 2 : 0];
+    return xent_fwd(x, targets, ignore, mode, false)[0];
 }
 
 // --------------------------------------------------------------- gradient norm

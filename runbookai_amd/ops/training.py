@@ -30,7 +30,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     On the GPU: bfloat16, D 64 or 128. q, k and v may be views (slices of a
     fused projection, say): rows at 16-byte boundaries are read in place,
     others are copied first. The starts stay on the device and nothing waits
-    for the host, so forward and backward can be captured into a graph.
+    for the host, so forward and backward can be captured into a graph (by
+    autograd.grad, or while no eager step's graph of the same leaves lives).
     Starts on the host are checked; starts on the device cannot be without
     waiting for them: where they fall or leave [0, T], every output and
     gradient is NaN. A value that is not finite reaches no other sequence.
@@ -63,8 +64,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if q.shape[2] not in (64, 128):
         raise ValueError(f"on the GPU the head dim must be 64 or 128, not {q.shape[2]}")
     starts = seq_starts
-    if starts.dtype != torch.int32 or starts.device != q.device or not starts.is_contiguous():
-        starts = starts.to(device=q.device, dtype=torch.int32).contiguous()
+    if starts.dtype != torch.int32:
+        starts = starts.clamp(-1, 2 ** 31 - 1).to(torch.int32)   # no other value's low bits
+    if starts.device != q.device or not starts.is_contiguous():
+        starts = starts.to(q.device).contiguous()
     return _get_ext().packed_attention(q, k, v, starts, scale)
 
 

@@ -105,6 +105,11 @@ def test_attention_reference(lens, heads):
         torch.testing.assert_close(x, y, rtol=1e-12, atol=1e-12)
 
 
+def test_attention_reference_without_sequences():
+    q, k, v, dout = _inputs([3], (2, 1), 4)
+    assert not any(x.any() for x in _attend(q, k, v, dout, torch.tensor([0])))
+
+
 def test_attention_reference_gradcheck():
     q, k, v, _ = _inputs([4, 3], (2, 1), 4, pad=1, dtype=torch.float64)
     starts = torch.tensor([0, 4, 7])
@@ -255,11 +260,45 @@ def test_attention_gpu_not_finite_elsewhere():
 
 
 @gpu
-@pytest.mark.parametrize("starts", [[0, 300], [0, 120, 60, 200], [-4, 200], [5, 3]])
-def test_attention_gpu_wrong_starts(starts):
-    q, k, v, dout = _inputs([200], (4, 2), 64, device="cuda")
-    got = _attend(q, k, v, dout, torch.tensor(starts, dtype=torch.int32, device="cuda"))
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("heads", [(4, 2), (128, 2)])   # without and with a table of tiles
+@pytest.mark.parametrize("starts", [[0, 300], [0, 120, 60, 200], [-4, 200], [5, 3],
+                                    [0, 2 ** 32 + 200], [0] + [150, 100] * 40])
+def test_attention_gpu_wrong_starts(starts, heads, dtype):
+    if dtype == torch.int32 and max(starts) > 2 ** 31:
+        pytest.skip("no 32-bit value")
+    q, k, v, dout = _inputs([200], heads, 64, device="cuda")
+    got = _attend(q, k, v, dout, torch.tensor(starts, dtype=dtype, device="cuda"))
     assert all(torch.isnan(x).all() for x in got)
+
+
+@gpu
+@pytest.mark.parametrize("heads", [(4, 2), (128, 2)])
+def test_attention_gpu_starts_may_change_before_the_backward_pass(heads):
+    """A buffer of starts that the next batch is written to."""
+    q, k, v, dout = _inputs([100, 60], heads, 64, device="cuda")
+    starts = torch.tensor([0, 100, 160], dtype=torch.int32, device="cuda")
+    want = _attend(q, k, v, dout, starts.clone())
+    parts = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = ops.packed_attention(*parts, starts)
+    starts.copy_(torch.tensor([0, 7, 8], dtype=torch.int32))
+    got = torch.autograd.grad(out, parts, dout)
+    assert all(torch.equal(x, y) for x, y in zip(got, want[1:]))
+
+
+@gpu
+def test_attention_gpu_two_passes_over_one_graph():
+    q, k, v, dout = _inputs([100, 60], (4, 2), 64, device="cuda")
+    starts = torch.tensor([0, 100, 160], device="cuda")
+    parts = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = ops.packed_attention(*parts, starts)
+    other = torch.randn_like(dout)
+    a = torch.autograd.grad(out, parts, dout, retain_graph=True)
+    b = torch.autograd.grad(out, parts, other, retain_graph=True)
+    c = torch.autograd.grad(out, parts, dout)
+    assert all(torch.equal(x, y) for x, y in zip(a, c))
+    want = _attend(q, k, v, other, starts)[1:]
+    assert all(torch.equal(x, y) for x, y in zip(b, want))
 
 
 @gpu
@@ -490,6 +529,49 @@ def test_loss_views(dtype, device):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@gpu
+def test_loss_gpu_more_rows_than_one_grid_counts():
+    n = (1 << 26) + 37
+    x = torch.zeros(n, 2, dtype=torch.float16, device="cuda")
+    t = torch.ones(n, dtype=torch.int64, device="cuda")
+    x[-1, 0] = 1.0
+    loss, grad = _loss_and_grad(x, t, "sum")
+    want = (n - 1) * math.log(2) + math.log(1 + math.e)
+    assert abs(float(loss) / want - 1) <= 2.0 ** -22
+    assert (grad[:-1, 0] == 0.5).all() and (grad[:-1, 1] == -0.5).all()
+    p = 1 / (1 + math.exp(-1))
+    assert abs(float(grad[-1, 0]) - p) <= 2.0 ** -11 and abs(float(grad[-1, 1]) + p) <= 2.0 ** -11
+
+
+@gpu
+def test_loss_gpu_captured():
+    x, t = _loss_inputs(50, 4099, torch.bfloat16, "cuda")
+    x.requires_grad_()
+
+    def step():
+        loss = ops.cross_entropy(x, t)
+        return loss, torch.autograd.grad(loss, x)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = step()
+    for seed in range(1, 4):
+        y, u = _loss_inputs(50, 4099, torch.bfloat16, "cuda", seed=seed)
+        with torch.no_grad():
+            x.copy_(y)
+            t.copy_(u)
+        graph.replay()
+        got = [z.detach().clone() for z in static]
+        want = _loss_and_grad(y, u, "mean")
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        torch.cuda.synchronize()
+
+
 def test_loss_agrees_with_torch():
     x, t = _loss_inputs(20, 33, torch.float32, "cpu")
     torch.testing.assert_close(ops.cross_entropy(x, t), torch.nn.functional.cross_entropy(x, t))
@@ -645,6 +727,27 @@ def test_clip_forms(device):
     none = torch.nn.Parameter(torch.zeros(0, device=device))
     none.grad = torch.zeros(0, device=device)
     assert float(ops.clip_grad_norm_(none, 1.0)) == 0.0
+
+
+@gpu
+def test_clip_gpu_captured():
+    """The norm and whether it clips are of each replay's own gradients."""
+    params = _params([(300, 7), (9001,)], MIXED, "cuda")
+    twins = _params([(300, 7), (9001,)], MIXED, "cuda")
+    ops.clip_grad_norm_(params, 1.0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = ops.clip_grad_norm_(params, 1.0)
+    for std in (0.1, 1e-4, 3.0):
+        new = _params([(300, 7), (9001,)], MIXED, "cuda", std=std)
+        for p, q, n in zip(params, twins, new):
+            p.grad.copy_(n.grad)
+            q.grad.copy_(n.grad)
+        graph.replay()
+        want = ops.clip_grad_norm_(twins, 1.0)
+        assert torch.equal(norm, want)
+        assert all(torch.equal(p.grad, q.grad) for p, q in zip(params, twins))
+        torch.cuda.synchronize()
 
 
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
