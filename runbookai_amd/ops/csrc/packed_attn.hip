@@ -389,6 +389,22 @@ DEVINL int4_t find_tile(const int* __restrict__ starts, int B, int T, int p) {
     return int4_t{r0, min(r0 + ROWS, e), real ? s : r0, real ? e : wrong ? -1 : r0};
 }
 
+// Which tile (or half tile) and head workgroup i of the forward and dq kernels
+// takes.  Workgroups go round the 8 XCDs in turn, and each XCD has an L2 of its
+// own, so all heads of a group take a tile one after the other on one XCD: its
+// keys come there once.  With 8n kv heads an XCD has kv heads of its own; with
+// 1, 2 or 4, 8/Hk XCDs share one and take every 8/Hk-th tile of it.
+struct Place { int tile, hk, h; };
+DEVINL Place place_of(int i, int Hq, int Hk) {
+    const int group = Hq / Hk;
+    if (8 % Hk == 0) {
+        const int share = 8 / Hk, lane = i % 8, turn = i / 8, hk = lane % Hk;
+        return {turn / group * share + lane / Hk, hk, hk * group + turn % group};
+    }
+    const int hk = i % Hk;
+    return {i / Hq, hk, hk * group + i % Hq / Hk};
+}
+
 // ------------------------------------------------------------------ forward
 //
 // A workgroup takes a tile of 128 rows of one head, a wave 32 of the rows.  64
@@ -401,17 +417,15 @@ __global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
 packed_attn_fwd_kernel(const PackedArgs a) {
     const int T = a.T, Hq = a.Hq, Hk = a.Hk;
     const int4_t* tiles = (const int4_t*)a.tiles;
-    const int at_tile = blockIdx.x / (Hq * TEAMS);
+    const Place place = place_of(blockIdx.x, Hq, Hk);
+    const int hk = place.hk, h = place.h, at_tile = place.tile / TEAMS;
+    if (at_tile >= a.max_tiles) return;
     const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile);
-    const int row0 = tile[0] + blockIdx.x / Hq % TEAMS * (ROWS / TEAMS);
+    const int row0 = tile[0] + place.tile % TEAMS * (ROWS / TEAMS);
     const int row1 = min(tile[1], row0 + ROWS / TEAMS), seq0 = tile[2], seq1 = tile[3];
     if (SAVE && !tiles && blockIdx.x == 0)   // for the backward pass, which runs later
         for (int i = threadIdx.x; i <= a.B; i += 256) a.kept_starts[i] = a.starts[i];
     if (row0 >= row1) return;
-    // the kv head runs fastest: workgroups go round the 8 XCDs in turn, so with
-    // 1, 2, 4 or 8n of them an XCD's L2 sees the same heads' keys every time
-    const int hk = blockIdx.x % Hk;
-    const int h = hk * (Hq / Hk) + blockIdx.x % Hq / Hk;
     const bool real = seq1 > seq0;
     const int kv0 = seq0, kv1 = real ? row1 : seq0;
     const int lane = threadIdx.x & (WAVE - 1);
@@ -535,13 +549,13 @@ __global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
 packed_attn_dq_kernel(const PackedArgs a) {
     const int T = a.T, Hq = a.Hq, Hk = a.Hk;
     const int4_t* tiles = (const int4_t*)a.tiles;
-    const int at_tile = blockIdx.x / (Hq * TEAMS);
+    const Place place = place_of(blockIdx.x, Hq, Hk);
+    const int hk = place.hk, h = place.h, at_tile = place.tile / TEAMS;
+    if (at_tile >= a.max_tiles) return;
     const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile);
-    const int row0 = tile[0] + blockIdx.x / Hq % TEAMS * (ROWS / TEAMS);
+    const int row0 = tile[0] + place.tile % TEAMS * (ROWS / TEAMS);
     const int row1 = min(tile[1], row0 + ROWS / TEAMS), seq0 = tile[2], seq1 = tile[3];
     if (row0 >= row1) return;
-    const int hk = blockIdx.x % Hk;
-    const int h = hk * (Hq / Hk) + blockIdx.x % Hq / Hk;
     const bool real = seq1 > seq0;
     const int kv0 = seq0, kv1 = real ? row1 : seq0;
     const int lane = threadIdx.x & (WAVE - 1);
@@ -847,9 +861,15 @@ extern "C" int launch_packed_tiles(const PackedArgs* a, void* stream) {
 
 namespace {
 
+// Workgroups that place_of() gives each of `tiles` tiles and every head
+dim3 grid_of(const PackedArgs* a, int tiles) {
+    const int share = 8 % a->Hk ? 1 : 8 / a->Hk;
+    return dim3((unsigned)((tiles + share - 1) / share * share) * a->Hq);
+}
+
 template <int D, int TEAMS>
 void fwd(const PackedArgs* a, hipStream_t st) {
-    const dim3 grid((unsigned)a->max_tiles * a->Hq * TEAMS), block(256);
+    const dim3 grid = grid_of(a, a->max_tiles * TEAMS), block(256);
     if (a->lse)
         hipLaunchKernelGGL((packed_attn_fwd_kernel<D, TEAMS, true>), grid, block, 0, st, *a);
     else hipLaunchKernelGGL((packed_attn_fwd_kernel<D, TEAMS, false>), grid, block, 0, st, *a);
@@ -858,7 +878,7 @@ void fwd(const PackedArgs* a, hipStream_t st) {
 template <int D, int TEAMS>
 void dq_(const PackedArgs* a, hipStream_t st) {
     hipLaunchKernelGGL((packed_attn_dq_kernel<D, TEAMS>),
-                       dim3((unsigned)a->max_tiles * a->Hq * TEAMS), dim3(256), 0, st, *a);
+                       grid_of(a, a->max_tiles * TEAMS), dim3(256), 0, st, *a);
 }
 
 template <int D, int KS, int TEAMS, int QB, int NBUF>
