@@ -70,7 +70,7 @@ DEVINL double chunk_sum(const void* p, long n, long at) {
 }
 
 template <typename T>
-DEVINL void chunk_scale(void* p, long n, long at, float f) {
+DEVINL void chunk_scale(void* p, long n, long at, double f) {
     constexpr int VEC = 16 / sizeof(T), PER = GRAD_CHUNK / VEC / 256;
     const unsigned long a = reinterpret_cast<unsigned long>(p);
     const long skip = (long)(a & 15) / (long)sizeof(T);
@@ -87,12 +87,12 @@ DEVINL void chunk_scale(void* p, long n, long at, float f) {
         const long e = at + (long)(threadIdx.x + i * 256) * VEC;
         if (e >= skip && e + VEC <= end) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[i][j] = (T)((float)v[i][j] * f);
+            for (int j = 0; j < VEC; ++j) v[i][j] = (T)(float)((double)(float)v[i][j] * f);
             *reinterpret_cast<Vec16<T>*>(base + e) = v[i];
         } else {
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
-                if (e + j >= skip && e + j < end) base[e + j] = (T)((float)base[e + j] * f);
+                if (e + j >= skip && e + j < end) base[e + j] = (T)(float)((double)(float)base[e + j] * f);
         }
     }
 }
@@ -139,11 +139,10 @@ grad_clip_kernel(GradTable t, const double* __restrict__ sums, int n, double lim
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)x;
     const double f = limit / (x + eps);
     if (f >= 1.0) return;   // not for a NaN, which goes into every gradient
-    const float by = (float)f;
     each_chunk(t, [&](int i, long at) {
-        if (t.kind[i] == 0) chunk_scale<float>(t.ptr[i], t.size[i], at, by);
-        else if (t.kind[i] == 1) chunk_scale<__bf16>(t.ptr[i], t.size[i], at, by);
-        else chunk_scale<_Float16>(t.ptr[i], t.size[i], at, by);
+        if (t.kind[i] == 0) chunk_scale<float>(t.ptr[i], t.size[i], at, f);
+        else if (t.kind[i] == 1) chunk_scale<__bf16>(t.ptr[i], t.size[i], at, f);
+        else chunk_scale<_Float16>(t.ptr[i], t.size[i], at, f);
     });
 }
 

@@ -410,7 +410,7 @@ Grads collect(const std::vector<Tensor>& grads, bool write) {
     std::sort(spans.begin(), spans.end());
     for (size_t i = 1; i < spans.size(); ++i)
         TORCH_CHECK_VALUE(spans[i].first >= spans[i - 1].second,
-                          "two of the gradients share memory");
+                          "two of the gradients share or interleave their memory");
     for (const Tensor& d : g.at) {
         const long size = d.element_size();
         const auto p = reinterpret_cast<uintptr_t>(d.data_ptr());

@@ -255,15 +255,19 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int
     return each.sum() / real.sum() if reduction == "mean" else each.sum()
 
 
+def _norm64(grads: list[torch.Tensor]) -> torch.Tensor:
+    return torch.stack([g.double().square().sum() for g in grads]).sum().sqrt()
+
+
 def grad_norm(grads: list[torch.Tensor]) -> torch.Tensor:
     """2-norm of all tensors together, summed in fp64."""
-    return torch.stack([g.double().square().sum() for g in grads]).sum().sqrt().float()
+    return _norm64(grads).float()
 
 
 def grad_clip(grads: list[torch.Tensor], max_norm: float, eps: float) -> torch.Tensor:
     """Scales the tensors in place so that their norm is at most max_norm."""
-    norm = grad_norm(grads)
-    factor = (max_norm / (norm.double() + eps)).clamp(max=1.0).float()
+    norm = _norm64(grads)
+    factor = (max_norm / (norm + eps)).clamp(max=1.0)
     for g in grads:
-        g.copy_(g.float() * factor)
-    return norm
+        g.copy_(g.double() * factor)
+    return norm.float()

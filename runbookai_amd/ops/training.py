@@ -34,7 +34,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     autograd.grad, or while no eager step's graph of the same leaves lives).
     Starts on the host are checked; starts on the device cannot be without
     waiting for them: where they fall or leave [0, T], every output and
-    gradient is NaN. A value that is not finite reaches no other sequence.
+    gradient is NaN. A value that is not finite may reach any row of its own
+    sequence (a shut place's product is 0 times the value), but no other's.
 
     The training counterpart of prefill_attention, which has no gradients."""
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
@@ -42,6 +43,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError(f"shapes do not fit: q {tuple(q.shape)}, k {tuple(k.shape)}, "
                          f"v {tuple(v.shape)}")
+    if q.shape[2] == 0:
+        raise ValueError("the head dim must not be 0")
     if k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
         raise ValueError(f"{q.shape[1]} query heads are no multiple of "
                          f"{k.shape[1]} key/value heads")
@@ -51,8 +54,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             or seq_starts.dtype not in (torch.int32, torch.int64)):
         raise ValueError("seq_starts must be a vector of whole numbers, one more than sequences")
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"scale must be positive and finite, not {scale}")
+    if not 0.0 < scale < 2.0 ** 127:   # times log2(e) it is still an fp32 number
+        raise ValueError(f"scale must be positive and an fp32 number, not {scale}")
     if not seq_starts.is_cuda:
         starts = seq_starts.tolist()
         if starts[0] < 0 or starts[-1] > q.shape[0] or starts != sorted(starts):
@@ -121,8 +124,9 @@ def _grads(parameters) -> list[torch.Tensor]:
     return [g for g in [p.grad for p in parameters] if g is not None]
 
 
-def _check_host(grads: list[torch.Tensor]) -> None:
+def _check_host(grads: list[torch.Tensor], write: bool = False) -> None:
     """What the kernels' bindings check of gradients on the GPU."""
+    spans = []
     for g in grads:
         if g.layout != torch.strided or g.dtype not in (torch.float32, torch.bfloat16,
                                                         torch.float16):
@@ -130,6 +134,12 @@ def _check_host(grads: list[torch.Tensor]) -> None:
                              f"not {g.layout} {g.dtype}")
         if g.device != grads[0].device:
             raise ValueError("gradients must be on one device")
+        if g.numel():
+            last = sum((n - 1) * step for n, step in zip(g.shape, g.stride()))
+            spans.append((g.data_ptr(), g.data_ptr() + (last + 1) * g.element_size()))
+    spans.sort()
+    if write and any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+        raise ValueError("two of the gradients share or interleave their memory")
 
 
 def grad_norm(parameters) -> torch.Tensor:
@@ -149,13 +159,14 @@ def clip_grad_norm_(parameters, max_norm: float,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scales all parameters' gradients in place by
     min(1, max_norm / (norm + 1e-6)) and returns their norm before that (fp32
-    scalar on their device).
+    scalar on their device). Two gradients whose memory overlaps or interleaves
+    (the same one twice, columns of one buffer) are refused.
 
     On the GPU: any mix of float32, bfloat16 and float16 gradients of any
-    sizes, strides and alignment on one device; two that share memory are
-    refused. The norm is summed in fp64. The host waits for nothing (so it can
-    be captured into a graph) unless error_if_nonfinite is set, which raises
-    for a norm that is not finite and leaves the gradients as they were."""
+    sizes, strides and alignment on one device. The norm is summed in fp64 and
+    the factor applied in fp64. The host waits for nothing (so it can be
+    captured into a graph) unless error_if_nonfinite is set, which raises for a
+    norm that is not finite and leaves the gradients as they were."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative: {max_norm}")
@@ -171,6 +182,6 @@ def clip_grad_norm_(parameters, max_norm: float,
         return torch.zeros(())
     if grads[0].is_cuda:
         return _get_ext().grad_clip(grads, max_norm, _EPS)
-    _check_host(grads)
+    _check_host(grads, write=True)
     with torch.no_grad():
         return reference.grad_clip(grads, max_norm, _EPS)

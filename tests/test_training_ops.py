@@ -7,6 +7,7 @@ all fp32 arithmetic on the way to a sum (a score is a sum of at most 128
 products: 128 * 2^-24 = 2^-17 of sum |q||k| scale, which is below 20 at these
 inputs, so a probability is off by less than 2^-12 of itself, twice)."""
 import math
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -140,9 +141,11 @@ def test_attention_refuses(device):
     for args in bad:
         with pytest.raises(ValueError):
             call(*args)
-    for scale in (0.0, -1.0, math.inf, math.nan):
+    for scale in (0.0, -1.0, math.inf, math.nan, 1e39):
         with pytest.raises(ValueError):
             call(q, k, v, starts, scale=scale)
+    with pytest.raises(ValueError):
+        call(q[..., :0], k[..., :0], v[..., :0], starts)
     if device == "cuda":
         with pytest.raises(ValueError):
             call(q.float(), k.float(), v.float(), starts)
@@ -529,6 +532,49 @@ def test_loss_views(dtype, device):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_loss_of_no_rows_and_of_one_row_repeated(reduction, device):
+    none = torch.zeros(0, 9, device=device, requires_grad=True)
+    loss = ops.cross_entropy(none, torch.zeros(0, dtype=torch.int64, device=device),
+                             reduction=reduction)
+    loss.backward(torch.ones_like(loss))
+    assert none.grad.shape == (0, 9) and loss.numel() == (reduction != "none")
+    row = torch.randn(1, 901).to(device).requires_grad_()
+    t = torch.tensor([3, 900, -100, 0, 3], device=device)
+    loss = ops.cross_entropy(row.expand(5, 901), t, reduction=reduction)
+    loss.backward(torch.ones_like(loss))
+    want, grad = loss_oracle(row.expand(5, 901), t, reduction, torch.ones_like(loss))
+    # five rows' gradients, and their sum, each within a few steps of values below 1
+    assert ((row.grad.double().cpu()[0] - grad.sum(0)).abs() <= 5 * 2.0 ** -18).all()
+    assert ((loss.double().cpu() - want).abs() <= 2.0 ** -18 * (1 + want.abs())).all()
+
+
+@gpu
+def test_ops_gpu_from_two_threads():
+    """Each on a stream of its own, forward and backward."""
+    lens, steps = [300, 40], 20
+    starts = torch.tensor(_starts(lens), dtype=torch.int32, device="cuda")
+    data = [_inputs(lens, (4, 2), 64, seed=i, device="cuda") for i in range(2)]
+    logits = [_loss_inputs(50, 9001, torch.bfloat16, "cuda", seed=i) for i in range(2)]
+    want = [(_attend(*d, starts), _loss_and_grad(*x, "mean")) for d, x in zip(data, logits)]
+    torch.cuda.synchronize()
+
+    def work(i):
+        out = []
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(steps):
+                out.append((_attend(*data[i], starts), _loss_and_grad(*logits[i], "mean")))
+            torch.cuda.current_stream().synchronize()
+        return out
+
+    with ThreadPoolExecutor(2) as pool:
+        for i, got in enumerate(pool.map(work, range(2))):
+            for attended, loss in got:
+                assert all(torch.equal(x, y) for x, y in zip(attended, want[i][0]))
+                assert all(torch.equal(x, y) for x, y in zip(loss, want[i][1]))
+
+
 @gpu
 def test_loss_gpu_more_rows_than_one_grid_counts():
     n = (1 << 26) + 37
@@ -690,6 +736,32 @@ def test_clip_range(device):
     before = params[0].grad.clone()
     ops.clip_grad_norm_(params, 1.0)
     assert torch.equal(params[0].grad, before)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_clip_factor_below_the_smallest_normal_number(device):
+    """1e-3 / 1e38 has few bits in fp32; the results, near 1e-4, have all."""
+    params = _params([(500,), (8, 9)], MIXED[:2], device, std=3e36)
+    _check_clip(params, 1e-3)
+    assert 1e-6 < float(params[0].grad.abs().max()) < 1e-3
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_clip_refuses_shared_memory(device):
+    one, two = _params([(4, 6), (4, 6)], MIXED[:1], device)
+    both = torch.randn(4, 12, device=device)
+    keep = both.clone()
+    one.grad, two.grad = both[:, :6], both[:, 6:]
+    for params in ([one, one], [one, two]):
+        with pytest.raises(ValueError, match="share or interleave"):
+            ops.clip_grad_norm_(params, 0.1)
+    assert torch.equal(both, keep)
+    norm = float(keep.double().square().sum().sqrt())
+    assert abs(float(ops.grad_norm([one, two])) / norm - 1) < 1e-6
+    one, two = _params([(2, 6), (2, 6)], MIXED[:1], device)
+    one.grad, two.grad = both[:2, :6], both[2:, :6]     # one after the other is fine
+    _check_clip([one, two], 0.1)
+    assert torch.equal(both[:, 6:], keep[:, 6:])
 
 
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
