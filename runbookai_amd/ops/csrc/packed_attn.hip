@@ -36,7 +36,7 @@
 // keeps what o's rounding left over (out_lo, as bf16), which takes the rounding
 // out of delta; and the first tile of each sequence, whose rows have few places
 // to attend to, takes delta_i = sum_j P_ij dP_ij in fp32, by a sweep of its own
-// over its (at most 128) keys.  Of the policy's batch, dq is then 1.45 times as
+// over its (at most 128) keys.  Of the policy's batch, dq is then 1.46 times as
 // far from exact as its own rounding alone; from the rounded o it was 1.50.
 #include "common.h"
 
@@ -188,7 +188,7 @@ DEVINL void move64(const float* from, int i, const float* to) {
                  :
                  : "s"(__builtin_amdgcn_readfirstlane(
                        (unsigned)(unsigned long)(__attribute__((address_space(3))) const float*)to)),
-                   "v"(i * 4), "s"(from)
+                   "v"((unsigned)i * 4u), "s"(from)
                  : "memory", "m0");
 }
 
@@ -412,6 +412,16 @@ DEVINL Place place_of(int i, int Hq, int Hk) {
 // With two TEAMS it takes half a tile, and each team half of the keys, whose
 // sums are joined at the end: for grids that leave CUs idle, where a wave's own
 // chain of steps is what takes the time.
+//
+// Bound by the SIMDs: a wave's MFMA (16 a block of 32 keys at D 128, 15 ns each)
+// and the softmax's VALU work (3.4 ns an exp2, 1 ns an add) add up where other
+// waves' do not hide beneath them.  A wave keeps 32 rows because each fragment
+// of K and V from LDS then serves a product of 32 columns, and 128 registers of
+// accumulators and queries still leave two workgroups a CU.  Two of them overlap
+// each other's softmax and products better than one with longer tiles (two
+// blocks at a time in one wave: 631 against 590 us).  8192 rows, 32/8 heads of
+// 128: 0.53 ms, 1.03 PFLOP/s; 32768 rows in sequences of 64 to 1536, 8/4 heads
+// of 64: 58 us, 0.62 PFLOP/s (46 with all inputs in L2).
 template <int D, int TEAMS, bool SAVE>
 __global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
 packed_attn_fwd_kernel(const PackedArgs a) {
@@ -543,7 +553,10 @@ packed_attn_fwd_kernel(const PackedArgs a) {
 
 // ----------------------------------------------------------------------- dq
 //
-// The forward kernel's split.  Also writes -delta for the kernel below.
+// The forward kernel's split.  Also writes -delta for the kernel below.  24 MFMA
+// a block of 32 keys at D 128 and less VALU work than forward (no maximum), so
+// the matrix cores bound it first.  4096 + 2500 + 1000 + 596 rows, 32/8 heads of
+// 128: 0.32 ms, 0.95 PFLOP/s; 32768 rows of the policy: 80 us, 0.68 PFLOP/s.
 template <int D, int TEAMS>
 __global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
 packed_attn_dq_kernel(const PackedArgs a) {
@@ -684,6 +697,15 @@ packed_attn_dq_kernel(const PackedArgs a) {
 // time.  A wave keeps k and v of one set in registers; KS waves share the keys,
 // TEAMS of them the queries, and their sums are joined at the end.  (TEAMS 4,
 // with half the keys or twice the waves, is for grids that leave CUs idle.)
+//
+// 32 MFMA a block of 32 x 32 at D 128, and as many 1 KB fragments from LDS, 8
+// cycles of its 128 bytes a cycle each: with four SIMDs LDS has to be read as
+// long as the matrix cores run, and both bound it.  64 keys a wave would halve
+// the reads, but its 4 x 64 x D sums and operands do not fit 512 registers (761
+// against 510 us).  At D 128 one workgroup of 8 waves has all of LDS, so that a
+// tile of 128 queries serves 128 keys; at D 64 three buffers of 64 queries keep
+// two tiles on their way.  4096 + 2500 + 1000 + 596 rows, 32/8 heads of 128:
+// 0.50 ms, 0.80 PFLOP/s; 32768 rows of the policy: 102 us, 0.71 PFLOP/s.
 template <int D, int KS, int TEAMS, int QB, int NBUF>
 __global__ void __launch_bounds__(KS * TEAMS * 64, D == 128 || KS * TEAMS > 4 ? 2 : 3)
 packed_attn_dkv_kernel(const PackedArgs a) {
