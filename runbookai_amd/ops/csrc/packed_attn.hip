@@ -42,6 +42,8 @@
 
 #include "packed_attn.h"
 
+#include <type_traits>
+
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
@@ -136,6 +138,18 @@ DEVINL bf16x8_t cols_frag(char* tile, const Lane<D>& l, int db) {
         (lds_short4_t*)(tile + (l.cols ^ (db << 6) ^ 32) + 16 * D));
     return u.v;
 }
+
+// Keeps what is written before it before what is written behind it.  With D 128
+// the kernels read some fragments ahead of the products that take them, and put
+// the softmax between products; the compiler alone reads each pair of fragments
+// right before its products (dq 322 against 311 us).  With D 64 four waves a SIMD
+// cover for each other, and there are no registers to read ahead.
+template <int D>
+DEVINL void in_order() { if (D == 128) __builtin_amdgcn_sched_barrier(0); }
+
+// The first of a fragment's 16 elements whose exp goes beneath product i of n:
+// none beneath the first, while the product that makes them ends.
+DEVINL constexpr int beneath(int i, int n) { return i ? (i - 1) * 16 / (n - 1) : 0; }
 
 // Moves N rows from global memory straight into an LDS tile, 16 bytes a lane,
 // by a workgroup of THREADS.  A wave's lanes fill consecutive chunks, so the
@@ -419,9 +433,10 @@ DEVINL Place place_of(int i, int Hq, int Hk) {
 // of K and V from LDS then serves a product of 32 columns, and 128 registers of
 // accumulators and queries still leave two workgroups a CU.  Two of them overlap
 // each other's softmax and products better than one with longer tiles (two
-// blocks at a time in one wave: 631 against 590 us).  8192 rows, 32/8 heads of
-// 128: 0.53 ms, 1.03 PFLOP/s; 32768 rows in sequences of 64 to 1536, 8/4 heads
-// of 64: 58 us, 0.62 PFLOP/s (46 with all inputs in L2).
+// blocks at a time in one wave: 631 against 590 us).  Without loads and barriers
+// 8192 rows still took 477 us of 558; the rest is these.  8192 rows, 32/8 heads of
+// 128: 0.53 ms, 1.04 PFLOP/s; 32768 rows in sequences of 64 to 1536, 8/4 heads
+// of 64: 57 us, 0.63 PFLOP/s.
 template <int D, int TEAMS, bool SAVE>
 __global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
 packed_attn_fwd_kernel(const PackedArgs a) {
@@ -446,8 +461,10 @@ packed_attn_fwd_kernel(const PackedArgs a) {
     const int wrow = row0 + wid % SETS * 32;
     const int row = wrow + (lane & 31);
     const bool mine = row < row1;
-    const float c2 = a.scale * LOG2E;
+    const float c2 = __uint_as_float(__builtin_amdgcn_readfirstlane(
+        __float_as_uint(a.scale * LOG2E)));
 
+    constexpr int N = D / 16, AHEAD = 4;   // products of a kind, fragments read ahead
     // two tiles of keys, two of values
     constexpr int TILE = 64 * D * 2;
     __shared__ __attribute__((aligned(256))) char lds[4 * TILE];
@@ -474,52 +491,72 @@ packed_attn_fwd_kernel(const PackedArgs a) {
     for (int it = 0; it < steps; ++it) {
         // into the tiles that were last read before the barrier of the step before
         if (it + 1 < steps) fetch(it + 1);
-        const Lane<D> at = lanes.fresh((it & 1) * TILE);
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) {
             const int key0 = kv0 + it * 64 + sub * 32;
             if (key0 >= wave_end || (TEAMS > 1 && sub != team)) continue;
+            // a product each: N fragments of K, then N of V^T
+            const Lane<D> at = lanes.fresh((it & 1) * TILE + sub * (TILE / 2));
+            auto fragment = [&](int i) {
+                return i < N ? rows_frag<D>(lds, at, i)
+                             : cols_frag<D>(lds + 2 * TILE + (i - N) / (D / 32) * (TILE / 4), at,
+                                            (i - N) % (D / 32));
+            };
+            bf16x8_t f[AHEAD];
+            auto next = [&](int i) {
+                if (i + AHEAD < 2 * N) f[i % AHEAD] = fragment(i + AHEAD);
+                in_order<D>();
+            };
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) f[i] = fragment(i);
+            in_order<D>();
             f32x16_t s = zero16();
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d)
-                s = mfma(rows_frag<D>(lds + sub * (TILE / 2), at, d), qf[d], s);
+            for (int i = 0; i < N; ++i) {
+                s = mfma(f[i % AHEAD], qf[i], s);
+                next(i);
+            }
             if (key0 + 31 > wrow) {   // not every key open to every row
                 const int open = seldom(row - key0 - 4 * hi);
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (crow(r, 0) > open) s[r] = -INFINITY;
             }
-            float top = s[0];
+            f32x16_t p;
+            float sum;
+            auto weigh = [&](float base) {
+                sum = 0.f;
 #pragma unroll
-            for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-            top = both_max(top) * c2;
-            // the sums follow the maximum only when a row's has grown by over
-            // 2^8: until then P stays below 2^8, which costs no bits
-            if (!__all(top <= m + 8.f)) {
-                const float to = fmaxf(m, top);
-                const float f = to == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to);
+                for (int r = 0; r < 16; ++r) {
+                    p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -base));
+                    sum += p[r];
+                }
+            };
+            weigh(m);
+            // P is taken by the maximum so far: as long as no half row sums to more
+            // than 2^13 that costs no bits, and the block's own maximum is not
+            // needed.  (At first m is -inf, and the sum infinite or NaN.)
+            if (!__all(sum <= 8192.f)) {
+                float top = s[0];
+#pragma unroll
+                for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+                const float to = fmaxf(m, both_max(top) * c2);
+                const float base = to == -INFINITY ? 0.f : to;
+                const float f = __builtin_amdgcn_exp2f(m - base);
                 m = to;
                 l *= f;
 #pragma unroll
                 for (int db = 0; db < D / 32; ++db)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) acc[db][r] *= f;
-            }
-            const float base = m == -INFINITY ? 0.f : m;
-            float sum = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -base));
-                sum += s[r];
+                weigh(base);
             }
             l += sum;
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                const bf16x8_t pf = pack8(s, ks);
-#pragma unroll
-                for (int db = 0; db < D / 32; ++db)
-                    acc[db] = mfma(cols_frag<D>(lds + 2 * TILE + (2 * sub + ks) * (TILE / 4), at,
-                                                db), pf, acc[db]);
+            for (int i = 0; i < N; ++i) {
+                acc[i % (D / 32)] = mfma(f[(N + i) % AHEAD], pack8(p, i / (N / 2)),
+                                         acc[i % (D / 32)]);
+                next(N + i);
             }
         }
         arrived();
@@ -556,7 +593,7 @@ packed_attn_fwd_kernel(const PackedArgs a) {
 // The forward kernel's split.  Also writes -delta for the kernel below.  24 MFMA
 // a block of 32 keys at D 128 and less VALU work than forward (no maximum), so
 // the matrix cores bound it first.  4096 + 2500 + 1000 + 596 rows, 32/8 heads of
-// 128: 0.32 ms, 0.95 PFLOP/s; 32768 rows of the policy: 80 us, 0.68 PFLOP/s.
+// 128: 0.31 ms, 0.97 PFLOP/s; 32768 rows of the policy: 80 us, 0.68 PFLOP/s.
 template <int D, int TEAMS>
 __global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
 packed_attn_dq_kernel(const PackedArgs a) {
@@ -579,8 +616,10 @@ packed_attn_dq_kernel(const PackedArgs a) {
     const int wrow = row0 + wid % SETS * 32;
     const int row = wrow + (lane & 31);
     const bool mine = row < row1;
-    const float c2 = a.scale * LOG2E;
+    const float c2 = __uint_as_float(__builtin_amdgcn_readfirstlane(
+        __float_as_uint(a.scale * LOG2E)));
 
+    constexpr int N = D / 16, AHEAD = D == 128 ? 4 : 1;   // products of a kind, fragments read ahead
     constexpr int TILE = 64 * D * 2;
     __shared__ __attribute__((aligned(256))) char lds[4 * TILE];
     const Lane<D> lanes(lane);
@@ -616,24 +655,62 @@ packed_attn_dq_kernel(const PackedArgs a) {
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) acc[db] = zero16();
     const int wave_end = min(wrow + 32, row1);
-    // One pass over the keys.  Of s and dP, `use` makes what the pass is for.
-    auto sweep = [&](auto use) {
+    // One pass over the keys.  Of P and dP, `use` makes what the pass is for, with
+    // COUNT fragments of each block read in all.
+    auto sweep = [&](auto count, auto use) {
+        constexpr int COUNT = decltype(count)::value;
         arrived();   // the first tiles
         __syncthreads();
         for (int it = 0; it < steps; ++it) {
             if (it + 1 < steps) fetch(it + 1);
-            const Lane<D> at = lanes.fresh((it & 1) * TILE);
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
                 const int key0 = kv0 + it * 64 + sub * 32;
                 if (key0 >= wave_end || (TEAMS > 1 && sub != team)) continue;
-                f32x16_t s = zero16(), dp = zero16();
+                // a product each: N fragments of K, N of V, N of K^T for `use`
+                const Lane<D> at = lanes.fresh((it & 1) * TILE + sub * (TILE / 2));
+                auto fragment = [&](int i) {
+                    return i < N       ? rows_frag<D>(lds, at, i)
+                           : i < 2 * N ? rows_frag<D>(lds + 2 * TILE, at, i - N)
+                                       : cols_frag<D>(lds + (i - 2 * N) / (D / 32) * (TILE / 4),
+                                                      at, (i - 2 * N) % (D / 32));
+                };
+                bf16x8_t f[AHEAD];
+                auto next = [&](int i) {
+                    if (i + AHEAD < COUNT) f[i % AHEAD] = fragment(i + AHEAD);
+                    in_order<D>();
+                };
 #pragma unroll
-                for (int d = 0; d < D / 16; ++d) {
-                    s = mfma(rows_frag<D>(lds + sub * (TILE / 2), at, d), qf[d], s);
-                    dp = mfma(rows_frag<D>(lds + 2 * TILE + sub * (TILE / 2), at, d), of[d], dp);
+                for (int i = 0; i < AHEAD; ++i) f[i] = fragment(i);
+                in_order<D>();
+                f32x16_t s = zero16(), dp = zero16();
+                auto weigh = [&](int r) {
+                    s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -ls));
+                };
+                // with D 128 the exp of S goes beneath the products of dP
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    s = mfma(f[i % AHEAD], qf[i], s);
+                    next(i);
                 }
-                use(s, dp, key0, at, sub);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    dp = mfma(f[(N + i) % AHEAD], of[i], dp);
+                    if (D == 128)
+#pragma unroll
+                        for (int r = beneath(i, N); r < beneath(i + 1, N); ++r) weigh(r);
+                    next(N + i);
+                }
+                if (D == 64)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) weigh(r);
+                if (key0 + 31 > wrow) {   // not every key open to every row
+                    const int open = seldom(row - key0 - 4 * hi);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (crow(r, 0) > open) s[r] = 0.f;
+                }
+                use(s, dp, f, next);
             }
             arrived();
             __syncthreads();
@@ -642,11 +719,9 @@ packed_attn_dq_kernel(const PackedArgs a) {
     float* join = reinterpret_cast<float*>(lds) + wid % SETS * (D / 2) * 64 + lane;
     if (tile[0] == seq0) {
         float sum = 0.f;
-        sweep([&](f32x16_t& s, f32x16_t& dp, int key0, const Lane<D>&, int) {
+        sweep(std::integral_constant<int, 2 * N>{}, [&](f32x16_t& p, f32x16_t& dp, auto&, auto&) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (crow(r, 0) <= row - key0 - 4 * hi)
-                    sum = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], c2, -ls)), dp[r], sum);
+            for (int r = 0; r < 16; ++r) sum = fmaf(p[r], dp[r], sum);
         });
         if (TEAMS > 1) {
             // each team's sum to the other
@@ -659,23 +734,19 @@ packed_attn_dq_kernel(const PackedArgs a) {
         if (steps > 0) fetch(0);
     }
     if (mine && hi == 0 && team == 0) a.delta[(long)h * T + row] = -dl;
-    sweep([&](f32x16_t& s, f32x16_t& dp, int key0, const Lane<D>& at, int sub) {
+    sweep(std::integral_constant<int, 3 * N>{}, [&](f32x16_t& p, f32x16_t& dp, auto& f, auto& next) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -ls)) * (dp[r] - dl);
-        if (key0 + 31 > wrow) {   // not every key open to every row
-            const int open = seldom(row - key0 - 4 * hi);
+        for (int r = 0; r < 8; ++r) p[r] *= dp[r] - dl;
+        bf16x8_t df = pack8(p, 0);
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (crow(r, 0) > open) s[r] = 0.f;
-        }
+        for (int i = 0; i < N; ++i) {
+            if (i == N / 2) df = pack8(p, 1);
+            acc[i % (D / 32)] = mfma(f[(2 * N + i) % AHEAD], df, acc[i % (D / 32)]);
+            if (i < N / 2)
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            const bf16x8_t df = pack8(s, ks);
-#pragma unroll
-            for (int db = 0; db < D / 32; ++db)
-                acc[db] = mfma(cols_frag<D>(lds + (2 * sub + ks) * (TILE / 4), at, db), df,
-                               acc[db]);
+                for (int r = 8 + i * (16 / N); r < 8 + (i + 1) * (16 / N); ++r)
+                    p[r] *= dp[r] - dl;
+            next(2 * N + i);
         }
     });
     if (TEAMS > 1) {
