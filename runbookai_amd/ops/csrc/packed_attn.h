@@ -28,4 +28,13 @@ struct PackedArgs {
     long ot, oh;
     float* delta;   // negated
     unsigned short *dq, *dk, *dv;
+    // in how many parts the queries may be taken for dk and dv and, where that is
+    // more than one, the parts' sums and how many are there for each workgroup's keys
+    int parts, counters;
+    float* sums;
+    int* counts;
 };
+
+// The kernel for dk and dv: keys a workgroup, and workgroups that run at once.
+constexpr int packed_keys(int D) { return D == 128 ? 128 : 64; }
+constexpr int packed_slots(int D) { return D == 128 ? 256 : 3 * 256; }

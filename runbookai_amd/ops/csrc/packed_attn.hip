@@ -292,14 +292,15 @@ DEVINL void store_row(const f32x16_t (&acc)[D / 32], float factor, ushort_t* row
 // most keys first, `by_key` those with the most queries, so that the longest
 // run first and the short ones fill the gaps; entries that are left over hold
 // no rows.  One workgroup, a wave a sequence and a lane a tile: a pass that
-// counts tiles by their number in the sequence, a scan, a pass that places
-// them.  (The order within one count is free and changes no result.)
+// counts tiles by their number in the sequence, a scan (with `pairs`, how often
+// a tile of queries meets one of keys), a pass that places them.  (The order within one count is free and changes no result.)
 #define BUCKETS 4096
 #define BUILDERS 1024
 
 __global__ void __launch_bounds__(BUILDERS)
 packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
-                    int4_t* __restrict__ by_query, int4_t* __restrict__ by_key) {
+                    int4_t* __restrict__ by_query, int4_t* __restrict__ by_key,
+                    float* __restrict__ pairs) {
     __shared__ int first[BUCKETS], fill_q[BUCKETS], fill_k[BUCKETS];
     __shared__ int total;
     const int tid = threadIdx.x;
@@ -345,6 +346,7 @@ packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
     // first[k] = number of tiles in buckets above k
     if (tid < WAVE) {
         int above = 0;
+        float meet = 0.f;
         for (int top = used - 1; top >= 0; top -= WAVE) {
             const int k = top - tid;
             const int n = k >= 0 ? first[k] : 0;
@@ -355,9 +357,15 @@ packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
                 if (tid >= off) sum += v;
             }
             if (k >= 0) first[k] = above + sum - n;
+            meet += (float)n * (float)((k << shift) + 1);
             above += __shfl(sum, WAVE - 1, WAVE);
         }
-        if (tid == 0) total = above;
+#pragma unroll
+        for (int off = 1; off < WAVE; off <<= 1) meet += __shfl_xor(meet, off, WAVE);
+        if (tid == 0) {
+            total = above;
+            *pairs = meet;
+        }
     }
     __syncthreads();
     each([&](int b, int s, int e, int n, int i) {
@@ -375,10 +383,10 @@ packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
 }
 
 // Without a table (tiles null): tile `p` in the order of the sequences, found by
-// every wave for itself, a lane a sequence.  For up to PACKED_FEW sequences and so few
+// every wave for itself, a lane a sequence, and what `pairs` is above.  For up to PACKED_FEW sequences and so few
 // workgroups that all run at once, when the order does not matter: it saves a
 // launch that is 3 us on its way and 3 us of host time.
-DEVINL int4_t find_tile(const int* __restrict__ starts, int B, int T, int p) {
+DEVINL int4_t find_tile(const int* __restrict__ starts, int B, int T, int p, float& pairs) {
     const int b = threadIdx.x & (WAVE - 1);
     int s = b > 0 && b < B + 2 ? starts[b - 1] : 0;
     int e = b <= B ? starts[b] : b < B + 2 ? T : 0;
@@ -388,6 +396,9 @@ DEVINL int4_t find_tile(const int* __restrict__ starts, int B, int T, int p) {
         e = b == 0 ? T : 0;
     }
     const int n = (e - s + ROWS - 1) / ROWS;
+    pairs = 0.5f * n * (n + 1.f);
+#pragma unroll
+    for (int off = 1; off < WAVE; off <<= 1) pairs += __shfl_xor(pairs, off, WAVE);
     int upto = n;
 #pragma unroll
     for (int off = 1; off < WAVE; off <<= 1) {
@@ -445,7 +456,8 @@ packed_attn_fwd_kernel(const PackedArgs a) {
     const Place place = place_of(blockIdx.x, Hq, Hk);
     const int hk = place.hk, h = place.h, at_tile = place.tile / TEAMS;
     if (at_tile >= a.max_tiles) return;
-    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile);
+    float pairs;
+    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile, pairs);
     const int row0 = tile[0] + place.tile % TEAMS * (ROWS / TEAMS);
     const int row1 = min(tile[1], row0 + ROWS / TEAMS), seq0 = tile[2], seq1 = tile[3];
     if (SAVE && !tiles && blockIdx.x == 0)   // for the backward pass, which runs later
@@ -601,8 +613,13 @@ packed_attn_dq_kernel(const PackedArgs a) {
     const int4_t* tiles = (const int4_t*)a.tiles;
     const Place place = place_of(blockIdx.x, Hq, Hk);
     const int hk = place.hk, h = place.h, at_tile = place.tile / TEAMS;
+    if (a.parts > 1 && threadIdx.x < 2) {   // for the kernel below
+        const unsigned i = 2 * blockIdx.x + threadIdx.x;
+        if (i < (unsigned)a.counters) a.counts[i] = 0;
+    }
     if (at_tile >= a.max_tiles) return;
-    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile);
+    float pairs;
+    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile, pairs);
     const int row0 = tile[0] + place.tile % TEAMS * (ROWS / TEAMS);
     const int row1 = min(tile[1], row0 + ROWS / TEAMS), seq0 = tile[2], seq1 = tile[3];
     if (row0 >= row1) return;
@@ -766,31 +783,58 @@ packed_attn_dq_kernel(const PackedArgs a) {
 // A workgroup takes KS sets of 32 keys of one kv head (a tile or a half of it);
 // the queries of all the group's heads that see them pass through LDS, QB at a
 // time.  A wave keeps k and v of one set in registers; KS waves share the keys,
-// TEAMS of them the queries, and their sums are joined at the end.  (TEAMS 4,
-// with half the keys or twice the waves, is for grids that leave CUs idle.)
+// two teams of them the queries, and their sums are joined at the end.
 //
-// 32 MFMA a block of 32 x 32 at D 128, and as many 1 KB fragments from LDS, 8
-// cycles of its 128 bytes a cycle each: with four SIMDs LDS has to be read as
-// long as the matrix cores run, and both bound it.  64 keys a wave would halve
-// the reads, but its 4 x 64 x D sums and operands do not fit 512 registers (761
-// against 510 us).  At D 128 one workgroup of 8 waves has all of LDS, so that a
-// tile of 128 queries serves 128 keys; at D 64 three buffers of 64 queries keep
-// two tiles on their way.  4096 + 2500 + 1000 + 596 rows, 32/8 heads of 128:
-// 0.50 ms, 0.80 PFLOP/s; 32768 rows of the policy: 102 us, 0.71 PFLOP/s.
-template <int D, int KS, int TEAMS, int QB, int NBUF>
-__global__ void __launch_bounds__(KS * TEAMS * 64, D == 128 || KS * TEAMS > 4 ? 2 : 3)
+// These workgroups are few and of unequal length (the first keys are seen by all
+// queries), and the longest can take far longer than the card's share of the
+// work.  So the queries of a long one are split in up to `parts` workgroups.
+// Each leaves its sums in memory and counts itself; the last to come adds all
+// sums in their order, so the same inputs give the same bits, and nobody waits.
+// Sums and count go past the caches (relaxed atomics of agent scope): a fence
+// would write back and drop an XCD's whole L2, which made everything slower (1.06
+// ms instead of 0.81).  The parts are the outer order of the grid, as the many
+// that are not there would else leave every other CU idle.
+//
+// 32 MFMA a block of 32 x 32 at D 128, and as many 1 KB fragments from LDS, each
+// read for one product.  LDS is busy a quarter of the time and the matrix cores
+// 37 %; VALU work (a quarter) overlaps with neither in full, and a wave has no
+// registers left to read far ahead (254; 64 keys a wave, which would halve the
+// reads, spilled: 761 against 510 us).  At D 128 one workgroup of 8 waves has all
+// of LDS, so that a tile of 128 queries serves 128 keys; at D 64 three buffers of
+// 64 queries keep two tiles on their way.  4096 + 2500 + 1000 + 596 rows, 32/8
+// heads of 128: 0.46 ms, 0.87 PFLOP/s (0.51 unsplit); 32768 rows of the policy: 102 us, 0.71
+// PFLOP/s.
+template <int D, int KS, int QB, int NBUF>
+__global__ void __launch_bounds__(KS * 128, D == 128 ? 2 : 3)
 packed_attn_dkv_kernel(const PackedArgs a) {
     const int T = a.T, Hq = a.Hq, Hk = a.Hk;
     const int4_t* tiles = a.tiles ? (const int4_t*)a.tiles + a.max_tiles : nullptr;
-    constexpr int PARTS = 4 / KS;
+    float pairs = tiles ? *(const float*)(tiles + a.max_tiles) : 0.f;
+    static_assert(QB == KS * 32 && QB == packed_keys(D), "as many queries as keys");
+    constexpr int TEAMS = 2, BITS = 4 / KS, SLOTS = packed_slots(D), WORTH = D == 128 ? 8 : 16;
     const int hk = blockIdx.x % Hk;
     const int group = Hq / Hk;
-    const int at_tile = blockIdx.x / (Hk * PARTS);
-    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile);
-    const int row0 = tile[0] + blockIdx.x / Hk % PARTS * (KS * 32);
+    // first the last parts, which few tiles have, and those few the first ones
+    const int bits = a.max_tiles * BITS;
+    const int part = a.parts - 1 - blockIdx.x / Hk / bits;
+    const int bit = blockIdx.x / Hk % bits;
+    const int at_tile = bit / BITS;
+    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile, pairs);
+    const int row0 = tile[0] + bit % BITS * (KS * 32);
     const int row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
     if (row0 >= row1) return;
     const bool real = seq1 > seq0;
+    // Steps of QB of one head's queries that see the keys, and the steps that come
+    // to each slot if all are shared out: what would take WORTH steps longer is
+    // split (where all workgroups run at once, already over three quarters of it).
+    const int turns = (seq1 - row0 + QB - 1) / QB, all = real ? turns * group : 0;
+    const float share =
+        pairs * ((ROWS / QB) * (ROWS / QB) * Hq) / SLOTS * (a.parts > 2 ? 0.75f : 1.f);
+    const int parts = __builtin_amdgcn_readfirstlane(
+        all > share + WORTH ? min(a.parts, (int)ceilf(all / fmaxf(share, WORTH / 2.f))) : 1);
+    if (part >= parts) return;
+    const int step0 = (int)((long)all * part / parts);
+    const int steps = (int)((long)all * (part + 1) / parts) - step0;
     const int lane = threadIdx.x & (WAVE - 1);
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int hi = lane >> 5;
@@ -821,20 +865,20 @@ packed_attn_dkv_kernel(const PackedArgs a) {
 
     const Mover<D, QB, KS * TEAMS * 64> mq(a.qt), mo(a.ot);
     // each wave also moves 64 rows' log-sums or deltas (where there are more
-    // waves than parts, two move the same)
+    // waves than these, two move the same)
     static_assert(QB % 64 == 0 && KS * TEAMS % (QB / 32) == 0, "by wave");
-    const int part = wid % (QB / 32) / 2;
+    const int rows64 = wid % (QB / 32) / 2;
     const bool sums = wid % 2 == 0;
     auto fetch = [&](int h, int r0, int buf) {
         mq.move(a.q + h * a.qh, r0, seq1 - 1, ql + buf * TILE);
         mo.move(a.dout + h * a.oh, r0, seq1 - 1, ol + buf * TILE);
         const float* from = (sums ? a.lse : a.delta) + (long)h * T;
-        const float* to = (sums ? lds.ls[buf] : lds.dl[buf]) + part * 64;
-        move64(from, min(r0 + part * 64 + lane, seq1 - 1), to);
+        const float* to = (sums ? lds.ls[buf] : lds.dl[buf]) + rows64 * 64;
+        move64(from, min(r0 + rows64 * 64 + lane, seq1 - 1), to);
     };
     constexpr int AHEAD = NBUF - 1, LEFT = (NBUF - 2) * (2 * mq.LOADS + 1);
-    const int steps = real ? (seq1 - row0 + QB - 1) / QB * group : 0;
-    int h = hk * group, r0 = row0;     // what is fetched next
+    const int start = real ? row0 + step0 % turns * QB : row0;
+    int h = hk * group + (real ? step0 / turns : 0), r0 = start;   // what is fetched next
     auto next = [&](int buf) {
         fetch(h, r0, buf);
         r0 += QB;
@@ -851,7 +895,7 @@ packed_attn_dkv_kernel(const PackedArgs a) {
     if (steps >= AHEAD) arrived<LEFT>();
     else arrived<0>();
     __syncthreads();
-    int now = row0;   // first row of the step
+    int now = start;   // first row of the step
     for (int it = 0, buf = 0; it < steps; ++it, buf = buf + 1 < NBUF ? buf + 1 : 0) {
         const bool more = it + AHEAD < steps;
         if (more) next(buf ? buf - 1 : NBUF - 1);
@@ -917,29 +961,62 @@ packed_attn_dkv_kernel(const PackedArgs a) {
         else arrived<0>();
         __syncthreads();
     }
-    // the other teams' dv to the first, then their dk to the second
+    // dv to the first team, then dk to the second
     auto joined = [&](f32x16_t (&x)[D / 32], int to) {
         float* join = reinterpret_cast<float*>(lds.x) + wid % KS * 32 * D + lane;
-        static_assert((TEAMS - 1) * KS * 32 * D * 4 <= 2 * NBUF * TILE, "fits the tiles");
-        if (team != to) {
-            join += (team < to ? team : team - 1) * KS * 32 * D;
+        static_assert(KS * 32 * D * 4 <= 2 * NBUF * TILE, "fits the tiles");
+        if (team != to)
 #pragma unroll
             for (int i = 0; i < D / 2; ++i) join[i * 64] = x[i / 16][i % 16];
-        }
         __syncthreads();
         if (team == to)
 #pragma unroll
-            for (int other = 0; other < TEAMS - 1; ++other)
-#pragma unroll
-                for (int i = 0; i < D / 2; ++i)
-                    x[i / 16][i % 16] += join[other * KS * 32 * D + i * 64];
+            for (int i = 0; i < D / 2; ++i) x[i / 16][i % 16] += join[i * 64];
     };
-    const long to = ((long)key * Hk + hk) * D;
     joined(av, 0);
-    if (team == 0) store_row<D>(av, seq1 < 0 ? NAN : 1.f, a.dv + to, hi, nullptr, mine);
     __syncthreads();
     joined(ak, 1);
-    if (team == 1) store_row<D>(ak, seq1 < 0 ? NAN : a.scale, a.dk + to, hi, nullptr, mine);
+    if (team == 1)   // from here on av is dv with team 0 and dk with team 1
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) av[db] = ak[db];
+    if (parts > 1) {
+        // The last workgroup of the parts adds them all, in their order.
+        union Two { float f[2]; unsigned long u; };
+        const long slot = (long)bit * Hk + hk;
+        auto sums = [&](int part) {
+            return reinterpret_cast<unsigned long*>(
+                       a.sums + (((slot * a.parts + part) * 2 + team) * KS + wid % KS) * (32 * D)) +
+                   lane;
+        };
+        unsigned long* const to = sums(part);
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i)
+            __hip_atomic_store(to + i * 64, Two{{av[i / 8][i % 8 * 2], av[i / 8][i % 8 * 2 + 1]}}.u,
+                               __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        arrived();
+        __syncthreads();
+        int& before = reinterpret_cast<int*>(lds.x)[0];
+        if (threadIdx.x == 0)
+            before = __hip_atomic_fetch_add(a.counts + slot, 1, __ATOMIC_RELAXED,
+                                            __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (before != parts - 1) return;
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) av[db] = zero16();
+        for (int p = 0; p < parts; ++p) {
+            unsigned long* const from = sums(p);
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) {
+                Two v;
+                v.u = __hip_atomic_load(from + i * 64, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                av[i / 8][i % 8 * 2] += v.f[0];
+                av[i / 8][i % 8 * 2 + 1] += v.f[1];
+            }
+        }
+    }
+    const long to = ((long)key * Hk + hk) * D;
+    const float factor = seq1 < 0 ? NAN : team ? a.scale : 1.f;
+    store_row<D>(av, factor, (team ? a.dk : a.dv) + to, hi, nullptr, mine);
 }
 
 // ---------------------------------------------------------------- launchers
@@ -948,7 +1025,8 @@ packed_attn_dkv_kernel(const PackedArgs a) {
 extern "C" int launch_packed_tiles(const PackedArgs* a, void* stream) {
     int4_t* tiles = (int4_t*)a->tiles;
     hipLaunchKernelGGL(packed_tiles_kernel, dim3(1), dim3(BUILDERS), 0, (hipStream_t)stream,
-                       a->starts, a->B, a->T, a->max_tiles, tiles, tiles + a->max_tiles);
+                       a->starts, a->B, a->T, a->max_tiles, tiles, tiles + a->max_tiles,
+                       (float*)(tiles + 2 * (long)a->max_tiles));
     return (int)hipGetLastError();
 }
 
@@ -974,31 +1052,28 @@ void dq_(const PackedArgs* a, hipStream_t st) {
                        grid_of(a, a->max_tiles * TEAMS), dim3(256), 0, st, *a);
 }
 
-template <int D, int KS, int TEAMS, int QB, int NBUF>
+template <int D, int KS, int QB, int NBUF>
 void dkv(const PackedArgs* a, hipStream_t st) {
-    hipLaunchKernelGGL((packed_attn_dkv_kernel<D, KS, TEAMS, QB, NBUF>),
-                       dim3((unsigned)a->max_tiles * a->Hk * (4 / KS)), dim3(KS * TEAMS * 64), 0,
-                       st, *a);
+    hipLaunchKernelGGL((packed_attn_dkv_kernel<D, KS, QB, NBUF>),
+                       dim3((unsigned)a->max_tiles * a->Hk * (4 / KS) * a->parts), dim3(KS * 128),
+                       0, st, *a);
 }
 
 // Whether the usual split leaves CUs with a workgroup or two less than fit: then
-// more waves take a tile.  With and without (us; 8/4 heads of 64, 32/8 of 128):
-//   workgroups           forward     dq          dk/dv
-//   88   1024, 8/4       14.5 19.2   17.0 22.1   24.3 32.1
-//   328  3 x 1536, 8/4   26.4 32.5   31.4 37.5   36.8 49.6
-//   448  6 x 1024, 8/4   23.4 27.5   28.3 32.5   41.1 41.8
+// two teams of waves take a tile.  With and without (us; 8/4 heads of 64, 32/8 of
+// 128):
+//   workgroups           forward     dq
+//   88   1024, 8/4       14.5 19.2   17.0 22.1
+//   328  3 x 1536, 8/4   26.4 32.5   31.4 37.5
+//   448  6 x 1024, 8/4   23.4 27.5   28.3 32.5
 //   736  1916, 32/8      33.6 33.4   47.4 43.7
-//   152  2048, 32/8                              147 221
-//   592  8 x 1024, 32/8                          229 151
-bool sparse(const PackedArgs* a, int heads, int fit = 2) {
-    return a->max_tiles * heads <= 256 * fit;
-}
+bool sparse(const PackedArgs* a) { return a->max_tiles * a->Hq <= 512; }
 
 }  // namespace
 
 extern "C" int launch_packed_attn_fwd(const PackedArgs* a, void* stream) {
     const hipStream_t st = (hipStream_t)stream;
-    const bool few = sparse(a, a->Hq);
+    const bool few = sparse(a);
     if (a->D == 128) few ? fwd<128, 2>(a, st) : fwd<128, 1>(a, st);
     else few ? fwd<64, 2>(a, st) : fwd<64, 1>(a, st);
     return (int)hipGetLastError();
@@ -1006,7 +1081,7 @@ extern "C" int launch_packed_attn_fwd(const PackedArgs* a, void* stream) {
 
 extern "C" int launch_packed_attn_dq(const PackedArgs* a, void* stream) {
     const hipStream_t st = (hipStream_t)stream;
-    const bool few = sparse(a, a->Hq);
+    const bool few = sparse(a);
     if (a->D == 128) few ? dq_<128, 2>(a, st) : dq_<128, 1>(a, st);
     else few ? dq_<64, 2>(a, st) : dq_<64, 1>(a, st);
     return (int)hipGetLastError();
@@ -1014,8 +1089,7 @@ extern "C" int launch_packed_attn_dq(const PackedArgs* a, void* stream) {
 
 extern "C" int launch_packed_attn_dkv(const PackedArgs* a, void* stream) {
     const hipStream_t st = (hipStream_t)stream;
-    if (a->D == 128)   // one workgroup a CU
-        sparse(a, a->Hk, 1) ? dkv<128, 2, 4, 128, 2>(a, st) : dkv<128, 4, 2, 128, 2>(a, st);
-    else sparse(a, 2 * a->Hk) ? dkv<64, 2, 4, 128, 2>(a, st) : dkv<64, 2, 2, 64, 3>(a, st);
+    if (a->D == 128) dkv<128, 4, 128, 2>(a, st);
+    else dkv<64, 2, 64, 3>(a, st);
     return (int)hipGetLastError();
 }

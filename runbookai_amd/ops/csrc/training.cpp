@@ -130,12 +130,30 @@ bool plan_tiles(PackedArgs& a, long B) {
     return B > PACKED_FEW || most * a.Hq > 512;
 }
 
+// In how many parts the kernel for dk and dv may take a workgroup's queries.  It
+// splits only what is longer than the card's share; but workgroups of parts that
+// are not there cost a little, and their sums need memory.  dq and dk/dv with 1, 2
+// and 4 parts at most (us), by workgroups:
+//   32/8 heads of 128 (256 run at once)      8/4 heads of 64 (768)
+//     88  1024             143 102  84         88  1024            51  41  39
+//    152  2048             290 203 197        280  4096           175 139 118
+//    280  4096             655 585 587        536  8192           400 347 343
+//    304  4 x 1024         201 180 181        792  12288          669 638 639
+//    560  4096 to 596      775 731 739       1528  24000         2014 2001 2015
+//    592  8 x 1024         328 327 327       2350  36 x 64..1536  188 189 193
+void plan_parts(PackedArgs& a, bool keys) {
+    const long slots = packed_slots(a.D);
+    const long all = (long)a.max_tiles * a.Hk * (PACKED_ROWS / packed_keys(a.D));
+    a.parts = !keys || all > 3 * slots ? 1 : all > slots ? 2 : 4;
+    a.counters = a.parts > 1 ? (int)all : 0;
+}
+
 // What the forward pass keeps for the backward one, and the table of tiles.
 struct Kept {
     Parts parts;
     size_t tiles, rest = 0, lse = 0;
     Kept(const PackedArgs& a, bool table, bool save)
-        : tiles(parts.add(table ? 32 * (size_t)a.max_tiles : save ? 4 * ((size_t)a.B + 1) : 0)) {
+        : tiles(parts.add(table ? 32 * (size_t)a.max_tiles + 16 : save ? 4 * ((size_t)a.B + 1) : 0)) {
         if (!save) return;
         rest = parts.add(2 * (size_t)a.T * a.Hq * a.D);
         lse = parts.add(4 * (size_t)a.T * a.Hq);
@@ -187,8 +205,14 @@ std::vector<Tensor> packed_attn_bwd(const Tensor& dout, const Tensor& q, const T
         dv = torch::empty({a.T, a.Hk, a.D}, opt);
     }
     if (a.T > 0) {
-        const Tensor delta = torch::empty({a.Hq, a.T}, opt.dtype(torch::kFloat32));
         const bool table = plan_tiles(a, B);
+        Parts parts;
+        const size_t delta = parts.add(4 * (size_t)a.Hq * a.T);
+        plan_parts(a, keys);
+        const size_t counts = parts.add(a.parts > 1 ? 4 * (size_t)a.counters : 0);
+        const size_t sums = parts.add(a.parts > 1 ? 8 * (size_t)a.counters * a.parts *
+                                                        packed_keys(a.D) * a.D : 0);
+        const Tensor scratch = parts.make(q);
         const Kept at(a, table, true);
         if (table) a.tiles = part<void>(kept, at.tiles);
         else a.starts = part<int>(kept, at.tiles);
@@ -196,7 +220,9 @@ std::vector<Tensor> packed_attn_bwd(const Tensor& dout, const Tensor& q, const T
         a.out_lo = part<unsigned short>(kept, at.rest);
         a.lse = part<float>(kept, at.lse);
         a.dout = bf16(dout); a.ot = dout.stride(0); a.oh = dout.stride(1);
-        a.delta = delta.data_ptr<float>();
+        a.delta = part<float>(scratch, delta);
+        a.counts = part<int>(scratch, counts);
+        a.sums = part<float>(scratch, sums);
         a.dq = bf16(dq);
         void* st = stream_of(q);
         launched(launch_packed_attn_dq(&a, st), "packed_attention's gradient");

@@ -191,6 +191,23 @@ def test_attention_gpu_large_grids(lens, heads, d):
 
 
 @gpu
+@pytest.mark.parametrize("lens,heads,d", [
+    ([2300], (8, 1), 64), ([1, 1900, 130], (4, 4), 64), ([700] * 4, (4, 2), 64),
+    ([1500, 40, 700], (8, 2), 128), ([300] * 5 + [2000], (16, 2), 128), ([1100], (2, 2), 128)])
+def test_attention_gpu_split_gradients(lens, heads, d):
+    """Long sequences in few tiles, whose dk and dv are summed by several
+    workgroups: right, and the same bits every time."""
+    q, k, v, dout = _inputs(lens, heads, d, pad=5, device="cuda")
+    starts = torch.tensor(_starts(lens), dtype=torch.int32, device="cuda")
+    got = _attend(q, k, v, dout, starts)
+    want, tol = attention_oracle(q, k, v, dout, _starts(lens), 1.0 / math.sqrt(d))
+    _within(got, want, tol)
+    for _ in range(20):
+        for x, y in zip(_attend(q, k, v, dout, starts), got):
+            assert torch.equal(x, y)
+
+
+@gpu
 @pytest.mark.parametrize("d", [64, 128])
 def test_attention_gpu_sharp_scores(d):
     """Scores far apart: the running maximum grows many times, and most
@@ -330,10 +347,12 @@ def test_attention_gpu_repeats_bit_for_bit_on_another_stream():
 
 
 @gpu
-def test_attention_gpu_captured():
+@pytest.mark.parametrize("T,cuts", [
+    (400, ([100, 100, 380], [1, 399, 400], [0, 0, 256])),
+    (2100, ([2100] * 3, [1, 1000, 1100], [0, 0, 1700], [600, 1200, 2100], [2100] * 3))])
+def test_attention_gpu_captured(T, cuts):
     """Forward and backward in one graph: new data and new sequences in the
     same buffers, replayed between eager calls."""
-    T = 400
     q, k, v, dout = _inputs([T], (4, 2), 64, device="cuda")
     starts = torch.tensor([0, 100, 100, 380], dtype=torch.int32, device="cuda")
     leaves = [x.requires_grad_() for x in (q, k, v)]
@@ -350,7 +369,7 @@ def test_attention_gpu_captured():
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         static = step()
-    for i, ends in enumerate(([100, 100, 380], [1, 399, 400], [0, 0, 256])):
+    for i, ends in enumerate(cuts):
         with torch.no_grad():
             for x, y in zip((q, k, v, dout), _inputs([T], (4, 2), 64, device="cuda", seed=i)):
                 x.copy_(y)
