@@ -172,17 +172,20 @@ struct Mover {
         off = row * (unsigned)pitch + chunk;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE) * (WAVE * 16);
     }
+    DEVINL const char* at(const ushort_t* base, int row) const {
+        return reinterpret_cast<const char*>(base) + row * pitch;
+    }
     DEVINL static void issue(unsigned to, unsigned at, const char* from) {
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                      :
                      : "s"(to), "v"(at), "s"(from)
                      : "memory", "m0");
     }
-    DEVINL void move(const ushort_t* base, int row0, int last, char* tile) const {
-        const char* from = reinterpret_cast<const char*>(base) + row0 * pitch;
+    // from row 0 of the tile on, which ends with row `last`
+    DEVINL void move(const char* from, int last, char* tile) const {
         const unsigned to =
             (unsigned)(unsigned long)(__attribute__((address_space(3))) char*)tile + wave;
-        if (row0 + N - 1 <= last) {
+        if (N - 1 <= last) {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i)
                 issue(to + i * STEP * D * 2, off, from + i * STEP * pitch);
@@ -191,7 +194,7 @@ struct Mover {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i)
                 issue(to + i * STEP * D * 2,
-                      __umul24(min(r + i * STEP, last - row0), (unsigned)pitch) + chunk, from);
+                      __umul24(min(r + i * STEP, last), (unsigned)pitch) + chunk, from);
         }
     }
 };
@@ -491,9 +494,12 @@ packed_attn_fwd_kernel(const PackedArgs a) {
     const ushort_t *k = a.k + hk * a.kh, *v = a.v + hk * a.vh;
     const Mover<D, 64, 256> mk(a.kt), mv(a.vt);
     const int steps = (kv1 - kv0 + 63) / 64;
+    const char *knext = mk.at(k, kv0), *vnext = mv.at(v, kv0);
     auto fetch = [&](int it) {
-        mk.move(k, kv0 + it * 64, kv1 - 1, lds + (it & 1) * TILE);
-        mv.move(v, kv0 + it * 64, kv1 - 1, lds + (2 + (it & 1)) * TILE);
+        mk.move(knext, kv1 - 1 - (kv0 + it * 64), lds + (it & 1) * TILE);
+        mv.move(vnext, kv1 - 1 - (kv0 + it * 64), lds + (2 + (it & 1)) * TILE);
+        knext += 64 * mk.pitch;
+        vnext += 64 * mv.pitch;
     };
     if (steps > 0) fetch(0);
     settle(qf);
@@ -644,9 +650,12 @@ packed_attn_dq_kernel(const PackedArgs a) {
     const ushort_t *k = a.k + hk * a.kh, *v = a.v + hk * a.vh;
     const Mover<D, 64, 256> mk(a.kt), mv(a.vt);
     const int steps = (kv1 - kv0 + 63) / 64;
+    const char *knext = mk.at(k, kv0), *vnext = mv.at(v, kv0);
     auto fetch = [&](int it) {
-        mk.move(k, kv0 + it * 64, kv1 - 1, lds + (it & 1) * TILE);
-        mv.move(v, kv0 + it * 64, kv1 - 1, lds + (2 + (it & 1)) * TILE);
+        mk.move(knext, kv1 - 1 - (kv0 + it * 64), lds + (it & 1) * TILE);
+        mv.move(vnext, kv1 - 1 - (kv0 + it * 64), lds + (2 + (it & 1)) * TILE);
+        knext += 64 * mk.pitch;
+        vnext += 64 * mv.pitch;
     };
     if (steps > 0) fetch(0);
     bf16x8_t qf[D / 16], of[D / 16];
@@ -748,6 +757,8 @@ packed_attn_dq_kernel(const PackedArgs a) {
             __syncthreads();
         }
         dl = both_sum(sum);
+        knext = mk.at(k, kv0);
+        vnext = mv.at(v, kv0);
         if (steps > 0) fetch(0);
     }
     if (mine && hi == 0 && team == 0) a.delta[(long)h * T + row] = -dl;
@@ -802,8 +813,8 @@ packed_attn_dq_kernel(const PackedArgs a) {
 // reads, spilled: 761 against 510 us).  At D 128 one workgroup of 8 waves has all
 // of LDS, so that a tile of 128 queries serves 128 keys; at D 64 three buffers of
 // 64 queries keep two tiles on their way.  4096 + 2500 + 1000 + 596 rows, 32/8
-// heads of 128: 0.46 ms, 0.87 PFLOP/s (0.51 unsplit); 32768 rows of the policy: 102 us, 0.71
-// PFLOP/s.
+// heads of 128: 0.46 ms, 0.87 PFLOP/s (0.51 unsplit); 32768 rows of the policy:
+// 102 us, 0.71 PFLOP/s.
 template <int D, int KS, int QB, int NBUF>
 __global__ void __launch_bounds__(KS * 128, D == 128 ? 2 : 3)
 packed_attn_dkv_kernel(const PackedArgs a) {
@@ -869,22 +880,33 @@ packed_attn_dkv_kernel(const PackedArgs a) {
     static_assert(QB % 64 == 0 && KS * TEAMS % (QB / 32) == 0, "by wave");
     const int rows64 = wid % (QB / 32) / 2;
     const bool sums = wid % 2 == 0;
-    auto fetch = [&](int h, int r0, int buf) {
-        mq.move(a.q + h * a.qh, r0, seq1 - 1, ql + buf * TILE);
-        mo.move(a.dout + h * a.oh, r0, seq1 - 1, ol + buf * TILE);
-        const float* from = (sums ? a.lse : a.delta) + (long)h * T;
-        const float* to = (sums ? lds.ls[buf] : lds.dl[buf]) + rows64 * 64;
-        move64(from, min(r0 + rows64 * 64 + lane, seq1 - 1), to);
-    };
     constexpr int AHEAD = NBUF - 1, LEFT = (NBUF - 2) * (2 * mq.LOADS + 1);
+    // what is fetched next
     const int start = real ? row0 + step0 % turns * QB : row0;
-    int h = hk * group + (real ? step0 / turns : 0), r0 = start;   // what is fetched next
+    int h = hk * group + (real ? step0 / turns : 0), r0 = start;
+    const float* const rows = sums ? a.lse : a.delta;
+    const char *qnext, *onext;
+    const float* snext;
+    auto begin = [&] {
+        qnext = mq.at(a.q + h * a.qh, r0);
+        onext = mo.at(a.dout + h * a.oh, r0);
+        snext = rows + (long)h * T + r0;
+    };
+    begin();
     auto next = [&](int buf) {
-        fetch(h, r0, buf);
+        const int last = seq1 - 1 - r0;
+        mq.move(qnext, last, ql + buf * TILE);
+        mo.move(onext, last, ol + buf * TILE);
+        move64(snext, min(rows64 * 64 + lane, last),
+               (sums ? lds.ls[buf] : lds.dl[buf]) + rows64 * 64);
         r0 += QB;
+        qnext += QB * mq.pitch;
+        onext += QB * mo.pitch;
+        snext += QB;
         if (r0 >= seq1) {
             r0 = row0;
             ++h;
+            begin();
         }
     };
 #pragma unroll
