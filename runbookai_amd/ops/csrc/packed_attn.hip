@@ -385,11 +385,24 @@ packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
         by_query[i] = by_key[i] = int4_t{0, 0, 0, 0};
 }
 
-// Without a table (tiles null): tile `p` in the order of the sequences, found by
-// every wave for itself, a lane a sequence, and what `pairs` is above.  For up to PACKED_FEW sequences and so few
-// workgroups that all run at once, when the order does not matter: it saves a
-// launch that is 3 us on its way and 3 us of host time.
-DEVINL int4_t find_tile(const int* __restrict__ starts, int B, int T, int p, float& pairs) {
+// op(x, y, ...) of the wave's lanes, with 0 for none
+template <typename Op>
+DEVINL int wave_fold(int x, Op op) {
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));   // row_shr 1, 2,
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));   // 4, 8: within
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));   // each 16 lanes
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));   // row_bcast 15, 31
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+    return __builtin_amdgcn_readlane(x, WAVE - 1);
+}
+
+// Entry p of that table, without a table (tiles null): found by every wave for
+// itself, a lane a sequence, for up to PACKED_FEW sequences.  How many tiles are
+// the i-th or later of their sequence falls with i: a search for the i where it
+// passes p.  (Also `pairs`.)
+DEVINL int4_t find_tile(const int* __restrict__ starts, int B, int T, int p, bool by_key,
+                        float& pairs) {
     const int b = threadIdx.x & (WAVE - 1);
     int s = b > 0 && b < B + 2 ? starts[b - 1] : 0;
     int e = b <= B ? starts[b] : b < B + 2 ? T : 0;
@@ -402,17 +415,25 @@ DEVINL int4_t find_tile(const int* __restrict__ starts, int B, int T, int p, flo
     pairs = 0.5f * n * (n + 1.f);
 #pragma unroll
     for (int off = 1; off < WAVE; off <<= 1) pairs += __shfl_xor(pairs, off, WAVE);
-    int upto = n;
-#pragma unroll
-    for (int off = 1; off < WAVE; off <<= 1) {
-        const int v = __shfl_up(upto, off, WAVE);
-        if (b >= off) upto += v;
+    const auto sum = [](int x, int y) { return x + y; };
+    if (wave_fold(n, sum) <= p) return int4_t{0, 0, 0, 0};
+    int i = 0, past = wave_fold(n, [](int x, int y) { return max(x, y); });
+    int before = 0;   // tiles that are the past-th or later
+    while (past - i > 1) {
+        const int mid = (i + past) / 2, later = wave_fold(max(n - mid, 0), sum);
+        if (later > p) {
+            i = mid;
+        } else {
+            past = mid;
+            before = later;
+        }
     }
-    const int seq = __popcll(__ballot(upto <= p));   // those that end before it
-    if (seq == WAVE) return int4_t{0, 0, 0, 0};
+    const unsigned long have = __ballot(n > i);
+    const int rank = __popcll(have & ((1ul << b) - 1));
+    const int seq = __ffsll(__ballot(n > i && rank == p - before)) - 1;
     s = __builtin_amdgcn_readlane(s, seq);
     e = __builtin_amdgcn_readlane(e, seq);
-    const int r0 = s + (p - __builtin_amdgcn_readlane(upto - n, seq)) * ROWS;
+    const int r0 = s + (by_key ? __builtin_amdgcn_readlane(n, seq) - 1 - i : i) * ROWS;
     const bool real = !wrong && seq > 0 && seq <= B;
     return int4_t{r0, min(r0 + ROWS, e), real ? s : r0, real ? e : wrong ? -1 : r0};
 }
@@ -460,7 +481,7 @@ packed_attn_fwd_kernel(const PackedArgs a) {
     const int hk = place.hk, h = place.h, at_tile = place.tile / TEAMS;
     if (at_tile >= a.max_tiles) return;
     float pairs;
-    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile, pairs);
+    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile, false, pairs);
     const int row0 = tile[0] + place.tile % TEAMS * (ROWS / TEAMS);
     const int row1 = min(tile[1], row0 + ROWS / TEAMS), seq0 = tile[2], seq1 = tile[3];
     if (SAVE && !tiles && blockIdx.x == 0)   // for the backward pass, which runs later
@@ -625,7 +646,7 @@ packed_attn_dq_kernel(const PackedArgs a) {
     }
     if (at_tile >= a.max_tiles) return;
     float pairs;
-    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile, pairs);
+    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile, false, pairs);
     const int row0 = tile[0] + place.tile % TEAMS * (ROWS / TEAMS);
     const int row1 = min(tile[1], row0 + ROWS / TEAMS), seq0 = tile[2], seq1 = tile[3];
     if (row0 >= row1) return;
@@ -830,7 +851,7 @@ packed_attn_dkv_kernel(const PackedArgs a) {
     const int part = a.parts - 1 - blockIdx.x / Hk / bits;
     const int bit = blockIdx.x / Hk % bits;
     const int at_tile = bit / BITS;
-    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile, pairs);
+    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile, true, pairs);
     const int row0 = tile[0] + bit % BITS * (KS * 32);
     const int row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
     if (row0 >= row1) return;

@@ -118,16 +118,18 @@ PackedArgs packed_args(const Tensor& q, const Tensor& k, const Tensor& v, double
     return a;
 }
 
-// Where the tiles come from: a table or, for few sequences in few tiles, just
-// the starts (a workgroup of 128 rows for each head: up to 512 run at once
-// whatever the head dim).  -> whether by a table
-bool plan_tiles(PackedArgs& a, long B) {
+// Where the tiles come from: a table or, for few sequences, just the starts.  The
+// table is a launch of 4 to 5 us; to search the starts makes each kernel 1 to 2 us
+// longer where workgroups follow one another (0.5 where all run at once, up to
+// about 512), so a forward pass alone searches, and three kernels share a table.
+// -> whether by a table
+bool plan_tiles(PackedArgs& a, long B, bool gradients) {
     const long most = a.T / PACKED_ROWS + B + 2;
     // a launch's threads are counted in 32 bits
     TORCH_CHECK(most * a.Hq * 512 < (1L << 32), "too many rows and sequences for one call");
     a.B = (int)B;
     a.max_tiles = (int)most;
-    return B > PACKED_FEW || most * a.Hq > 512;
+    return B > PACKED_FEW || (gradients && most * a.Hq > 512);
 }
 
 // In how many parts the kernel for dk and dv may take a workgroup's queries.  It
@@ -169,7 +171,7 @@ std::vector<Tensor> packed_attn_fwd(const Tensor& q, const Tensor& k, const Tens
                 "seq_starts must be a dense int32 vector on the device of q");
     const c10::cuda::CUDAGuard guard(q.device());
     const Tensor out = torch::empty({a.T, a.Hq, a.D}, q.options());
-    const bool table = plan_tiles(a, starts.numel() - 1);
+    const bool table = plan_tiles(a, starts.numel() - 1, save);
     const Kept at(a, table, save);
     Tensor kept;
     if (at.parts.size) kept = at.parts.make(q);
@@ -205,7 +207,7 @@ std::vector<Tensor> packed_attn_bwd(const Tensor& dout, const Tensor& q, const T
         dv = torch::empty({a.T, a.Hk, a.D}, opt);
     }
     if (a.T > 0) {
-        const bool table = plan_tiles(a, B);
+        const bool table = plan_tiles(a, B, true);
         Parts parts;
         const size_t delta = parts.add(4 * (size_t)a.Hq * a.T);
         plan_parts(a, keys);

@@ -208,6 +208,21 @@ def test_attention_gpu_split_gradients(lens, heads, d):
 
 
 @gpu
+@pytest.mark.parametrize("lens,heads,d", [
+    ([1500, 0, 700, 64, 1, 1300], (8, 4), 64), ([4000], (32, 8), 128), ([129] * 62, (16, 2), 64),
+    ([129] * 63, (16, 2), 64), (list(range(20, 320, 5)), (8, 8), 128)])
+def test_attention_gpu_forward_alone(lens, heads, d):
+    """Without gradients to come, tiles are found another way: the same bits."""
+    q, k, v, dout = _inputs(lens, heads, d, pad=200, device="cuda")
+    starts = torch.tensor(_starts(lens), dtype=torch.int32, device="cuda") + 100
+    want = _attend(q, k, v, dout, starts)[0]
+    q[:100] = math.nan
+    q[100 + sum(lens):] = math.nan
+    with torch.no_grad():
+        assert torch.equal(ops.packed_attention(q, k, v, starts), want)
+
+
+@gpu
 @pytest.mark.parametrize("d", [64, 128])
 def test_attention_gpu_sharp_scores(d):
     """Scores far apart: the running maximum grows many times, and most
