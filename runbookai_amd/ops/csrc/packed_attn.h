@@ -12,17 +12,16 @@ struct PackedArgs {
     long qt, qh, kt, kh, vt, vh;
     int T, Hq, Hk, D;
     float scale;
-    // where the tiles are: a table of max_tiles by query and as many by key, or
-    // (tiles null) the starts of B sequences
+    // the tiles: a table of max_tiles by query, as many by key, and how many pairs
+    // of them meet.  It is built from the starts of B sequences or (search) found
+    // by the forward kernel, which leaves it where a backward pass will follow.
     const int* starts;
     void* tiles;
-    int B, max_tiles;
+    int B, max_tiles, search;
     // the forward pass writes out and, where a backward pass will follow (lse not
-    // null), what out's rounding left over, the rows' log-sums and, without
-    // tiles, a copy of the starts; the backward pass reads them
+    // null), what out's rounding left over and the rows' log-sums
     unsigned short *out, *out_lo;
     float* lse;
-    int* kept_starts;
     // the backward pass
     const unsigned short* dout;
     long ot, oh;

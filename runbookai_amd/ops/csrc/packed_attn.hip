@@ -397,11 +397,11 @@ DEVINL int wave_fold(int x, Op op) {
     return __builtin_amdgcn_readlane(x, WAVE - 1);
 }
 
-// Entry p of that table, without a table (tiles null): found by every wave for
-// itself, a lane a sequence, for up to PACKED_FEW sequences.  How many tiles are
-// the i-th or later of their sequence falls with i: a search for the i where it
-// passes p.  (Also `pairs`.)
-DEVINL int4_t find_tile(const int* __restrict__ starts, int B, int T, int p, bool by_key,
+// Entry p of that table by query, found by every wave for itself, a lane a
+// sequence, for up to PACKED_FEW sequences.  How many tiles are the i-th or later
+// of their sequence falls with i: a search for the i where it passes p.  (Also
+// entry p by key, and `pairs`.)
+DEVINL int4_t find_tile(const int* __restrict__ starts, int B, int T, int p, int4_t& by_key,
                         float& pairs) {
     const int b = threadIdx.x & (WAVE - 1);
     int s = b > 0 && b < B + 2 ? starts[b - 1] : 0;
@@ -416,7 +416,8 @@ DEVINL int4_t find_tile(const int* __restrict__ starts, int B, int T, int p, boo
 #pragma unroll
     for (int off = 1; off < WAVE; off <<= 1) pairs += __shfl_xor(pairs, off, WAVE);
     const auto sum = [](int x, int y) { return x + y; };
-    if (wave_fold(n, sum) <= p) return int4_t{0, 0, 0, 0};
+    by_key = int4_t{0, 0, 0, 0};
+    if (wave_fold(n, sum) <= p) return by_key;
     int i = 0, past = wave_fold(n, [](int x, int y) { return max(x, y); });
     int before = 0;   // tiles that are the past-th or later
     while (past - i > 1) {
@@ -433,9 +434,14 @@ DEVINL int4_t find_tile(const int* __restrict__ starts, int B, int T, int p, boo
     const int seq = __ffsll(__ballot(n > i && rank == p - before)) - 1;
     s = __builtin_amdgcn_readlane(s, seq);
     e = __builtin_amdgcn_readlane(e, seq);
-    const int r0 = s + (by_key ? __builtin_amdgcn_readlane(n, seq) - 1 - i : i) * ROWS;
+    const int last = __builtin_amdgcn_readlane(n, seq) - 1;
     const bool real = !wrong && seq > 0 && seq <= B;
-    return int4_t{r0, min(r0 + ROWS, e), real ? s : r0, real ? e : wrong ? -1 : r0};
+    const auto tile = [&](int i) {
+        const int r0 = s + i * ROWS;
+        return int4_t{r0, min(r0 + ROWS, e), real ? s : r0, real ? e : wrong ? -1 : r0};
+    };
+    by_key = tile(last - i);
+    return tile(i);
 }
 
 // Which tile (or half tile) and head workgroup i of the forward and dq kernels
@@ -476,16 +482,26 @@ template <int D, int TEAMS, bool SAVE>
 __global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
 packed_attn_fwd_kernel(const PackedArgs a) {
     const int T = a.T, Hq = a.Hq, Hk = a.Hk;
-    const int4_t* tiles = (const int4_t*)a.tiles;
+    int4_t* tiles = (int4_t*)a.tiles;
     const Place place = place_of(blockIdx.x, Hq, Hk);
     const int hk = place.hk, h = place.h, at_tile = place.tile / TEAMS;
     if (at_tile >= a.max_tiles) return;
-    float pairs;
-    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile, false, pairs);
+    int4_t tile;
+    if (a.search) {
+        int4_t by_key;
+        float pairs;
+        tile = find_tile(a.starts, a.B, T, at_tile, by_key, pairs);
+        // the table for the backward pass
+        if (SAVE && h == 0 && place.tile % TEAMS == 0 && threadIdx.x == 0) {
+            tiles[at_tile] = tile;
+            tiles[a.max_tiles + at_tile] = by_key;
+            if (at_tile == 0) *(float*)(tiles + 2 * (long)a.max_tiles) = pairs;
+        }
+    } else {
+        tile = tiles[at_tile];
+    }
     const int row0 = tile[0] + place.tile % TEAMS * (ROWS / TEAMS);
     const int row1 = min(tile[1], row0 + ROWS / TEAMS), seq0 = tile[2], seq1 = tile[3];
-    if (SAVE && !tiles && blockIdx.x == 0)   // for the backward pass, which runs later
-        for (int i = threadIdx.x; i <= a.B; i += 256) a.kept_starts[i] = a.starts[i];
     if (row0 >= row1) return;
     const bool real = seq1 > seq0;
     const int kv0 = seq0, kv1 = real ? row1 : seq0;
@@ -645,8 +661,7 @@ packed_attn_dq_kernel(const PackedArgs a) {
         if (i < (unsigned)a.counters) a.counts[i] = 0;
     }
     if (at_tile >= a.max_tiles) return;
-    float pairs;
-    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile, false, pairs);
+    const int4_t tile = tiles[at_tile];
     const int row0 = tile[0] + place.tile % TEAMS * (ROWS / TEAMS);
     const int row1 = min(tile[1], row0 + ROWS / TEAMS), seq0 = tile[2], seq1 = tile[3];
     if (row0 >= row1) return;
@@ -840,8 +855,8 @@ template <int D, int KS, int QB, int NBUF>
 __global__ void __launch_bounds__(KS * 128, D == 128 ? 2 : 3)
 packed_attn_dkv_kernel(const PackedArgs a) {
     const int T = a.T, Hq = a.Hq, Hk = a.Hk;
-    const int4_t* tiles = a.tiles ? (const int4_t*)a.tiles + a.max_tiles : nullptr;
-    float pairs = tiles ? *(const float*)(tiles + a.max_tiles) : 0.f;
+    const int4_t* tiles = (const int4_t*)a.tiles + a.max_tiles;
+    const float pairs = *(const float*)(tiles + a.max_tiles);
     static_assert(QB == KS * 32 && QB == packed_keys(D), "as many queries as keys");
     constexpr int TEAMS = 2, BITS = 4 / KS, SLOTS = packed_slots(D), WORTH = D == 128 ? 8 : 16;
     const int hk = blockIdx.x % Hk;
@@ -851,7 +866,7 @@ packed_attn_dkv_kernel(const PackedArgs a) {
     const int part = a.parts - 1 - blockIdx.x / Hk / bits;
     const int bit = blockIdx.x / Hk % bits;
     const int at_tile = bit / BITS;
-    const int4_t tile = tiles ? tiles[at_tile] : find_tile(a.starts, a.B, T, at_tile, true, pairs);
+    const int4_t tile = tiles[at_tile];
     const int row0 = tile[0] + bit % BITS * (KS * 32);
     const int row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
     if (row0 >= row1) return;

@@ -118,18 +118,15 @@ PackedArgs packed_args(const Tensor& q, const Tensor& k, const Tensor& v, double
     return a;
 }
 
-// Where the tiles come from: a table or, for few sequences, just the starts.  The
-// table is a launch of 4 to 5 us; to search the starts makes each kernel 1 to 2 us
-// longer where workgroups follow one another (0.5 where all run at once, up to
-// about 512), so a forward pass alone searches, and three kernels share a table.
-// -> whether by a table
-bool plan_tiles(PackedArgs& a, long B, bool gradients) {
+// How many tiles there may be, and whether the forward kernel searches the starts
+// for them: that makes it 2 us longer, where the table is a launch of 4 to 5.
+void plan_tiles(PackedArgs& a, long B) {
     const long most = a.T / PACKED_ROWS + B + 2;
     // a launch's threads are counted in 32 bits
     TORCH_CHECK(most * a.Hq * 512 < (1L << 32), "too many rows and sequences for one call");
     a.B = (int)B;
     a.max_tiles = (int)most;
-    return B > PACKED_FEW || (gradients && most * a.Hq > 512);
+    a.search = B <= PACKED_FEW;
 }
 
 // In how many parts the kernel for dk and dv may take a workgroup's queries.  It
@@ -154,8 +151,8 @@ void plan_parts(PackedArgs& a, bool keys) {
 struct Kept {
     Parts parts;
     size_t tiles, rest = 0, lse = 0;
-    Kept(const PackedArgs& a, bool table, bool save)
-        : tiles(parts.add(table ? 32 * (size_t)a.max_tiles + 16 : save ? 4 * ((size_t)a.B + 1) : 0)) {
+    Kept(const PackedArgs& a, bool save)
+        : tiles(parts.add(save || !a.search ? 32 * (size_t)a.max_tiles + 16 : 0)) {
         if (!save) return;
         rest = parts.add(2 * (size_t)a.T * a.Hq * a.D);
         lse = parts.add(4 * (size_t)a.T * a.Hq);
@@ -171,21 +168,22 @@ std::vector<Tensor> packed_attn_fwd(const Tensor& q, const Tensor& k, const Tens
                 "seq_starts must be a dense int32 vector on the device of q");
     const c10::cuda::CUDAGuard guard(q.device());
     const Tensor out = torch::empty({a.T, a.Hq, a.D}, q.options());
-    const bool table = plan_tiles(a, starts.numel() - 1, save);
-    const Kept at(a, table, save);
+    plan_tiles(a, starts.numel() - 1);
+    const Kept at(a, save);
     Tensor kept;
-    if (at.parts.size) kept = at.parts.make(q);
+    if (at.parts.size) {
+        kept = at.parts.make(q);
+        a.tiles = part<void>(kept, at.tiles);
+    }
     a.starts = starts.data_ptr<int>();
     a.out = bf16(out);
-    if (table) a.tiles = part<void>(kept, at.tiles);
     if (save) {
         a.out_lo = part<unsigned short>(kept, at.rest);
         a.lse = part<float>(kept, at.lse);
-        if (!table) a.kept_starts = part<int>(kept, at.tiles);
     }
     if (a.T > 0) {
         void* st = stream_of(q);
-        if (table) launched(launch_packed_tiles(&a, st), "packed_attention");
+        if (!a.search) launched(launch_packed_tiles(&a, st), "packed_attention");
         launched(launch_packed_attn_fwd(&a, st), "packed_attention");
     }
     return {out, kept};
@@ -207,7 +205,7 @@ std::vector<Tensor> packed_attn_bwd(const Tensor& dout, const Tensor& q, const T
         dv = torch::empty({a.T, a.Hk, a.D}, opt);
     }
     if (a.T > 0) {
-        const bool table = plan_tiles(a, B, true);
+        plan_tiles(a, B);
         Parts parts;
         const size_t delta = parts.add(4 * (size_t)a.Hq * a.T);
         plan_parts(a, keys);
@@ -215,9 +213,8 @@ std::vector<Tensor> packed_attn_bwd(const Tensor& dout, const Tensor& q, const T
         const size_t sums = parts.add(a.parts > 1 ? 8 * (size_t)a.counters * a.parts *
                                                         packed_keys(a.D) * a.D : 0);
         const Tensor scratch = parts.make(q);
-        const Kept at(a, table, true);
-        if (table) a.tiles = part<void>(kept, at.tiles);
-        else a.starts = part<int>(kept, at.tiles);
+        const Kept at(a, true);
+        a.tiles = part<void>(kept, at.tiles);
         a.out = bf16(out);
         a.out_lo = part<unsigned short>(kept, at.rest);
         a.lse = part<float>(kept, at.lse);
