@@ -100,42 +100,51 @@ DEVINL unsigned turn(unsigned row) {
 // Where a lane's parts of a tile begin.  `turn` and the position in a row only
 // meet in exclusive-ors, so all fragments are one exclusive-or with a constant
 // away from one address for each kind of read: `rows` for a fragment of rows,
-// `cols` for one of the transpose.  The kernels make these anew every step
-// (`fresh`), or the compiler would keep each fragment's address in a register.
-template <int D>
+// `cols` for one of the transpose.  Where registers allow (KEPT), each of these is
+// kept, and which tile is meant goes into the reads' constant offsets; else they
+// are made anew from two every step (`fresh`), or the compiler would keep them.
+// (8192 rows forward: 539 us kept, 551 made anew; dq of 8192 packed: 309, 313.)
+template <int D, bool KEPT>
 struct Lane {
-    unsigned rows, cols;
+    static constexpr int N = KEPT ? D / 16 : 1;
+    unsigned rows[N], cols[N];
     DEVINL explicit Lane(int lane) {
-        const unsigned r = lane & 31, hi = lane >> 5, i = lane & 15;
-        rows = r * (D * 2) + ((hi ^ turn<D>(r)) << 4);
-        const unsigned c = 4 * hi + (i >> 2);
-        cols = c * (D * 2) + (((2 * ((lane >> 4) & 1) + ((i >> 1) & 1)) ^ turn<D>(c)) << 4) +
-               8 * (i & 1);
+        const unsigned r = lane & 31, hi = lane >> 5, i = lane & 15, c = 4 * hi + (i >> 2);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            rows[n] = (r * (D * 2) + ((hi ^ turn<D>(r)) << 4)) ^ (n << 5);
+            cols[n] = (c * (D * 2) + 8 * (i & 1) +
+                       (((2 * ((lane >> 4) & 1) + ((i >> 1) & 1)) ^ turn<D>(c)) << 4)) ^ (n << 5);
+            if (KEPT) asm volatile("" : "+v"(rows[n]), "+v"(cols[n]));
+        }
     }
     DEVINL Lane fresh(unsigned tile) const {
         Lane l = *this;
-        l.rows += tile;
-        l.cols += tile;
-        asm volatile("" : "+v"(l.rows), "+v"(l.cols));
+        if (!KEPT) {
+            l.rows[0] += tile;
+            l.cols[0] += tile;
+            asm volatile("" : "+v"(l.rows[0]), "+v"(l.cols[0]));
+        }
         return l;
     }
+    DEVINL unsigned row(int n) const { return KEPT ? rows[n % N] : rows[0] ^ (n << 5); }
+    DEVINL unsigned col(int n) const { return KEPT ? cols[n % N] : cols[0] ^ (n << 5); }
 };
 
 // A fragment of 32 rows from `tile`, columns 16 s..16 s+15
-template <int D>
-DEVINL bf16x8_t rows_frag(const char* tile, const Lane<D>& l, int s) {
-    return *reinterpret_cast<const bf16x8_t*>(tile + (l.rows ^ (s << 5)));
+template <typename L>
+DEVINL bf16x8_t rows_frag(const char* tile, const L& l, int s) {
+    return *reinterpret_cast<const bf16x8_t*>(tile + l.row(s));
 }
 
 // A fragment of the transpose: columns 32 db..32 db+31 as its rows, and the
 // rows k' (as above, slice 0) from `tile` as its columns
-template <int D>
-DEVINL bf16x8_t cols_frag(char* tile, const Lane<D>& l, int db) {
+template <int D, typename L>
+DEVINL bf16x8_t cols_frag(char* tile, const L& l, int db) {
     union { short4_t h[2]; bf16x8_t v; } u;
-    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_short4_t*)(tile + (l.cols ^ (db << 6))));
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)(tile + l.col(2 * db)));
     u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(   // 8 rows on
-        (lds_short4_t*)(tile + (l.cols ^ (db << 6) ^ 32) + 16 * D));
+        (lds_short4_t*)(tile + l.col(2 * db + 1) + 16 * D));
     return u.v;
 }
 
@@ -296,7 +305,8 @@ DEVINL void store_row(const f32x16_t (&acc)[D / 32], float factor, ushort_t* row
 // run first and the short ones fill the gaps; entries that are left over hold
 // no rows.  One workgroup, a wave a sequence and a lane a tile: a pass that
 // counts tiles by their number in the sequence, a scan (with `pairs`, how often
-// a tile of queries meets one of keys), a pass that places them.  (The order within one count is free and changes no result.)
+// a tile of queries meets one of keys), a pass that places them.  (The order
+// within one count is free and changes no result.)
 #define BUCKETS 4096
 #define BUILDERS 1024
 
@@ -520,7 +530,7 @@ packed_attn_fwd_kernel(const PackedArgs a) {
     // two tiles of keys, two of values
     constexpr int TILE = 64 * D * 2;
     __shared__ __attribute__((aligned(256))) char lds[4 * TILE];
-    const Lane<D> lanes(lane);
+    const Lane<D, true> lanes(lane);
 
     bf16x8_t qf[D / 16];
     load_row<D>(qf, a.q + row * a.qt + h * a.qh, mine, hi);
@@ -543,7 +553,7 @@ packed_attn_fwd_kernel(const PackedArgs a) {
     arrived();
     __syncthreads();
     const int wave_end = min(wrow + 32, row1);   // keys this wave's rows reach
-    for (int it = 0; it < steps; ++it) {
+    auto step = [&](auto buf, int it) {
         // into the tiles that were last read before the barrier of the step before
         if (it + 1 < steps) fetch(it + 1);
 #pragma unroll
@@ -551,11 +561,11 @@ packed_attn_fwd_kernel(const PackedArgs a) {
             const int key0 = kv0 + it * 64 + sub * 32;
             if (key0 >= wave_end || (TEAMS > 1 && sub != team)) continue;
             // a product each: N fragments of K, then N of V^T
-            const Lane<D> at = lanes.fresh((it & 1) * TILE + sub * (TILE / 2));
+            char* const tile = lds + buf * TILE + sub * (TILE / 2);
             auto fragment = [&](int i) {
-                return i < N ? rows_frag<D>(lds, at, i)
-                             : cols_frag<D>(lds + 2 * TILE + (i - N) / (D / 32) * (TILE / 4), at,
-                                            (i - N) % (D / 32));
+                return i < N ? rows_frag(tile, lanes, i)
+                             : cols_frag<D>(tile + 2 * TILE + (i - N) / (D / 32) * (TILE / 4),
+                                            lanes, (i - N) % (D / 32));
             };
             bf16x8_t f[AHEAD];
             auto next = [&](int i) {
@@ -616,6 +626,10 @@ packed_attn_fwd_kernel(const PackedArgs a) {
         }
         arrived();
         __syncthreads();
+    };
+    for (int it = 0; it < steps; it += 2) {
+        step(std::integral_constant<int, 0>{}, it);
+        if (it + 1 < steps) step(std::integral_constant<int, 1>{}, it + 1);
     }
     if (TEAMS > 1) {
         // the second team's rows to the first
@@ -681,7 +695,8 @@ packed_attn_dq_kernel(const PackedArgs a) {
     constexpr int N = D / 16, AHEAD = D == 128 ? 4 : 1;   // products of a kind, fragments read ahead
     constexpr int TILE = 64 * D * 2;
     __shared__ __attribute__((aligned(256))) char lds[4 * TILE];
-    const Lane<D> lanes(lane);
+    constexpr bool KEPT = D == 128;
+    const Lane<D, KEPT> lanes(lane);
 
     const ushort_t *k = a.k + hk * a.kh, *v = a.v + hk * a.vh;
     const Mover<D, 64, 256> mk(a.kt), mv(a.vt);
@@ -721,20 +736,28 @@ packed_attn_dq_kernel(const PackedArgs a) {
     // COUNT fragments of each block read in all.
     auto sweep = [&](auto count, auto use) {
         constexpr int COUNT = decltype(count)::value;
+        // dP is summed onto -delta, for which D 64 has no 16 registers to spare
+        constexpr bool LESS = D == 128 && COUNT == 3 * N;
+        f32x16_t less;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) less[r] = -dl;
+        if (LESS) asm volatile("" : "+v"(less));   // once, not every block
         arrived();   // the first tiles
         __syncthreads();
-        for (int it = 0; it < steps; ++it) {
+        auto step = [&](auto buf, int it) {
             if (it + 1 < steps) fetch(it + 1);
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
                 const int key0 = kv0 + it * 64 + sub * 32;
                 if (key0 >= wave_end || (TEAMS > 1 && sub != team)) continue;
                 // a product each: N fragments of K, N of V, N of K^T for `use`
-                const Lane<D> at = lanes.fresh((it & 1) * TILE + sub * (TILE / 2));
+                const int off = buf * TILE + sub * (TILE / 2);
+                const Lane<D, KEPT> at = lanes.fresh(off);
+                char* const tile = KEPT ? lds + off : lds;
                 auto fragment = [&](int i) {
-                    return i < N       ? rows_frag<D>(lds, at, i)
-                           : i < 2 * N ? rows_frag<D>(lds + 2 * TILE, at, i - N)
-                                       : cols_frag<D>(lds + (i - 2 * N) / (D / 32) * (TILE / 4),
+                    return i < N       ? rows_frag(tile, at, i)
+                           : i < 2 * N ? rows_frag(tile + 2 * TILE, at, i - N)
+                                       : cols_frag<D>(tile + (i - 2 * N) / (D / 32) * (TILE / 4),
                                                       at, (i - 2 * N) % (D / 32));
                 };
                 bf16x8_t f[AHEAD];
@@ -745,7 +768,7 @@ packed_attn_dq_kernel(const PackedArgs a) {
 #pragma unroll
                 for (int i = 0; i < AHEAD; ++i) f[i] = fragment(i);
                 in_order<D>();
-                f32x16_t s = zero16(), dp = zero16();
+                f32x16_t s = zero16(), dp = LESS ? less : zero16();
                 auto weigh = [&](int r) {
                     s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, -ls));
                 };
@@ -776,6 +799,14 @@ packed_attn_dq_kernel(const PackedArgs a) {
             }
             arrived();
             __syncthreads();
+        };
+        for (int it = 0; it < steps; it += KEPT ? 2 : 1) {
+            if (KEPT) {
+                step(std::integral_constant<int, 0>{}, it);
+                if (it + 1 < steps) step(std::integral_constant<int, 1>{}, it + 1);
+            } else {
+                step(it & 1, it);
+            }
         }
     };
     float* join = reinterpret_cast<float*>(lds) + wid % SETS * (D / 2) * 64 + lane;
@@ -800,7 +831,7 @@ packed_attn_dq_kernel(const PackedArgs a) {
     if (mine && hi == 0 && team == 0) a.delta[(long)h * T + row] = -dl;
     sweep(std::integral_constant<int, 3 * N>{}, [&](f32x16_t& p, f32x16_t& dp, auto& f, auto& next) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) p[r] *= dp[r] - dl;
+        for (int r = 0; r < 8; ++r) p[r] *= D == 128 ? dp[r] : dp[r] - dl;
         bf16x8_t df = pack8(p, 0);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -809,7 +840,7 @@ packed_attn_dq_kernel(const PackedArgs a) {
             if (i < N / 2)
 #pragma unroll
                 for (int r = 8 + i * (16 / N); r < 8 + (i + 1) * (16 / N); ++r)
-                    p[r] *= dp[r] - dl;
+                    p[r] *= D == 128 ? dp[r] : dp[r] - dl;
             next(2 * N + i);
         }
     });
@@ -901,7 +932,7 @@ packed_attn_dkv_kernel(const PackedArgs a) {
     __shared__ Lds lds;
     char* const ql = lds.x;
     char* const ol = lds.x + NBUF * TILE;
-    const Lane<D> lanes(lane);
+    const Lane<D, false> lanes(lane);
 
     bf16x8_t kf[D / 16], vf[D / 16];
     f32x16_t ak[D / 32], av[D / 32];
@@ -963,11 +994,11 @@ packed_attn_dkv_kernel(const PackedArgs a) {
             const int first = now + in;
             // queries all before the wave's keys, or past the sequence
             if (first + 31 < wkey || first >= seq1) continue;
-            const Lane<D> at = lanes.fresh(buf * TILE + in * (D * 2));
+            const Lane<D, false> at = lanes.fresh(buf * TILE + in * (D * 2));
             f32x16_t s = zero16(), dp;
 #pragma unroll
             for (int d = 0; d < D / 16; ++d)
-                s = mfma(rows_frag<D>(ql, at, d), kf[d], s);
+                s = mfma(rows_frag(ql, at, d), kf[d], s);
             // dP - delta, summed onto the deltas
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -978,7 +1009,7 @@ packed_attn_dkv_kernel(const PackedArgs a) {
             }
 #pragma unroll
             for (int d = 0; d < D / 16; ++d)
-                dp = mfma(rows_frag<D>(ol, at, d), vf[d], dp);
+                dp = mfma(rows_frag(ol, at, d), vf[d], dp);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const float4_t ls = *reinterpret_cast<const float4_t*>(
