@@ -14,7 +14,7 @@
 //
 // 4096 x 128256 bf16: forward 0.20 ms (5.2 TB/s), gradient 0.37 ms (5.7 TB/s);
 // 32768 x 4096 with three of ten rows labelled: 19.5 us (the labelled rows' 81 MB
-// at 4.1 TB/s) and 50 us (81 MB read, 268 written: 7.0 TB/s, as the rows were in
+// at 4.1 TB/s) and 52 us (81 MB read, 268 written: 6.7 TB/s, as the rows were in
 // cache).  Where rows have no labels the gradient's zeros are most of the work.
 //
 // m and l are kept apart, not as one log-sum: x - m is nearly exact, while a
