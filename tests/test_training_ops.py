@@ -585,9 +585,10 @@ def test_loss_of_no_rows_and_of_one_row_repeated(reduction, device):
 
 
 @gpu
-def test_ops_gpu_from_two_threads():
+@pytest.mark.parametrize("lens", [[300, 40], [1500, 40, 700]])
+def test_ops_gpu_from_two_threads(lens):
     """Each on a stream of its own, forward and backward."""
-    lens, steps = [300, 40], 20
+    steps = 20
     starts = torch.tensor(_starts(lens), dtype=torch.int32, device="cuda")
     data = [_inputs(lens, (4, 2), 64, seed=i, device="cuda") for i in range(2)]
     logits = [_loss_inputs(50, 9001, torch.bfloat16, "cuda", seed=i) for i in range(2)]
