@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <optional>
 #include <tuple>
 #include <vector>
 
@@ -257,8 +258,37 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     }
 };
 
-Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v,
-                        const Tensor& starts, double scale) {
+// The starts as the kernels take them.  No other value's low 32 bits.
+Tensor starts32(const Tensor& starts, const Tensor& q) {
+    Tensor s = starts;
+    if (s.scalar_type() != torch::kInt32) s = s.clamp(-1, (1L << 31) - 1).to(torch::kInt32);
+    if (s.device() != q.device()) s = s.to(q.device());
+    return s.contiguous();
+}
+
+Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& starts0,
+                        std::optional<double> scale0) {
+    TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && v.dim() == 3,
+                      "q, k and v must be [tokens, heads, head dim]");
+    TORCH_CHECK_VALUE(k.sizes() == v.sizes() && q.size(0) == k.size(0) && q.size(2) == k.size(2),
+                      "shapes do not fit: q ", q.sizes(), ", k ", k.sizes(), ", v ", v.sizes());
+    TORCH_CHECK_VALUE(q.size(1) > 0 && k.size(1) > 0 && q.size(1) % k.size(1) == 0, q.size(1),
+                      " query heads are no multiple of ", k.size(1), " key/value heads");
+    TORCH_CHECK_VALUE(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type() &&
+                          q.device() == k.device() && q.device() == v.device(),
+                      "q, k and v must have one type and device");
+    const auto kind = starts0.scalar_type();
+    TORCH_CHECK_VALUE(starts0.dim() == 1 && starts0.numel() >= 1 &&
+                          (kind == torch::kInt32 || kind == torch::kInt64),
+                      "seq_starts must be a vector of whole numbers, one more than sequences");
+    TORCH_CHECK_VALUE(q.scalar_type() == torch::kBFloat16,
+                      "on the GPU q, k and v must be bfloat16, not ", q.scalar_type());
+    TORCH_CHECK_VALUE(q.size(2) == 64 || q.size(2) == 128,
+                      "on the GPU the head dim must be 64 or 128, not ", q.size(2));
+    const double scale = scale0 ? *scale0 : 1.0 / std::sqrt((double)q.size(2));
+    TORCH_CHECK_VALUE(scale > 0.0 && scale < 0x1p127,
+                      "scale must be positive and an fp32 number, not ", scale);
+    const Tensor starts = starts32(starts0, q);
     if (torch::GradMode::is_enabled() &&
         (q.requires_grad() || k.requires_grad() || v.requires_grad()))
         return PackedAttention::apply(q, k, v, starts, scale);
@@ -376,7 +406,19 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
     }
 };
 
-Tensor cross_entropy(const Tensor& x, const Tensor& targets, int64_t ignore, int64_t mode) {
+Tensor cross_entropy(const Tensor& x0, const Tensor& targets0, int64_t ignore, int64_t mode) {
+    TORCH_CHECK_VALUE(x0.dim() == 2 && x0.size(1) >= 1 && targets0.dim() == 1 &&
+                          targets0.size(0) == x0.size(0),
+                      "logits must be [rows, vocabulary] with one label a row: logits ",
+                      x0.sizes(), ", targets ", targets0.sizes());
+    const auto type = targets0.scalar_type();
+    TORCH_CHECK_VALUE(type == torch::kInt32 || type == torch::kInt64,
+                      "targets must be whole numbers, not ", type);
+    TORCH_CHECK_VALUE(targets0.device() == x0.device(),
+                      "logits and targets must be on one device");
+    kind_of(x0, "on the GPU logits");
+    const Tensor targets = targets0.to(torch::kInt64).contiguous();
+    const Tensor x = x0.stride(1) == 1 ? x0 : x0.contiguous();
     if (torch::GradMode::is_enabled() && x.requires_grad())
         return CrossEntropy::apply(x, targets, ignore, mode);
     return xent_fwd(x, targets, ignore, mode, false)[0];

@@ -2,7 +2,8 @@
 
 On the GPU the kernels of csrc/packed_attn.hip, cross_entropy.hip and
 grad_norm.hip, whose autograd nodes are in csrc/training.cpp; on the CPU the
-references of reference.py. Arguments are checked here for both.
+references of reference.py. Arguments are checked here or, where all are on the
+GPU, by the same rules in training.cpp (a short call is mostly host time).
 """
 from __future__ import annotations
 
@@ -38,6 +39,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     sequence (a shut place's product is 0 times the value), but no other's.
 
     The training counterpart of prefill_attention, which has no gradients."""
+    if q.is_cuda and seq_starts.is_cuda:
+        return _get_ext().packed_attention(q, k, v, seq_starts, scale)
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k and v must be [tokens, heads, head dim]")
     if k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
@@ -62,16 +65,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             raise ValueError(f"seq_starts must rise within 0 and {q.shape[0]}")
     if not q.is_cuda:
         return reference.packed_attention(q, k, v, seq_starts, scale)
-    if q.dtype != torch.bfloat16:
-        raise ValueError(f"on the GPU q, k and v must be bfloat16, not {q.dtype}")
-    if q.shape[2] not in (64, 128):
-        raise ValueError(f"on the GPU the head dim must be 64 or 128, not {q.shape[2]}")
-    starts = seq_starts
-    if starts.dtype != torch.int32:
-        starts = starts.clamp(-1, 2 ** 31 - 1).to(torch.int32)   # no other value's low bits
-    if starts.device != q.device or not starts.is_contiguous():
-        starts = starts.to(q.device).contiguous()
-    return _get_ext().packed_attention(q, k, v, starts, scale)
+    return _get_ext().packed_attention(q, k, v, seq_starts.to(q.device), scale)
 
 
 # ------------------------------------------------------------- cross-entropy
@@ -92,6 +86,10 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int
 
     On the GPU: float32, bfloat16 or float16 logits, in rows of any distance
     and alignment; the sums are fp32 and over rows fp64."""
+    if reduction not in _MODES:
+        raise ValueError(f"reduction must be one of {sorted(_MODES)}, not {reduction!r}")
+    if logits.is_cuda:
+        return _get_ext().cross_entropy(logits, targets, ignore_index, _MODES[reduction])
     if logits.dim() != 2 or logits.shape[1] < 1 or targets.shape != logits.shape[:1]:
         raise ValueError(f"logits must be [rows, vocabulary] with one label a row: logits "
                          f"{tuple(logits.shape)}, targets {tuple(targets.shape)}")
@@ -99,18 +97,7 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int
         raise ValueError(f"targets must be whole numbers, not {targets.dtype}")
     if targets.device != logits.device:
         raise ValueError("logits and targets must be on one device")
-    if reduction not in _MODES:
-        raise ValueError(f"reduction must be one of {sorted(_MODES)}, not {reduction!r}")
-    if targets.dtype != torch.int64 or not targets.is_contiguous():
-        targets = targets.long().contiguous()
-    if not logits.is_cuda:
-        return reference.cross_entropy(logits, targets, ignore_index, reduction)
-    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        raise ValueError(f"on the GPU logits must be float32, bfloat16 or float16, "
-                         f"not {logits.dtype}")
-    if logits.stride(1) != 1:
-        logits = logits.contiguous()
-    return _get_ext().cross_entropy(logits, targets, ignore_index, _MODES[reduction])
+    return reference.cross_entropy(logits, targets.long(), ignore_index, reduction)
 
 
 # ------------------------------------------------------------- gradient norm
