@@ -514,8 +514,16 @@ Tensor sums_of(const Grads& g, const Tensor& like, void* st) {
     return sums;
 }
 
-Tensor grad_norm(std::vector<Tensor> grads) {
-    TORCH_CHECK(!grads.empty(), "no gradients");
+std::vector<Tensor> grads_of(const std::vector<Tensor>& parameters) {
+    std::vector<Tensor> grads;
+    for (const Tensor& p : parameters)
+        if (p.grad().defined()) grads.push_back(p.grad());
+    return grads;
+}
+
+Tensor grad_norm(const std::vector<Tensor>& parameters) {
+    const std::vector<Tensor> grads = grads_of(parameters);
+    if (grads.empty()) return torch::zeros({});
     const at::NoGradGuard no_grad;
     const Grads g = collect(grads, false);
     const c10::cuda::CUDAGuard guard(grads[0].device());
@@ -527,8 +535,9 @@ Tensor grad_norm(std::vector<Tensor> grads) {
     return norm;
 }
 
-Tensor grad_clip(std::vector<Tensor> grads, double limit, double eps) {
-    TORCH_CHECK(!grads.empty(), "no gradients");
+Tensor grad_clip(const std::vector<Tensor>& parameters, double limit, double eps) {
+    const std::vector<Tensor> grads = grads_of(parameters);
+    if (grads.empty()) return torch::zeros({});
     const at::NoGradGuard no_grad;
     const Grads g = collect(grads, true);
     const c10::cuda::CUDAGuard guard(grads[0].device());

@@ -105,10 +105,8 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int
 _EPS = 1e-6   # in the divisor, so that a norm of zero divides
 
 
-def _grads(parameters) -> list[torch.Tensor]:
-    if isinstance(parameters, torch.Tensor):
-        parameters = (parameters,)
-    return [g for g in [p.grad for p in parameters] if g is not None]
+def _list(parameters) -> list[torch.Tensor]:
+    return [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
 
 
 def _check_host(grads: list[torch.Tensor], write: bool = False) -> None:
@@ -132,11 +130,12 @@ def _check_host(grads: list[torch.Tensor], write: bool = False) -> None:
 def grad_norm(parameters) -> torch.Tensor:
     """2-norm of all parameters' gradients together (fp32 scalar on their
     device); parameters without a gradient are passed over."""
-    grads = _grads(parameters)
+    parameters = _list(parameters)
+    if parameters and parameters[0].is_cuda:
+        return _get_ext().grad_norm(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.zeros(())
-    if grads[0].is_cuda:
-        return _get_ext().grad_norm(grads)
     _check_host(grads)
     with torch.no_grad():
         return reference.grad_norm(grads)
@@ -157,18 +156,17 @@ def clip_grad_norm_(parameters, max_norm: float,
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative: {max_norm}")
+    parameters = _list(parameters)
     if error_if_nonfinite:
-        parameters = ([parameters] if isinstance(parameters, torch.Tensor)
-                      else list(parameters))
         norm = grad_norm(parameters)
         if not torch.isfinite(norm):
             raise RuntimeError(f"the norm of the gradients is {float(norm)}; "
                                "they are left as they were")
-    grads = _grads(parameters)
+    if parameters and parameters[0].is_cuda:
+        return _get_ext().grad_clip(parameters, max_norm, _EPS)
+    grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.zeros(())
-    if grads[0].is_cuda:
-        return _get_ext().grad_clip(grads, max_norm, _EPS)
     _check_host(grads, write=True)
     with torch.no_grad():
         return reference.grad_clip(grads, max_norm, _EPS)
