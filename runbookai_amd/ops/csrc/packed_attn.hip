@@ -898,7 +898,11 @@ packed_attn_dkv_kernel(const PackedArgs a) {
     const int bit = blockIdx.x / Hk % bits;
     const int at_tile = bit / BITS;
     const int4_t tile = tiles[at_tile];
-    const int row0 = tile[0] + bit % BITS * (KS * 32);
+    // The first half of a tile is seen by more queries, and the second may be
+    // empty.  Workgroups go round the XCDs, and round the engines of one, in a
+    // fixed order: which half comes first changes from tile to tile so that no
+    // period of two, four or eight workgroups has all of a kind.
+    const int row0 = tile[0] + (bit + (BITS > 1 ? __popc(at_tile) : 0)) % BITS * (KS * 32);
     const int row1 = tile[1], seq0 = tile[2], seq1 = tile[3];
     if (row0 >= row1) return;
     const bool real = seq1 > seq0;
