@@ -37,9 +37,17 @@ HIP_FLAGS = ["-O3", "-std=c++17",
 
 
 def build(verbose: bool = False):
-    """Compile (or reuse) the extension; returns the imported module."""
+    """Compile the extension; returns the imported module.
+
+    Everything is compiled, whatever an earlier build left: the build tool does
+    not know which headers a kernel includes, so a kernel whose argument struct
+    changed in a header would keep its old object and read the new struct by the
+    old one's layout."""
     os.environ.setdefault("PYTORCH_ROCM_ARCH", "gfx950")
     os.makedirs(BUILD_DIR, exist_ok=True)
+    for fn in os.listdir(BUILD_DIR):
+        if fn.endswith((".o", ".so")):
+            os.remove(os.path.join(BUILD_DIR, fn))
     from torch.utils.cpp_extension import load
 
     module = load(
