@@ -45,6 +45,15 @@ void launched(int code, const char* what) {
     TORCH_CHECK(code == 0, what, ": the launch failed with HIP error ", code);
 }
 
+// The kernels take a tensor's memory.  One that only stands for memory (a fake
+// one, a wrapper, freed storage) would lead them to address 0.
+void plain(const Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(t.layout() == torch::kStrided &&
+                          !t.key_set().has(c10::DispatchKey::Python) && t.has_storage() &&
+                          (t.numel() == 0 || t.const_data_ptr()),
+                      name, " must be a plain tensor with memory of its own");
+}
+
 // What a backward pass returns: without a gradient of its own, and with an
 // error where somebody asks for one (create_graph).
 std::vector<Tensor> once(std::vector<Tensor> grads, const char* what) {
@@ -195,6 +204,7 @@ std::vector<Tensor> packed_attn_bwd(const Tensor& dout, const Tensor& q, const T
                                     const Tensor& v, const Tensor& out, const Tensor& kept,
                                     long B, double scale, bool keys) {
     PackedArgs a = packed_args(q, k, v, scale);
+    plain(dout, "the gradient");
     check_rows(dout, "the gradient", q);
     TORCH_CHECK(dout.sizes() == q.sizes(), "the gradient must have the shape of q");
     const c10::cuda::CUDAGuard guard(q.device());
@@ -285,6 +295,10 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
                       "on the GPU q, k and v must be bfloat16, not ", q.scalar_type());
     TORCH_CHECK_VALUE(q.size(2) == 64 || q.size(2) == 128,
                       "on the GPU the head dim must be 64 or 128, not ", q.size(2));
+    plain(q, "q");
+    plain(k, "k");
+    plain(v, "v");
+    plain(starts0, "seq_starts");
     const double scale = scale0 ? *scale0 : 1.0 / std::sqrt((double)q.size(2));
     TORCH_CHECK_VALUE(scale > 0.0 && scale < 0x1p127,
                       "scale must be positive and an fp32 number, not ", scale);
@@ -364,6 +378,7 @@ Tensor xent_bwd(const Tensor& gout, Tensor x, const Tensor& targets, int64_t ign
     check_logits(x, targets);
     const int kind = kind_of(x, "logits");
     const int N = (int)x.size(0), V = (int)x.size(1);
+    plain(gout, "the gradient");
     TORCH_CHECK(gout.device() == x.device() && gout.scalar_type() == torch::kFloat32 &&
                     (gout.dim() == 0 || (gout.dim() == 1 && gout.numel() == N)),
                 "the gradient must be float32, one value or one a row");
@@ -417,6 +432,8 @@ Tensor cross_entropy(const Tensor& x0, const Tensor& targets0, int64_t ignore, i
     TORCH_CHECK_VALUE(targets0.device() == x0.device(),
                       "logits and targets must be on one device");
     kind_of(x0, "on the GPU logits");
+    plain(x0, "logits");
+    plain(targets0, "targets");
     const Tensor targets = targets0.to(torch::kInt64).contiguous();
     const Tensor x = x0.stride(1) == 1 ? x0 : x0.contiguous();
     if (torch::GradMode::is_enabled() && x.requires_grad())
@@ -458,6 +475,7 @@ Grads collect(const std::vector<Tensor>& grads, bool write) {
                               t.device() == grads[0].device(),
                           "gradients must be dense and on one device");
         kind_of(t, "gradients");
+        plain(t, "a gradient");
         if (t.numel() == 0) continue;
         Tensor d = t;
         if (!t.is_non_overlapping_and_dense()) {

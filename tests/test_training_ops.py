@@ -1025,3 +1025,40 @@ def test_packed_model_gpu():
     norm = ops.clip_grad_norm_(model.parameters(), 0.5, error_if_nonfinite=True)
     assert float(norm) > 0
     assert float(ops.grad_norm(model.parameters())) <= 0.5 * (1 + 1e-5)
+
+
+# ------------------------------------------- tensors that are more than memory
+
+def test_ops_refuse_tensors_without_memory():
+    """Fake tensors have a shape and a device and no memory behind them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        q = torch.empty(4, 2, 64, dtype=torch.bfloat16, device="cuda")
+        starts = torch.empty(2, dtype=torch.int32, device="cuda")
+        logits = torch.empty(4, 9, device="cuda")
+        targets = torch.empty(4, dtype=torch.int64, device="cuda")
+        p = torch.nn.Parameter(torch.empty(5, device="cuda"))
+        p.grad = torch.empty(5, device="cuda")
+        for call in (lambda: ops.packed_attention(q, q, q, starts),
+                     lambda: ops.packed_attention(q.requires_grad_(), q, q, starts),
+                     lambda: ops.cross_entropy(logits, targets),
+                     lambda: ops.grad_norm([p]), lambda: ops.clip_grad_norm_([p], 1.0)):
+            with pytest.raises(ValueError, match="plain tensor"):
+                call()
+
+
+@gpu
+def test_ops_gpu_refuse_freed_memory():
+    """A parameter whose storage was let go until it is needed again."""
+    q, k, v, _ = _inputs([4], (4, 2), 64, device="cuda")
+    starts = torch.tensor([0, 4], device="cuda")
+    k.untyped_storage().resize_(0)
+    with pytest.raises(ValueError, match="plain tensor"):
+        ops.packed_attention(q, k, v, starts)
+    p = torch.nn.Parameter(torch.zeros(5, device="cuda"))
+    p.grad = torch.ones(5, device="cuda")
+    p.grad.untyped_storage().resize_(0)
+    for call in (lambda: ops.grad_norm([p]), lambda: ops.clip_grad_norm_([p], 1.0)):
+        with pytest.raises(ValueError, match="plain tensor"):
+            call()
