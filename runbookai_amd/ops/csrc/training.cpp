@@ -45,9 +45,13 @@ void launched(int code, const char* what) {
     TORCH_CHECK(code == 0, what, ": the launch failed with HIP error ", code);
 }
 
-// The kernels take a tensor's memory.  One that only stands for memory (a fake
-// one, a wrapper, freed storage) would lead them to address 0.
+// The kernels take a tensor's memory.  A tangent that it has beside it would be
+// lost without a word, and one that only stands for memory (a fake one, a wrapper,
+// freed storage) would lead them to address 0.
 void plain(const Tensor& t, const char* name) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name,
+                                " has a forward-mode derivative, which the training ops do not "
+                                "have on the GPU");
     TORCH_CHECK_VALUE(t.layout() == torch::kStrided &&
                           !t.key_set().has(c10::DispatchKey::Python) && t.has_storage() &&
                           (t.numel() == 0 || t.const_data_ptr()),

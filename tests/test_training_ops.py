@@ -1062,3 +1062,45 @@ def test_ops_gpu_refuse_freed_memory():
     for call in (lambda: ops.grad_norm([p]), lambda: ops.clip_grad_norm_([p], 1.0)):
         with pytest.raises(ValueError, match="plain tensor"):
             call()
+
+
+def _tangents(device):
+    """Outputs' tangents for tangents of one input each, and of a gradient."""
+    import torch.autograd.forward_ad as fwd
+
+    dtype = torch.bfloat16 if device == "cuda" else torch.float64
+    q, k, v, dout = _inputs([7, 2], (2, 1), 64, device=device, dtype=dtype)
+    starts = torch.tensor([0, 7, 9], device=device)
+    x, t = _loss_inputs(4, 9, torch.float32, device)
+    way = torch.ones_like
+    with fwd.dual_level():
+        def tangent(call):
+            return lambda: fwd.unpack_dual(call()).tangent
+
+        yield tangent(lambda: ops.packed_attention(fwd.make_dual(q, way(q)), k, v, starts))
+        yield tangent(lambda: ops.packed_attention(q, fwd.make_dual(k, way(k)), v, starts))
+        yield tangent(lambda: ops.packed_attention(q, k, fwd.make_dual(v, way(v)), starts))
+        yield tangent(lambda: ops.cross_entropy(fwd.make_dual(x, way(x)), t))
+        leaf = v.detach().requires_grad_()
+        yield tangent(lambda: torch.autograd.grad(ops.packed_attention(q, k, leaf, starts), leaf,
+                                                  fwd.make_dual(dout, way(dout)))[0])
+        rows = x.detach().requires_grad_()
+        yield tangent(lambda: torch.autograd.grad(ops.cross_entropy(rows, t), rows,
+                                                  fwd.make_dual(x.new_ones(()), x.new_ones(())))[0])
+        p = torch.nn.Parameter(torch.zeros_like(x))
+        p.grad = fwd.make_dual(x, way(x))
+        yield tangent(lambda: ops.grad_norm([p]))
+
+
+def test_forward_mode_derivatives():
+    """On the host every op carries tangents."""
+    for call in _tangents("cpu"):
+        assert call() is not None
+
+
+@gpu
+def test_forward_mode_derivatives_refused_gpu():
+    """The kernels do not, and must not return an output that looks constant."""
+    for call in _tangents("cuda"):
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call()
