@@ -7,6 +7,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <cmath>
@@ -45,10 +46,13 @@ void launched(int code, const char* what) {
     TORCH_CHECK(code == 0, what, ": the launch failed with HIP error ", code);
 }
 
-// The kernels take a tensor's memory.  A tangent that it has beside it would be
-// lost without a word, and one that only stands for memory (a fake one, a wrapper,
-// freed storage) would lead them to address 0.
+// The kernels take a tensor's memory.  What it has beside that (a tangent, its
+// place in a trace that is recorded) would be lost without a word, and one that
+// only stands for memory (a fake one, a wrapper, freed storage) would lead them to
+// address 0.
 void plain(const Tensor& t, const char* name) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(),
+                                "the training ops cannot be recorded by torch.jit.trace");
     TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name,
                                 " has a forward-mode derivative, which the training ops do not "
                                 "have on the GPU");

@@ -4,8 +4,8 @@ On the GPU the kernels of csrc/packed_attn.hip, cross_entropy.hip and
 grad_norm.hip, whose autograd nodes are in csrc/training.cpp; on the CPU the
 references of reference.py. Arguments are checked here or, where all are on the
 GPU, by the same rules in training.cpp (a short call is mostly host time).
-On the GPU forward-mode derivatives are refused (NotImplementedError); the CPU's
-references have them.
+On the GPU forward-mode derivatives and torch.jit.trace are refused
+(NotImplementedError); the CPU's references have them.
 """
 from __future__ import annotations
 

@@ -1104,3 +1104,19 @@ def test_forward_mode_derivatives_refused_gpu():
     for call in _tangents("cuda"):
         with pytest.raises(NotImplementedError, match="forward-mode"):
             call()
+
+
+@gpu
+def test_trace_refused_gpu():
+    """A recorded trace would hold the output's allocation and no kernel."""
+    q, k, v, _ = _inputs([9], (4, 2), 64, device="cuda")
+    starts = torch.tensor([0, 9], device="cuda")
+    x, t = _loss_inputs(4, 9, torch.float32, "cuda")
+    for call, args in ((lambda q: ops.packed_attention(q, k, v, starts), (q,)),
+                       (lambda x: ops.cross_entropy(x, t), (x,))):
+        with pytest.raises(NotImplementedError, match="trace"):
+            torch.jit.trace(call, args, check_trace=False)
+    for call in (lambda: torch.func.grad(lambda q: ops.packed_attention(q, k, v, starts).sum())(q),
+                 lambda: torch.func.vmap(lambda x: ops.cross_entropy(x, t))(x[None])):
+        with pytest.raises((RuntimeError, ValueError)):   # wrappers without memory
+            call()
