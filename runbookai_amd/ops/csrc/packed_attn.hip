@@ -304,9 +304,10 @@ DEVINL void store_row(const f32x16_t (&acc)[D / 32], float factor, ushort_t* row
 // most keys first, `by_key` those with the most queries, so that the longest
 // run first and the short ones fill the gaps; entries that are left over hold
 // no rows.  One workgroup, a wave a sequence and a lane a tile: a pass that
-// counts tiles by their number in the sequence, a scan (with `pairs`, how often
-// a tile of queries meets one of keys), a pass that places them.  (The order
-// within one count is free and changes no result.)
+// counts tiles by their number in the sequence (with `pairs`, how often a tile of
+// queries meets one of keys: those of rows in no sequence meet none), a scan, a
+// pass that places them.  (The order within one count is free and changes no
+// result.)
 #define BUCKETS 4096
 #define BUILDERS 1024
 
@@ -316,11 +317,13 @@ packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
                     float* __restrict__ pairs) {
     __shared__ int first[BUCKETS], fill_q[BUCKETS], fill_k[BUCKETS];
     __shared__ int total;
+    __shared__ unsigned long long meet;   // whole, as its order is free
     const int tid = threadIdx.x;
     int shift = 0;
     while (((T / ROWS) >> shift) >= BUCKETS) ++shift;
     const int used = ((T / ROWS) >> shift) + 1;
     for (int i = tid; i < used; i += BUILDERS) first[i] = fill_q[i] = fill_k[i] = 0;
+    if (tid == 0) meet = 0;
     // sequence 0 is the rows before the first one, B + 1 those behind the last;
     // a wave's lanes load 64 ranges at once, so that the loads overlap
     const int lane = tid & (WAVE - 1), wid = tid / WAVE;
@@ -354,12 +357,15 @@ packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
             }
         }
     };
-    each([&](int, int, int, int, int i) { atomicAdd(&first[i >> shift], 1); });
+    each([&](int b, int, int, int n, int i) {
+        atomicAdd(&first[i >> shift], 1);
+        if (i == 0 && !wrong && b > 0 && b <= B)
+            atomicAdd(&meet, (unsigned long long)n * (n + 1) / 2);
+    });
     __syncthreads();
     // first[k] = number of tiles in buckets above k
     if (tid < WAVE) {
         int above = 0;
-        float meet = 0.f;
         for (int top = used - 1; top >= 0; top -= WAVE) {
             const int k = top - tid;
             const int n = k >= 0 ? first[k] : 0;
@@ -370,14 +376,11 @@ packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
                 if (tid >= off) sum += v;
             }
             if (k >= 0) first[k] = above + sum - n;
-            meet += (float)n * (float)((k << shift) + 1);
             above += __shfl(sum, WAVE - 1, WAVE);
         }
-#pragma unroll
-        for (int off = 1; off < WAVE; off <<= 1) meet += __shfl_xor(meet, off, WAVE);
         if (tid == 0) {
             total = above;
-            *pairs = meet;
+            *pairs = (float)meet;
         }
     }
     __syncthreads();
@@ -422,7 +425,8 @@ DEVINL int4_t find_tile(const int* __restrict__ starts, int B, int T, int p, int
         e = b == 0 ? T : 0;
     }
     const int n = (e - s + ROWS - 1) / ROWS;
-    pairs = 0.5f * n * (n + 1.f);
+    const bool in = !wrong && b > 0 && b <= B;
+    pairs = in ? 0.5f * n * (n + 1.f) : 0.f;
 #pragma unroll
     for (int off = 1; off < WAVE; off <<= 1) pairs += __shfl_xor(pairs, off, WAVE);
     const auto sum = [](int x, int y) { return x + y; };

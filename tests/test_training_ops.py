@@ -1120,3 +1120,30 @@ def test_trace_refused_gpu():
                  lambda: torch.func.vmap(lambda x: ops.cross_entropy(x, t))(x[None])):
         with pytest.raises((RuntimeError, ValueError)):   # wrappers without memory
             call()
+
+
+# ----------------------------------------------------------- how work is split
+
+@gpu
+@pytest.mark.parametrize("empty", [0, 62])   # tiles from a search, from a table
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_gpu_unused_rows_change_no_split(d, empty):
+    """Where dk and dv are summed by several workgroups the split shows in their
+    last bits: a sequence in a buffer of several times its length is split as
+    by itself. The buffer's length chooses a plan too; here it is the same one:
+    at most 7000 / 128 + 63 + 2 = 119 tiles, times 4 heads below the 512 up to
+    which two teams take a tile, times 2 heads (and 2 halves at d 64) below the
+    256 (768) up to which four parts do."""
+    heads = (4, 2)
+    n, T = 1500, 7000
+    q, k, v, dout = _inputs([n], heads, d, device="cuda")
+    starts = torch.tensor([0] * (empty + 1) + [n], dtype=torch.int32, device="cuda")
+    want = _attend(q, k, v, dout, starts)
+    for before in (0, 4000):
+        wide = [torch.zeros(T, *x.shape[1:], dtype=x.dtype, device="cuda")
+                for x in (q, k, v, dout)]
+        for x, y in zip(wide, (q, k, v, dout)):
+            x[before:before + n] = y
+        for x, y in zip(_attend(*wide, starts + before), want):
+            assert torch.equal(x[before:before + n], y)
+            assert not x[:before].any() and not x[before + n:].any()
