@@ -28,12 +28,15 @@ struct PackedArgs {
     float* delta;   // negated
     unsigned short *dq, *dk, *dv;
     // in how many parts the queries may be taken for dk and dv and, where that is
-    // more than one, the parts' sums and how many are there for each workgroup's keys
+    // more than one, the parts' sums (dk and dv in fp32, each) and how many are there
+    // for each workgroup's keys
     int parts, counters;
     float* sums;
     int* counts;
 };
 
-// The kernel for dk and dv: keys a workgroup, and workgroups that run at once.
+// The kernel for dk and dv: keys a workgroup (and queries a step), workgroups that
+// run at once, and steps that a workgroup must have over its share to be split.
 constexpr int packed_keys(int D) { return D == 128 ? 128 : 64; }
 constexpr int packed_slots(int D) { return D == 128 ? 256 : 3 * 256; }
+constexpr int packed_worth(int D) { return D == 128 ? 8 : 16; }

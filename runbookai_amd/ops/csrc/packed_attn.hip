@@ -886,14 +886,18 @@ packed_attn_dq_kernel(const PackedArgs a) {
 // 64 queries keep two tiles on their way.  4096 + 2500 + 1000 + 596 rows, 32/8
 // heads of 128: 0.46 ms, 0.87 PFLOP/s (0.51 unsplit); 32768 rows of the policy:
 // 102 us, 0.71 PFLOP/s.
-template <int D, int KS, int QB, int NBUF>
+//
+// WHOLE: no workgroup is split that lacks some of its keys.  More than WORTH steps
+// are more than WORTH / group turns of QB queries, so with groups of up to 8 heads
+// at least the tile's 128 rows lie between its first key and the sequence's end.
+template <int D, int KS, int QB, int NBUF, bool WHOLE>
 __global__ void __launch_bounds__(KS * 128, D == 128 ? 2 : 3)
 packed_attn_dkv_kernel(const PackedArgs a) {
     const int T = a.T, Hq = a.Hq, Hk = a.Hk;
     const int4_t* tiles = (const int4_t*)a.tiles + a.max_tiles;
     const float pairs = *(const float*)(tiles + a.max_tiles);
     static_assert(QB == KS * 32 && QB == packed_keys(D), "as many queries as keys");
-    constexpr int TEAMS = 2, BITS = 4 / KS, SLOTS = packed_slots(D), WORTH = D == 128 ? 8 : 16;
+    constexpr int TEAMS = 2, BITS = 4 / KS, SLOTS = packed_slots(D), WORTH = packed_worth(D);
     const int hk = blockIdx.x % Hk;
     const int group = Hq / Hk;
     // first the last parts, which few tiles have, and those few the first ones
@@ -1077,19 +1081,29 @@ packed_attn_dkv_kernel(const PackedArgs a) {
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) av[db] = ak[db];
     if (parts > 1) {
-        // The last workgroup of the parts adds them all, in their order.
+        // The last workgroup of the parts adds them all, in their order.  A part's
+        // sums are laid out by the rows of dk and dv that they are for, a wave's rows
+        // one after the other element by element: no more memory than those rows.
         union Two { float f[2]; unsigned long u; };
         const long slot = (long)bit * Hk + hk;
-        auto sums = [&](int part) {
-            return reinterpret_cast<unsigned long*>(
-                       a.sums + (((slot * a.parts + part) * 2 + team) * KS + wid % KS) * (32 * D)) +
-                   lane;
-        };
-        unsigned long* const to = sums(part);
+        // (Where the rows are known the offsets are constants: 8/4 heads of 64, 1023
+        // rows and some short sequences, 19.0 us; as variables 19.9.)
+        const int wave_rows =   // below 1 none is `mine`
+            WHOLE ? 32 : __builtin_amdgcn_readfirstlane(min(32, row1 - wkey));
+        // use(pair i, where it is)
+        auto sums = [&](int part, auto use) {
+            unsigned long* const at =
+                reinterpret_cast<unsigned long*>(
+                    a.sums + ((((long)part * Hk + hk) * 2 + team) * T + wkey) * D) +
+                hi * wave_rows + (lane & 31);
+            if (WHOLE || mine)
 #pragma unroll
-        for (int i = 0; i < D / 4; ++i)
-            __hip_atomic_store(to + i * 64, Two{{av[i / 8][i % 8 * 2], av[i / 8][i % 8 * 2 + 1]}}.u,
+                for (int i = 0; i < D / 4; ++i) use(i, at + i * 2 * wave_rows);
+        };
+        sums(part, [&](int i, unsigned long* at) {
+            __hip_atomic_store(at, Two{{av[i / 8][i % 8 * 2], av[i / 8][i % 8 * 2 + 1]}}.u,
                                __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        });
         arrived();
         __syncthreads();
         int& before = reinterpret_cast<int*>(lds.x)[0];
@@ -1100,16 +1114,13 @@ packed_attn_dkv_kernel(const PackedArgs a) {
         if (before != parts - 1) return;
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) av[db] = zero16();
-        for (int p = 0; p < parts; ++p) {
-            unsigned long* const from = sums(p);
-#pragma unroll
-            for (int i = 0; i < D / 4; ++i) {
+        for (int p = 0; p < parts; ++p)
+            sums(p, [&](int i, unsigned long* at) {
                 Two v;
-                v.u = __hip_atomic_load(from + i * 64, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                v.u = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 av[i / 8][i % 8 * 2] += v.f[0];
                 av[i / 8][i % 8 * 2 + 1] += v.f[1];
-            }
-        }
+            });
     }
     const long to = ((long)key * Hk + hk) * D;
     const float factor = seq1 < 0 ? NAN : team ? a.scale : 1.f;
@@ -1151,9 +1162,11 @@ void dq_(const PackedArgs* a, hipStream_t st) {
 
 template <int D, int KS, int QB, int NBUF>
 void dkv(const PackedArgs* a, hipStream_t st) {
-    hipLaunchKernelGGL((packed_attn_dkv_kernel<D, KS, QB, NBUF>),
-                       dim3((unsigned)a->max_tiles * a->Hk * (4 / KS) * a->parts), dim3(KS * 128),
-                       0, st, *a);
+    static_assert(packed_worth(D) / 8 * QB >= ROWS, "WHOLE with up to 8 heads a group");
+    const dim3 grid((unsigned)a->max_tiles * a->Hk * (4 / KS) * a->parts), block(KS * 128);
+    if (a->Hq / a->Hk <= 8)
+        hipLaunchKernelGGL((packed_attn_dkv_kernel<D, KS, QB, NBUF, true>), grid, block, 0, st, *a);
+    else hipLaunchKernelGGL((packed_attn_dkv_kernel<D, KS, QB, NBUF, false>), grid, block, 0, st, *a);
 }
 
 // Whether the usual split leaves CUs with a workgroup or two less than fit: then

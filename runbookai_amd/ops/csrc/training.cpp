@@ -148,9 +148,10 @@ void plan_tiles(PackedArgs& a, long B) {
 }
 
 // In how many parts the kernel for dk and dv may take a workgroup's queries.  It
-// splits only what is longer than the card's share; but workgroups of parts that
-// are not there cost a little, and their sums need memory.  dq and dk/dv with 1, 2
-// and 4 parts at most (us), by workgroups:
+// splits only what is longer than the card's share, so nothing where all rows
+// together are not; workgroups of parts that are not there cost a little, and each
+// part's sums are a copy of dk and dv in fp32.  dq and dk/dv with 1, 2 and 4 parts at
+// most (us), by workgroups:
 //   32/8 heads of 128 (256 run at once)      8/4 heads of 64 (768)
 //     88  1024             143 102  84         88  1024            51  41  39
 //    152  2048             290 203 197        280  4096           175 139 118
@@ -161,7 +162,8 @@ void plan_tiles(PackedArgs& a, long B) {
 void plan_parts(PackedArgs& a, bool keys) {
     const long slots = packed_slots(a.D);
     const long all = (long)a.max_tiles * a.Hk * (PACKED_ROWS / packed_keys(a.D));
-    a.parts = !keys || all > 3 * slots ? 1 : all > slots ? 2 : 4;
+    const long steps = ((a.T - 1) / packed_keys(a.D) + 1) * (long)(a.Hq / a.Hk);
+    a.parts = !keys || steps <= packed_worth(a.D) || all > 3 * slots ? 1 : all > slots ? 2 : 4;
     a.counters = a.parts > 1 ? (int)all : 0;
 }
 
@@ -229,8 +231,7 @@ std::vector<Tensor> packed_attn_bwd(const Tensor& dout, const Tensor& q, const T
         const size_t delta = parts.add(4 * (size_t)a.Hq * a.T);
         plan_parts(a, keys);
         const size_t counts = parts.add(a.parts > 1 ? 4 * (size_t)a.counters : 0);
-        const size_t sums = parts.add(a.parts > 1 ? 8 * (size_t)a.counters * a.parts *
-                                                        packed_keys(a.D) * a.D : 0);
+        const size_t sums = parts.add(a.parts > 1 ? 8 * (size_t)a.parts * a.Hk * a.T * a.D : 0);
         const Tensor scratch = parts.make(q);
         const Kept at(a, true);
         a.tiles = part<void>(kept, at.tiles);

@@ -1147,3 +1147,28 @@ def test_attention_gpu_unused_rows_change_no_split(d, empty):
         for x, y in zip(_attend(*wide, starts + before), want):
             assert torch.equal(x[before:before + n], y)
             assert not x[:before].any() and not x[before + n:].any()
+
+
+@gpu
+@pytest.mark.parametrize("lens,heads,d,parts", [
+    ([37], (32, 8), 128, 0), ([1] * 93, (32, 8), 128, 0), ([12] * 58, (64, 8), 128, 2),
+    ([1] * 30, (64, 1), 64, 4), ([100, 7], (64, 2), 128, 4), ([1500, 40, 700], (8, 2), 128, 4)])
+def test_attention_gpu_scratch_goes_by_rows(lens, heads, d, parts):
+    """A backward pass takes what it returns, an fp32 number a row and head, and
+    an fp32 copy of dk and dv for each part (none where nothing can be long
+    enough for one), whatever the number of sequences."""
+    q, k, v, dout = _inputs(lens, heads, d, pad=5, device="cuda")
+    starts = torch.tensor(_starts(lens), dtype=torch.int32, device="cuda")
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = ops.packed_attention(*leaves, starts)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = torch.autograd.grad(out, leaves, dout)
+    took = torch.cuda.max_memory_allocated() - before
+    pair = k.numel() + v.numel()
+    most = 2 * (q.numel() + pair) + 4 * q.shape[0] * heads[0] + 4 * parts * pair
+    # and 4 bytes each of at most 3 * 768 counters, and every allocation's end
+    assert took <= most + 2 ** 16, (took, most)
+    want, tol = attention_oracle(q, k, v, dout, _starts(lens), 1.0 / math.sqrt(d))
+    _within(got, want[1:], tol[1:])
