@@ -545,12 +545,12 @@ std::vector<Tensor> grads_of(const std::vector<Tensor>& parameters) {
     std::vector<Tensor> grads;
     for (const Tensor& p : parameters)
         if (p.grad().defined()) grads.push_back(p.grad());
+    TORCH_CHECK_VALUE(!grads.empty(), "no parameter has a gradient");
     return grads;
 }
 
 Tensor grad_norm(const std::vector<Tensor>& parameters) {
     const std::vector<Tensor> grads = grads_of(parameters);
-    if (grads.empty()) return torch::zeros({});
     const at::NoGradGuard no_grad;
     const Grads g = collect(grads, false);
     const c10::cuda::CUDAGuard guard(grads[0].device());
@@ -564,7 +564,6 @@ Tensor grad_norm(const std::vector<Tensor>& parameters) {
 
 Tensor grad_clip(const std::vector<Tensor>& parameters, double limit, double eps) {
     const std::vector<Tensor> grads = grads_of(parameters);
-    if (grads.empty()) return torch::zeros({});
     const at::NoGradGuard no_grad;
     const Grads g = collect(grads, true);
     const c10::cuda::CUDAGuard guard(grads[0].device());

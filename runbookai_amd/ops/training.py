@@ -129,15 +129,27 @@ def _check_host(grads: list[torch.Tensor], write: bool = False) -> None:
         raise ValueError("two of the gradients share or interleave their memory")
 
 
+def _first(parameters: list[torch.Tensor]) -> Optional[torch.Tensor]:
+    """The first gradient, whose device decides where the call runs."""
+    return next((p.grad for p in parameters if p.grad is not None), None)
+
+
+def _none(parameters: list[torch.Tensor]) -> torch.Tensor:
+    """The norm where no parameter has a gradient."""
+    return torch.zeros((), device=parameters[0].device if parameters else None)
+
+
 def grad_norm(parameters) -> torch.Tensor:
-    """2-norm of all parameters' gradients together (fp32 scalar on their
-    device); parameters without a gradient are passed over."""
+    """2-norm of all parameters' gradients together (fp32 scalar on the
+    gradients' device, or the first parameter's if there are none); parameters
+    without a gradient are passed over, wherever they are."""
     parameters = _list(parameters)
-    if parameters and parameters[0].is_cuda:
+    first = _first(parameters)
+    if first is None:
+        return _none(parameters)
+    if first.is_cuda:
         return _get_ext().grad_norm(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]
-    if not grads:
-        return torch.zeros(())
     _check_host(grads)
     with torch.no_grad():
         return reference.grad_norm(grads)
@@ -146,8 +158,8 @@ def grad_norm(parameters) -> torch.Tensor:
 def clip_grad_norm_(parameters, max_norm: float,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scales all parameters' gradients in place by
-    min(1, max_norm / (norm + 1e-6)) and returns their norm before that (fp32
-    scalar on their device). Two gradients whose memory overlaps or interleaves
+    min(1, max_norm / (norm + 1e-6)) and returns their norm before that (as
+    grad_norm). Two gradients whose memory overlaps or interleaves
     (the same one twice, columns of one buffer) are refused.
 
     On the GPU: any mix of float32, bfloat16 and float16 gradients of any
@@ -164,11 +176,12 @@ def clip_grad_norm_(parameters, max_norm: float,
         if not torch.isfinite(norm):
             raise RuntimeError(f"the norm of the gradients is {float(norm)}; "
                                "they are left as they were")
-    if parameters and parameters[0].is_cuda:
+    first = _first(parameters)
+    if first is None:
+        return _none(parameters)
+    if first.is_cuda:
         return _get_ext().grad_clip(parameters, max_norm, _EPS)
     grads = [p.grad for p in parameters if p.grad is not None]
-    if not grads:
-        return torch.zeros(())
     _check_host(grads, write=True)
     with torch.no_grad():
         return reference.grad_clip(grads, max_norm, _EPS)

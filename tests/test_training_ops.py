@@ -1172,3 +1172,34 @@ def test_attention_gpu_scratch_goes_by_rows(lens, heads, d, parts):
     assert took <= most + 2 ** 16, (took, most)
     want, tol = attention_oracle(q, k, v, dout, _starts(lens), 1.0 / math.sqrt(d))
     _within(got, want[1:], tol[1:])
+
+
+# ------------------------------------------------- where a clipping call runs
+
+@gpu
+@pytest.mark.parametrize("frozen,device", [("cpu", "cuda"), ("cuda", "cpu"), ("cuda", "cuda")])
+def test_clip_gpu_frozen_parameters_decide_nothing(frozen, device, monkeypatch):
+    """Parameters without a gradient are passed over, the first one too: GPU
+    gradients go to the kernels, host gradients to the host's path."""
+    if device == "cuda":
+        monkeypatch.setattr(reference, "grad_norm", None)
+        monkeypatch.setattr(reference, "grad_clip", None)
+    shut = torch.nn.Parameter(torch.zeros(7, device=frozen), requires_grad=False)
+    params = _params([(500,), (3, 4)], MIXED[:1], device)
+    for order in ([shut] + params, params + [shut]):
+        assert ops.grad_norm(order).device.type == device
+        norm = float(torch.cat([p.grad.double().flatten() for p in params]).norm())
+        assert abs(float(ops.clip_grad_norm_(order, 0.25)) - norm) <= 2.0 ** -23 * norm
+        assert ops.clip_grad_norm_(order, 0.25, error_if_nonfinite=True).device.type == device
+        assert float(ops.grad_norm(order)) <= 0.25 * (1 + 2.0 ** -22)
+        for p in params:
+            p.grad.mul_(8.0)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_clip_without_gradients_stays_on_the_device(device):
+    params = [torch.nn.Parameter(torch.zeros(3, device=device)) for _ in range(2)]
+    for norm in (ops.grad_norm(params), ops.clip_grad_norm_(params, 1.0),
+                 ops.clip_grad_norm_(params, 1.0, error_if_nonfinite=True)):
+        assert norm.device.type == device and norm.dtype == torch.float32 and float(norm) == 0.0
+    assert float(ops.clip_grad_norm_([], 1.0)) == 0.0
