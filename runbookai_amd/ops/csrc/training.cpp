@@ -309,8 +309,9 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
     plain(v, "v");
     plain(starts0, "seq_starts");
     const double scale = scale0 ? *scale0 : 1.0 / std::sqrt((double)q.size(2));
-    TORCH_CHECK_VALUE(scale > 0.0 && scale < 0x1p127,
-                      "scale must be positive and an fp32 number, not ", scale);
+    // times log2(e) it is still an fp32 number; a 0 would make NaN of shut places' -inf
+    TORCH_CHECK_VALUE(scale >= 0x1p-126 && scale < 0x1p127,
+                      "scale must be positive and a normal fp32 number, not ", scale);
     const Tensor starts = starts32(starts0, q);
     if (torch::GradMode::is_enabled() &&
         (q.requires_grad() || k.requires_grad() || v.requires_grad()))

@@ -59,8 +59,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             or seq_starts.dtype not in (torch.int32, torch.int64)):
         raise ValueError("seq_starts must be a vector of whole numbers, one more than sequences")
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
-    if not 0.0 < scale < 2.0 ** 127:   # times log2(e) it is still an fp32 number
-        raise ValueError(f"scale must be positive and an fp32 number, not {scale}")
+    if not 2.0 ** -126 <= scale < 2.0 ** 127:   # times log2(e) it is still an fp32 number
+        raise ValueError(f"scale must be positive and a normal fp32 number, not {scale}")
     if not seq_starts.is_cuda:
         starts = seq_starts.tolist()
         if starts[0] < 0 or starts[-1] > q.shape[0] or starts != sorted(starts):

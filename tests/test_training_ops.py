@@ -1203,3 +1203,23 @@ def test_clip_without_gradients_stays_on_the_device(device):
                  ops.clip_grad_norm_(params, 1.0, error_if_nonfinite=True)):
         assert norm.device.type == device and norm.dtype == torch.float32 and float(norm) == 0.0
     assert float(ops.clip_grad_norm_([], 1.0)) == 0.0
+
+
+# ------------------------------------------------------------ scales at the end
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_attention_scales_at_the_ends(device):
+    """A scale that fp32 rounds to 0 (or to fewer bits) is refused; with the
+    smallest that it holds a row's probabilities are all alike, and its rows
+    are means of the values so far."""
+    q, k, v, dout = _inputs([40], (4, 2), 64, device=device)
+    starts = torch.tensor([0, 40], device=device)
+    for scale in (1e-46, 1e-300, 2.0 ** -149, 2.0 ** -127):
+        with pytest.raises(ValueError, match="scale"):
+            ops.packed_attention(q, k, v, starts, scale=scale)
+    for scale in (2.0 ** -126, 1e-30):
+        got = _attend(q, k, v, dout, starts, scale)
+        want, tol = attention_oracle(q, k, v, dout, [0, 40], scale)
+        # dq and dk are near the smallest numbers that bf16 holds, or below
+        _within([got[0], got[3]], [want[0], want[3]], [tol[0], tol[3]], ("out", "dv"))
+        assert all(torch.isfinite(x).all() for x in got)
