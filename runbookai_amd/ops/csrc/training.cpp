@@ -383,8 +383,8 @@ std::vector<Tensor> xent_fwd(const Tensor& x, const Tensor& targets, int64_t ign
     return {result, kept};
 }
 
-Tensor xent_bwd(const Tensor& gout, Tensor x, const Tensor& targets, int64_t ignore, int64_t mode,
-                const Tensor& kept) {
+Tensor xent_bwd(const Tensor& gout, const Tensor& x, const Tensor& targets, int64_t ignore,
+                int64_t mode, const Tensor& kept) {
     check_logits(x, targets);
     const int kind = kind_of(x, "logits");
     const int N = (int)x.size(0), V = (int)x.size(1);
@@ -394,13 +394,6 @@ Tensor xent_bwd(const Tensor& gout, Tensor x, const Tensor& targets, int64_t ign
                 "the gradient must be float32, one value or one a row");
     const c10::cuda::CUDAGuard guard(x.device());
     Tensor dx = torch::empty({N, V}, x.options());
-    // the kernel's vectors need the same distance to 16 bytes on both sides
-    const long size = x.element_size();
-    const auto off = [&](const Tensor& t) {
-        return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
-    };
-    if (!off(x) || (N > 1 && (x.stride(0) - V) * size % 16 != 0))
-        x = x.clone(at::MemoryFormat::Contiguous);
     const Losses at(N, N > 0 ? xent_parts(N, V) : 0, mode != 0, true);
     if (N > 0)
         launched(launch_xent_bwd(kind, x.data_ptr(), x.stride(0), targets.data_ptr(), ignore, N,

@@ -86,8 +86,9 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int
     row. A label outside the vocabulary makes its row's loss and gradient NaN.
     Logits of -inf (vocabulary shut off) have probability and gradient 0.
 
-    On the GPU: float32, bfloat16 or float16 logits, in rows of any distance
-    and alignment; the sums are fp32 and over rows fp64."""
+    On the GPU: float32, bfloat16 or float16 logits. Rows of any distance and
+    alignment are read in place (columns apart from each other are copied
+    first); the sums are fp32 and over rows fp64."""
     if reduction not in _MODES:
         raise ValueError(f"reduction must be one of {sorted(_MODES)}, not {reduction!r}")
     if logits.is_cuda:

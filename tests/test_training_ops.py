@@ -1223,3 +1223,28 @@ def test_attention_scales_at_the_ends(device):
         # dq and dk are near the smallest numbers that bf16 holds, or below
         _within([got[0], got[3]], [want[0], want[3]], [tol[0], tol[3]], ("out", "dv"))
         assert all(torch.isfinite(x).all() for x in got)
+
+
+# ------------------------------------------------------ logits that are views
+
+@gpu
+@pytest.mark.parametrize("dtype", MIXED)
+@pytest.mark.parametrize("n,width,cols", [
+    (256, 1009, slice(0, 1001)), (256, 1001, slice(1, None)), (200, 1003, slice(1, 1000)),
+    (24, 9003, slice(0, 9001)), (24, 9001, slice(3, None)), (300, 5, slice(1, 4))])
+def test_loss_gpu_views_are_not_copied(n, width, cols, dtype):
+    """Columns of a wider buffer, at every distance to a 16-byte boundary: the
+    backward pass takes its result's memory and no copy of the logits."""
+    wide, t = _loss_inputs(n + 1, width, dtype, "cuda")
+    x, t = wide[1:, cols], t[1:].clone()
+    t[t >= x.shape[1]] = 0
+    x = x.detach().requires_grad_()
+    loss = ops.cross_entropy(x, t)
+    one = torch.ones_like(loss)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    grad, = torch.autograd.grad(loss, x, one)
+    took = torch.cuda.max_memory_allocated() - before
+    assert took <= grad.numel() * grad.element_size() + 512
+    _check_loss((loss.detach(), grad), loss_oracle(x, t, "mean", one), dtype, one)
