@@ -35,8 +35,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     others are copied first. The starts stay on the device and nothing waits
     for the host, so forward and backward can be captured into a graph (by
     autograd.grad, or while no eager step's graph of the same leaves lives).
-    Starts on the host are checked; starts on the device cannot be without
-    waiting for them: where they fall or leave [0, T], every output and
+    Starts are checked where they or q are on the host; with all on the device
+    they cannot be without waiting for them: where they fall or leave [0, T], every output and
     gradient is NaN. A value that is not finite may reach any row of its own
     sequence (a shut place's product is 0 times the value), but no other's.
 
@@ -61,10 +61,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
     if not 2.0 ** -126 <= scale < 2.0 ** 127:   # times log2(e) it is still an fp32 number
         raise ValueError(f"scale must be positive and a normal fp32 number, not {scale}")
-    if not seq_starts.is_cuda:
-        starts = seq_starts.tolist()
-        if starts[0] < 0 or starts[-1] > q.shape[0] or starts != sorted(starts):
-            raise ValueError(f"seq_starts must rise within 0 and {q.shape[0]}")
+    starts = seq_starts.tolist()
+    if starts[0] < 0 or starts[-1] > q.shape[0] or starts != sorted(starts):
+        raise ValueError(f"seq_starts must rise within 0 and {q.shape[0]}")
     if not q.is_cuda:
         return reference.packed_attention(q, k, v, seq_starts, scale)
     return _get_ext().packed_attention(q, k, v, seq_starts.to(q.device), scale)

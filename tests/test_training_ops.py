@@ -1248,3 +1248,14 @@ def test_loss_gpu_views_are_not_copied(n, width, cols, dtype):
     took = torch.cuda.max_memory_allocated() - before
     assert took <= grad.numel() * grad.element_size() + 512
     _check_loss((loss.detach(), grad), loss_oracle(x, t, "mean", one), dtype, one)
+
+
+@gpu
+@pytest.mark.parametrize("starts", [[0, 5], [-1, 4], [0, 3, 2, 4]])
+def test_attention_on_the_host_checks_starts_of_the_gpu(starts):
+    q, k, v, _ = _inputs([4], (4, 2), 64)
+    with pytest.raises(ValueError):
+        ops.packed_attention(q, k, v, torch.tensor(starts, device="cuda"))
+    fine = torch.tensor([0, 3, 4])
+    assert torch.equal(ops.packed_attention(q, k, v, fine.cuda()),
+                       ops.packed_attention(q, k, v, fine))
