@@ -53,8 +53,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
         raise ValueError(f"{q.shape[1]} query heads are no multiple of "
                          f"{k.shape[1]} key/value heads")
-    if not (q.dtype == k.dtype == v.dtype) or not (q.device == k.device == v.device):
-        raise ValueError("q, k and v must have one type and device")
+    if (not (q.dtype == k.dtype == v.dtype) or not (q.device == k.device == v.device)
+            or not q.dtype.is_floating_point):
+        raise ValueError("q, k and v must have one floating-point type and one device")
     if (seq_starts.dim() != 1 or seq_starts.numel() < 1
             or seq_starts.dtype not in (torch.int32, torch.int64)):
         raise ValueError("seq_starts must be a vector of whole numbers, one more than sequences")
@@ -97,6 +98,8 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int
                          f"{tuple(logits.shape)}, targets {tuple(targets.shape)}")
     if targets.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"targets must be whole numbers, not {targets.dtype}")
+    if not logits.dtype.is_floating_point:
+        raise ValueError(f"logits must be floating-point numbers, not {logits.dtype}")
     if targets.device != logits.device:
         raise ValueError("logits and targets must be on one device")
     return reference.cross_entropy(logits, targets.long(), ignore_index, reduction)

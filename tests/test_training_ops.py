@@ -1259,3 +1259,16 @@ def test_attention_on_the_host_checks_starts_of_the_gpu(starts):
     fine = torch.tensor([0, 3, 4])
     assert torch.equal(ops.packed_attention(q, k, v, fine.cuda()),
                        ops.packed_attention(q, k, v, fine))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.complex64])
+def test_ops_refuse_other_numbers(dtype, device):
+    """A probability is no whole number."""
+    q, k, v, _ = _inputs([4], (4, 2), 64, device=device)
+    starts = torch.tensor([0, 4], device=device)
+    with pytest.raises(ValueError):
+        ops.packed_attention(q.to(dtype), k.to(dtype), v.to(dtype), starts)
+    x, t = _loss_inputs(4, 9, torch.float32, device)
+    with pytest.raises(ValueError):
+        ops.cross_entropy(x.to(dtype), t)
