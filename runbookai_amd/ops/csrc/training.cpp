@@ -140,8 +140,11 @@ PackedArgs packed_args(const Tensor& q, const Tensor& k, const Tensor& v, double
 // for them: that makes it 2 us longer, where the table is a launch of 4 to 5.
 void plan_tiles(PackedArgs& a, long B) {
     const long most = a.T / PACKED_ROWS + B + 2;
-    // a launch's threads are counted in 32 bits
-    TORCH_CHECK(most * a.Hq * 512 < (1L << 32), "too many rows and sequences for one call");
+    // a launch's threads are counted in 32 bits; tiles are rounded up to the XCDs that
+    // share a kv head
+    const long share = 8 % a.Hk ? 1 : 8 / a.Hk;
+    TORCH_CHECK((2 * most + share - 1) / share * share * a.Hq * 256 < (1L << 32),
+                "too many rows, sequences and heads for one call");
     a.B = (int)B;
     a.max_tiles = (int)most;
     a.search = B <= PACKED_FEW;

@@ -1272,3 +1272,16 @@ def test_ops_refuse_other_numbers(dtype, device):
     x, t = _loss_inputs(4, 9, torch.float32, device)
     with pytest.raises(ValueError):
         ops.cross_entropy(x.to(dtype), t)
+
+
+@gpu
+def test_attention_gpu_refuses_more_heads_than_one_grid_counts():
+    """3 tiles are rounded up to the 8 XCDs that share a kv head: with 2.7
+    million query heads that is more than 2^32 threads."""
+    x = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    q = x.expand(1, 2_700_000, 64)
+    starts = torch.tensor([0, 1], device="cuda")
+    with pytest.raises(RuntimeError, match="too many rows, sequences and heads"):
+        ops.packed_attention(q, x, x, starts)
+    got = ops.packed_attention(q[:, :100_000], x + 1, x + 1, starts)
+    assert (got == 1).all()
