@@ -874,8 +874,14 @@ packed_attn_dq_kernel(const PackedArgs a) {
 // sums in their order, so the same inputs give the same bits, and nobody waits.
 // Sums and count go past the caches (relaxed atomics of agent scope): a fence
 // would write back and drop an XCD's whole L2, which made everything slower (1.06
-// ms instead of 0.81).  The parts are the outer order of the grid, as the many
-// that are not there would else leave every other CU idle.
+// ms instead of 0.81).  So the order of sums before count rests on the hardware, not
+// on the language's memory model: s_waitcnt vmcnt(0) ends when every write-through
+// store of the wave has reached memory, all waves wait for that and meet at the
+// barrier, and only then one thread counts.  What keeps the compiler from moving the
+// stores past that wait is that it is volatile asm with a memory clobber; on the
+// other side the loads stand behind the barrier that follows the count.  The parts
+// are the outer order of the grid, as the many that are not there would else leave
+// every other CU idle.
 //
 // 32 MFMA a block of 32 x 32 at D 128, and as many 1 KB fragments from LDS, each
 // read for one product.  LDS is busy a quarter of the time and the matrix cores
