@@ -1285,3 +1285,35 @@ def test_attention_gpu_refuses_more_heads_than_one_grid_counts():
         ops.packed_attention(q, x, x, starts)
     got = ops.packed_attention(q[:, :100_000], x + 1, x + 1, starts)
     assert (got == 1).all()
+
+
+# ------------------------------------------------------------- closer bounds
+
+@gpu
+@pytest.mark.parametrize("n,v", [(1, 1), (1, 777), (1, 9001), (3, 4099), (999, 33), (40_000, 9),
+                                 (300, 9001), (100_001, 2)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_loss_gpu_sums_of_rows_are_rounded_once(n, v, dtype):
+    """The rows' losses, each as a loss of its own, added in 64 bits: a sum and
+    a mean are within half a step of fp32 (and what 64 bits round)."""
+    x, t = _loss_inputs(n, v, dtype, "cuda", labelled=0.9)
+    rows = ops.cross_entropy(x, t, reduction="none").double().cpu()
+    want = loss_oracle(x, t, "none", torch.ones(n))[0]
+    # exp of a product rounded once, summed, logarithm, two additions: as _check_loss
+    assert ((rows - want).abs() <= 2.0 ** -24 * (80 + want)).all()
+    for reduction, exact in (("sum", rows.sum()), ("mean", rows.sum() / (t != -100).sum().cpu())):
+        got = ops.cross_entropy(x, t, reduction=reduction).double().cpu()
+        assert (got - exact).abs() <= 2.0 ** -24 * (1 + 2.0 ** -20) * exact.abs()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_clip_leaves_gradients_whose_norm_is_not_finite(bad, device):
+    params = _params([(5,), (9000,)], MIXED[:1], device)
+    params[1].grad[77] = bad
+    before = [p.grad.clone() for p in params]
+    with pytest.raises(RuntimeError):
+        ops.clip_grad_norm_(params, 1.0, error_if_nonfinite=True)
+    for p, g in zip(params, before):
+        torch.testing.assert_close(p.grad, g, rtol=0, atol=0, equal_nan=True)
+    assert torch.isfinite(params[0].grad).all() and params[0].grad.any()
