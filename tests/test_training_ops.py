@@ -1317,3 +1317,66 @@ def test_clip_leaves_gradients_whose_norm_is_not_finite(bad, device):
     for p, g in zip(params, before):
         torch.testing.assert_close(p.grad, g, rtol=0, atol=0, equal_nan=True)
     assert torch.isfinite(params[0].grad).all() and params[0].grad.any()
+
+
+# ------------------------------------------------------------ every plan of dk, dv
+
+@gpu
+@pytest.mark.parametrize("lens,heads,d,parts", [
+    # in up to two parts, and split: more workgroups than run at once
+    ([0] * 25 + [1500], (32, 8), 128, 2), ([0] * 4 + [1500, 130], (64, 16), 128, 2),
+    ([0] * 50 + [1500], (16, 8), 64, 2), ([0] * 70 + [100, 1400], (16, 8), 64, 2),
+    # in one: more than three times as many
+    ([0] * 25 + [300, 1], (32, 32), 128, 1), ([0] * 32 + [500], (32, 32), 64, 1),
+    ([0] * 150 + [1100, 60], (32, 8), 64, 1), ([0] * 90 + [1100, 60], (32, 8), 128, 1)])
+def test_attention_gpu_plans_of_parts(lens, heads, d, parts):
+    """Which plan it is shows in the memory: a copy of dk and dv in fp32 a part,
+    where there are several."""
+    q, k, v, dout = _inputs(lens, heads, d, pad=5, device="cuda")
+    starts = torch.tensor(_starts(lens), dtype=torch.int32, device="cuda")
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = ops.packed_attention(*leaves, starts)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = torch.autograd.grad(out, leaves, dout)
+    took = torch.cuda.max_memory_allocated() - before
+    pair = k.numel() + v.numel()
+    rest = 2 * (q.numel() + pair) + 4 * q.shape[0] * heads[0]
+    # allocations end at 2 MiB at most behind what was asked for
+    copies = (took - rest) / (4 * pair)
+    assert round(copies) == (parts if parts > 1 else 0), copies
+    want, tol = attention_oracle(q, k, v, dout, _starts(lens), 1.0 / math.sqrt(d))
+    _within((out.detach(), *got), want, tol)
+    for _ in range(5):
+        for x, y in zip(_attend(q, k, v, dout, starts)[1:], got):
+            assert torch.equal(x, y)
+
+
+@gpu
+def test_attention_gpu_coarse_table():
+    """From 524288 rows on the table sorts tiles by two of their numbers at once:
+    the same bits as batches of a quarter each (which have the same plan: over
+    512 workgroups for out and dq, over 2304 for dk and dv), and some sequences
+    held to 64 bits."""
+    gen = torch.Generator().manual_seed(7)
+    quarters = []
+    for _ in range(4):
+        lens = torch.randint(0, 1500, (150,), generator=gen).tolist()
+        quarters.append(lens + [150_000 - sum(lens)])
+    d, heads = 64, (2, 1)
+    lens = sum(quarters, [])
+    q, k, v, dout = _inputs(lens, heads, d, device="cuda")
+    assert q.shape[0] == 600_000
+    starts = _starts(lens)
+    got = _attend(q, k, v, dout, torch.tensor(starts, dtype=torch.int32, device="cuda"))
+    for i, quarter in enumerate(quarters):
+        a, b = i * 150_000, (i + 1) * 150_000
+        part = _attend(q[a:b], k[a:b], v[a:b], dout[a:b],
+                       torch.tensor(_starts(quarter), dtype=torch.int32, device="cuda"))
+        assert all(torch.equal(x[a:b], y) for x, y in zip(got, part))
+    for i in (0, 1, 200, len(lens) - 3):
+        a, b = starts[i], starts[i + 1]
+        want, tol = attention_oracle(*(x[a:b] for x in (q, k, v, dout)), [0, b - a],
+                                     1.0 / math.sqrt(d))
+        _within([x[a:b] for x in got], want, tol)
