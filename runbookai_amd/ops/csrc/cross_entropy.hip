@@ -23,7 +23,17 @@
 
 #include <type_traits>
 
-#define XENT_SHORT 8192   // the longest row that a single wave takes
+// The longest row that a single wave takes; 16 take longer ones.  A step of 16 waves
+// is 64 KB of a row, which short rows leave mostly empty; one wave alone is slow where
+// the rows are few.  Loss / loss and gradient (us), one wave and 16, bf16 and fp32:
+//   65536 x 4096    97/314   458/982    188/607   445/902
+//   32768 x 8192    98/316   250/562    190/607   262/596
+//   16384 x 16384  100/314   147/351    196/626   176/588
+//   8388 x 32000   105/342   102/289    196/654   175/586
+//   2092 x 128256  106/388    96/316    206/724   183/622
+//   64 x 128256     35/ 93    12/ 61     56/149    13/ 61  (61 is the call's host time)
+// So fp32 changes sides here, and 16 bits, at twice as many columns a byte, would later.
+#define XENT_SHORT 8192
 
 namespace {
 
