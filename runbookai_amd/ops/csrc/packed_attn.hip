@@ -304,10 +304,9 @@ DEVINL void store_row(const f32x16_t (&acc)[D / 32], float factor, ushort_t* row
 // most keys first, `by_key` those with the most queries, so that the longest
 // run first and the short ones fill the gaps; entries that are left over hold
 // no rows.  One workgroup, a wave a sequence and a lane a tile: a pass that
-// counts tiles by their number in the sequence (with `pairs`, how often a tile of
-// queries meets one of keys: those of rows in no sequence meet none), a scan, a
-// pass that places them.  (The order within one count is free and changes no
-// result.)
+// counts tiles by their number in the sequence, a scan, a pass that places them.
+// (The order within one count is free and changes no result.)  Also `pairs`, how
+// often a tile of queries meets one of keys: those of rows in no sequence meet none.
 #define BUCKETS 4096
 #define BUILDERS 1024
 
@@ -336,12 +335,21 @@ packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
     int s0, e0;
     range(mine, s0, e0);   // all there are, up to 1022 sequences
     bool bad = s0 < 0 || e0 > T || e0 < s0;
+    const auto meetings = [&](int b, int s, int e) {
+        const unsigned long long n = ((unsigned)e - (unsigned)s + ROWS - 1) / ROWS;
+        return b > 0 && b <= B ? n * (n + 1) / 2 : 0;
+    };
+    unsigned long long own = meetings(mine, s0, e0);
     for (int b = mine + BUILDERS; b < B + 2; b += BUILDERS) {
         int s, e;
         range(b, s, e);
         bad |= s < 0 || e > T || e < s;
+        own += meetings(b, s, e);
     }
     const bool wrong = __syncthreads_or(bad);
+#pragma unroll
+    for (int off = 1; off < WAVE; off <<= 1) own += __shfl_xor(own, off, WAVE);
+    if (lane == 0 && !wrong) atomicAdd(&meet, own);
     auto each = [&](auto use) {
         for (int b0 = wid; b0 < B + 2; b0 += BUILDERS) {
             int s = s0, e = e0;
@@ -357,11 +365,7 @@ packed_tiles_kernel(const int* __restrict__ starts, int B, int T, int max_tiles,
             }
         }
     };
-    each([&](int b, int, int, int n, int i) {
-        atomicAdd(&first[i >> shift], 1);
-        if (i == 0 && !wrong && b > 0 && b <= B)
-            atomicAdd(&meet, (unsigned long long)n * (n + 1) / 2);
-    });
+    each([&](int, int, int, int, int i) { atomicAdd(&first[i >> shift], 1); });
     __syncthreads();
     // first[k] = number of tiles in buckets above k
     if (tid < WAVE) {
