@@ -487,15 +487,18 @@ DEVINL Place place_of(int i, int Hq, int Hk) {
 // chain of steps is what takes the time.
 //
 // Bound by the SIMDs: a wave's MFMA (16 a block of 32 keys at D 128, 15 ns each)
-// and the softmax's VALU work (3.4 ns an exp2, 1 ns an add) add up where other
-// waves' do not hide beneath them.  A wave keeps 32 rows because each fragment
+// and the softmax's VALU work (3.4 ns an exp2, 1 ns an add) hardly hide beneath each
+// other, other waves' neither.  By the counters, of all SIMDs' cycles: 8192 rows, D
+// 128: MFMA 56 %, VALU 42 %.  The policy's batch, D 64: MFMA 31 %, VALU 52 %, and
+// CUs are empty for 24 % of the time (starts, ends, short sequences' first loads;
+// also a tenth of its blocks are of waves whose rows lie past the sequence).  A wave keeps 32 rows because each fragment
 // of K and V from LDS then serves a product of 32 columns, and 128 registers of
 // accumulators and queries still leave two workgroups a CU.  Two of them overlap
 // each other's softmax and products better than one with longer tiles (two
 // blocks at a time in one wave: 631 against 590 us).  Without loads and barriers
 // 8192 rows still took 477 us of 558; the rest is these.  8192 rows, 32/8 heads of
-// 128: 0.53 ms, 1.04 PFLOP/s; 32768 rows in sequences of 64 to 1536, 8/4 heads
-// of 64: 57 us, 0.63 PFLOP/s.
+// 128: 0.49 to 0.55 ms by card and clock, 1.0 to 1.12 PFLOP/s; 32768 rows in sequences
+// of 64 to 1536, 8/4 heads of 64: 55 to 60 us, 0.6 to 0.65 PFLOP/s.
 template <int D, int TEAMS, bool SAVE>
 __global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
 packed_attn_fwd_kernel(const PackedArgs a) {
@@ -668,9 +671,10 @@ packed_attn_fwd_kernel(const PackedArgs a) {
 // ----------------------------------------------------------------------- dq
 //
 // The forward kernel's split.  Also writes -delta for the kernel below.  24 MFMA
-// a block of 32 keys at D 128 and less VALU work than forward (no maximum), so
-// the matrix cores bound it first.  4096 + 2500 + 1000 + 596 rows, 32/8 heads of
-// 128: 0.31 ms, 0.97 PFLOP/s; 32768 rows of the policy: 80 us, 0.68 PFLOP/s.
+// a block of 32 keys at D 128 and less VALU work than forward (no maximum): MFMA are
+// busy 54 % of the time and VALU 32 %, with D 64 35 and 49 %.  4096 + 2500 + 1000 + 596
+// rows, 32/8 heads of 128: 0.28 to 0.32 ms, 0.94 to 1.07 PFLOP/s; 32768 rows of the
+// policy: 76 to 85 us, 0.64 to 0.71 PFLOP/s.
 template <int D, int TEAMS>
 __global__ void __launch_bounds__(256, D == 128 ? 2 : 4)
 packed_attn_dq_kernel(const PackedArgs a) {
@@ -888,14 +892,14 @@ packed_attn_dq_kernel(const PackedArgs a) {
 // every other CU idle.
 //
 // 32 MFMA a block of 32 x 32 at D 128, and as many 1 KB fragments from LDS, each
-// read for one product.  LDS is busy a quarter of the time and the matrix cores
-// 37 %; VALU work (a quarter) overlaps with neither in full, and a wave has no
-// registers left to read far ahead (254; 64 keys a wave, which would halve the
+// read for one product.  LDS is busy 27 % of the time, the matrix cores 42 % and
+// VALU 27 %, none of which overlap in full, and a wave has no registers left to read
+// far ahead (256; 64 keys a wave, which would halve the
 // reads, spilled: 761 against 510 us).  At D 128 one workgroup of 8 waves has all
 // of LDS, so that a tile of 128 queries serves 128 keys; at D 64 three buffers of
 // 64 queries keep two tiles on their way.  4096 + 2500 + 1000 + 596 rows, 32/8
-// heads of 128: 0.46 ms, 0.87 PFLOP/s (0.51 unsplit); 32768 rows of the policy:
-// 102 us, 0.71 PFLOP/s.
+// heads of 128: 0.42 to 0.51 ms, 0.79 to 0.95 PFLOP/s (0.51 unsplit where that was
+// 0.46); 32768 rows of the policy: 97 to 106 us, 0.68 to 0.75 PFLOP/s.
 //
 // WHOLE: no workgroup is split that lacks some of its keys.  More than WORTH steps
 // are more than WORTH / group turns of QB queries, so with groups of up to 8 heads
