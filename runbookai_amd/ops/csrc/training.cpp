@@ -62,6 +62,14 @@ void plain(const Tensor& t, const char* name) {
                       name, " must be a plain tensor with memory of its own");
 }
 
+// Memory for a kernel to write.  Where a dispatch mode is on it may be none, though
+// all inputs are real.
+Tensor blank(at::IntArrayRef sizes, const torch::TensorOptions& options) {
+    const Tensor t = torch::empty(sizes, options);
+    plain(t, "a result");
+    return t;
+}
+
 // What a backward pass returns: without a gradient of its own, and with an
 // error where somebody asks for one (create_graph).
 std::vector<Tensor> once(std::vector<Tensor> grads, const char* what) {
@@ -83,7 +91,7 @@ struct Parts {
         return at;
     }
     Tensor make(const Tensor& like) const {
-        return torch::empty({(long)size}, like.options().dtype(torch::kUInt8));
+        return blank({(long)size}, like.options().dtype(torch::kUInt8));
     }
 };
 
@@ -106,6 +114,7 @@ Tensor rows16(const Tensor& t) {
 }
 
 void check_rows(const Tensor& t, const char* name, const Tensor& like) {
+    plain(t, name);
     TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device());
     TORCH_CHECK(t.scalar_type() == torch::kBFloat16, name, " must be bfloat16");
     TORCH_CHECK(t.dim() == 3, name, " must have 3 dimensions: tokens, heads, head dim");
@@ -187,11 +196,12 @@ struct Kept {
 std::vector<Tensor> packed_attn_fwd(const Tensor& q, const Tensor& k, const Tensor& v,
                                     const Tensor& starts, double scale, bool save) {
     PackedArgs a = packed_args(q, k, v, scale);
+    plain(starts, "seq_starts");
     TORCH_CHECK(starts.device() == q.device() && starts.scalar_type() == torch::kInt32 &&
                     starts.is_contiguous() && starts.dim() == 1 && starts.numel() >= 1,
                 "seq_starts must be a dense int32 vector on the device of q");
     const c10::cuda::CUDAGuard guard(q.device());
-    const Tensor out = torch::empty({a.T, a.Hq, a.D}, q.options());
+    const Tensor out = blank({a.T, a.Hq, a.D}, q.options());
     plan_tiles(a, starts.numel() - 1);
     const Kept at(a, save);
     Tensor kept;
@@ -218,16 +228,15 @@ std::vector<Tensor> packed_attn_bwd(const Tensor& dout, const Tensor& q, const T
                                     const Tensor& v, const Tensor& out, const Tensor& kept,
                                     long B, double scale, bool keys) {
     PackedArgs a = packed_args(q, k, v, scale);
-    plain(dout, "the gradient");
     check_rows(dout, "the gradient", q);
     TORCH_CHECK(dout.sizes() == q.sizes(), "the gradient must have the shape of q");
     const c10::cuda::CUDAGuard guard(q.device());
     const auto opt = q.options();
-    const Tensor dq = torch::empty({a.T, a.Hq, a.D}, opt);
+    const Tensor dq = blank({a.T, a.Hq, a.D}, opt);
     Tensor dk, dv;
     if (keys) {
-        dk = torch::empty({a.T, a.Hk, a.D}, opt);
-        dv = torch::empty({a.T, a.Hk, a.D}, opt);
+        dk = blank({a.T, a.Hk, a.D}, opt);
+        dv = blank({a.T, a.Hk, a.D}, opt);
     }
     if (a.T > 0) {
         plan_tiles(a, B);
@@ -335,6 +344,8 @@ int kind_of(const Tensor& t, const char* name) {
 }
 
 void check_logits(const Tensor& x, const Tensor& targets) {
+    plain(x, "logits");
+    plain(targets, "targets");
     TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.size(1) >= 1 &&
                     (x.size(1) == 1 || x.stride(1) == 1),
                 "logits must be [rows, vocabulary] on the GPU with dense rows");
@@ -368,7 +379,7 @@ std::vector<Tensor> xent_fwd(const Tensor& x, const Tensor& targets, int64_t ign
     const int N = (int)x.size(0), V = (int)x.size(1);
     const c10::cuda::CUDAGuard guard(x.device());
     const auto opt = x.options().dtype(torch::kFloat32);
-    const Tensor result = mode ? torch::empty({}, opt) : torch::empty({N}, opt);
+    const Tensor result = mode ? blank({}, opt) : blank({N}, opt);
     const int parts = N > 0 ? xent_parts(N, V) : 0;
     const Losses at(N, parts, mode != 0, save);
     Tensor kept;
@@ -397,7 +408,7 @@ Tensor xent_bwd(const Tensor& gout, const Tensor& x, const Tensor& targets, int6
                     (gout.dim() == 0 || (gout.dim() == 1 && gout.numel() == N)),
                 "the gradient must be float32, one value or one a row");
     const c10::cuda::CUDAGuard guard(x.device());
-    Tensor dx = torch::empty({N, V}, x.options());
+    Tensor dx = blank({N, V}, x.options());
     const Losses at(N, N > 0 ? xent_parts(N, V) : 0, mode != 0, true);
     if (N > 0)
         launched(launch_xent_bwd(kind, x.data_ptr(), x.stride(0), targets.data_ptr(), ignore, N,
@@ -489,6 +500,7 @@ Grads collect(const std::vector<Tensor>& grads, bool write) {
             TORCH_CHECK_VALUE(!write || apart(t),
                               "a gradient must not share memory between its elements");
             d = t.clone(at::MemoryFormat::Contiguous);
+            plain(d, "a gradient's copy");
             g.copied.push_back((long)i);
         }
         if (write) {
@@ -529,7 +541,7 @@ Grads collect(const std::vector<Tensor>& grads, bool write) {
 }
 
 Tensor sums_of(const Grads& g, const Tensor& like, void* st) {
-    Tensor sums = torch::empty({g.partial}, like.options().dtype(torch::kFloat64));
+    Tensor sums = blank({g.partial}, like.options().dtype(torch::kFloat64));
     int at = 0;
     for (size_t i = 0; i < g.tables.size(); ++i) {
         launched(launch_grad_sums(&g.tables[i], g.blocks[i], sums.data_ptr<double>() + at, st),
@@ -553,7 +565,7 @@ Tensor grad_norm(const std::vector<Tensor>& parameters) {
     const Grads g = collect(grads, false);
     const c10::cuda::CUDAGuard guard(grads[0].device());
     void* st = stream_of(grads[0]);
-    Tensor norm = torch::empty({}, grads[0].options().dtype(torch::kFloat32));
+    Tensor norm = blank({}, grads[0].options().dtype(torch::kFloat32));
     const Tensor sums = sums_of(g, norm, st);
     launched(launch_grad_norm(sums.data_ptr(), g.partial, norm.data_ptr(), st),
              "the gradient norm");
@@ -566,7 +578,7 @@ Tensor grad_clip(const std::vector<Tensor>& parameters, double limit, double eps
     const Grads g = collect(grads, true);
     const c10::cuda::CUDAGuard guard(grads[0].device());
     void* st = stream_of(grads[0]);
-    Tensor norm = torch::empty({}, grads[0].options().dtype(torch::kFloat32));
+    Tensor norm = blank({}, grads[0].options().dtype(torch::kFloat32));
     const Tensor sums = sums_of(g, norm, st);
     if (g.tables.empty())
         launched(launch_grad_norm(sums.data_ptr(), 0, norm.data_ptr(), st), "the gradient norm");

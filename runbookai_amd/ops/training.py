@@ -36,9 +36,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     for the host, so forward and backward can be captured into a graph (by
     autograd.grad, or while no eager step's graph of the same leaves lives).
     Starts are checked where they or q are on the host; with all on the device
-    they cannot be without waiting for them: where they fall or leave [0, T], every output and
-    gradient is NaN. A value that is not finite may reach any row of its own
-    sequence (a shut place's product is 0 times the value), but no other's.
+    they cannot be without waiting for them: where they fall or leave [0, T],
+    every output and gradient is NaN. A value that is not finite may reach any
+    row of its own sequence (a shut place's product is 0 times the value), but
+    no other's.
 
     The training counterpart of prefill_attention, which has no gradients."""
     if q.is_cuda and seq_starts.is_cuda:

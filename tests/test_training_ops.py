@@ -1064,6 +1064,34 @@ def test_ops_gpu_refuse_freed_memory():
             call()
 
 
+@gpu
+def test_ops_gpu_refuse_results_without_memory():
+    """Real inputs while a mode makes every new tensor a fake one."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    q, k, v, _ = _inputs([4], (4, 2), 64, device="cuda")
+    x, t = _loss_inputs(4, 9, torch.float32, "cuda")
+    p = torch.nn.Parameter(torch.zeros(5, device="cuda"))
+    p.grad = torch.ones(5, device="cuda")
+    rows = x.detach().requires_grad_()
+    loss = ops.cross_entropy(rows, t)
+    one = torch.ones_like(loss)
+    for kind in (torch.int32, torch.int64):
+        starts = torch.tensor([0, 4], dtype=kind, device="cuda")
+        leaf = q.detach().requires_grad_()
+        out = ops.packed_attention(leaf, k, v, starts)
+        with FakeTensorMode(allow_non_fake_inputs=True):
+            for call in (lambda: ops.packed_attention(q, k, v, starts),
+                         lambda: ops.packed_attention(leaf, k, v, starts),
+                         lambda: torch.autograd.grad(out, leaf, q, retain_graph=True),
+                         lambda: torch.autograd.grad(loss, rows, one, retain_graph=True),
+                         lambda: ops.cross_entropy(x, t), lambda: ops.grad_norm([p]),
+                         lambda: ops.clip_grad_norm_([p], 1.0)):
+                with pytest.raises(ValueError, match="plain tensor"):
+                    call()
+    assert (p.grad == 1).all()
+
+
 def _tangents(device):
     """Outputs' tangents for tangents of one input each, and of a gradient."""
     import torch.autograd.forward_ad as fwd
