@@ -32,7 +32,7 @@
 //   8388 x 32000   105/342   102/289    196/654   175/586
 //   2092 x 128256  106/388    96/316    206/724   183/622
 //   64 x 128256     35/ 93    12/ 61     56/149    13/ 61  (61 is the call's host time)
-// So fp32 changes sides here, and 16 bits, at twice as many columns a byte, would later.
+// So fp32 changes sides here; 16 bits, with twice the columns in a step, would later.
 #define XENT_SHORT 8192
 
 namespace {
