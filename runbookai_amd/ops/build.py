@@ -1,8 +1,8 @@
 """Build the gfx950 HIP extension IN-TREE.
 
-The built .so lands in runbookai_amd/ops/_build/ so it travels with the
-gpurun snapshot (a JIT cache under ~/.cache would not). hipcc
-cross-compiles for gfx950 without a GPU present.
+The built .so lands in runbookai_amd/ops/_build/, so that it goes where a copy
+of the tree goes (a JIT cache under ~/.cache would not). hipcc cross-compiles
+for gfx950 without a GPU present.
 """
 from __future__ import annotations
 
